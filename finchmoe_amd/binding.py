@@ -19,6 +19,39 @@ SCALE_BF16, SCALE_FP16 = 0, 1
 Q4_K, Q6_K = 12, 14
 ACCUMULATE, GUARD = 1, 2
 GATE, UP, DOWN = 0, 1, 2
+DTYPE_F32, DTYPE_BF16 = 0, 1
+GDN_L2NORM = 1
+MAX_SEQ = 256
+
+
+class GatedDeltaArgs(C.Structure):
+    """fm_gated_delta_args (see FinchHip.gated_delta_args)."""
+    _fields_ = ([(n, C.c_int32) for n in ("n_seq", "k_heads", "v_heads", "k_dim", "v_dim", "dtype", "flags")]
+                + [("scale", C.c_float)] + [(n, C.c_void_p) for n in ("d_q", "d_k", "d_v")]
+                + [(n, C.c_int64) for n in ("q_stride", "k_stride", "v_stride")]
+                + [("d_g", C.c_void_p), ("d_beta", C.c_void_p), ("seq_start", C.POINTER(C.c_int32)),
+                   ("d_state_in", C.POINTER(C.c_void_p)), ("d_state_out", C.POINTER(C.c_void_p)), ("d_out", C.c_void_p)])
+
+
+class KvCache(C.Structure):
+    """fm_kv_cache: device memory of the caller."""
+    _fields_ = ([(n, C.c_void_p) for n in ("d_k", "d_v", "d_k_scale", "d_v_scale")]
+                + [(n, C.c_int32) for n in ("n_pages", "page_tokens", "kv_heads", "head_dim")])
+
+
+class KvArgs(C.Structure):
+    """fm_kv_args (see FinchHip.kv_args)."""
+    _fields_ = [("cache", KvCache), ("n_seq", C.c_int32), ("dtype", C.c_int32), ("d_k", C.c_void_p), ("d_v", C.c_void_p),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("seq_start", C.POINTER(C.c_int32)),
+                ("d_len", C.c_void_p), ("d_pages", C.c_void_p), ("max_pages", C.c_int32)]
+
+
+class AttnArgs(C.Structure):
+    """fm_attn_args (see FinchHip.attn_args)."""
+    _fields_ = [("cache", KvCache), ("n_seq", C.c_int32), ("q_heads", C.c_int32), ("dtype", C.c_int32),
+                ("scale", C.c_float), ("d_q", C.c_void_p), ("q_stride", C.c_int64), ("seq_start", C.POINTER(C.c_int32)),
+                ("d_len", C.c_void_p), ("d_pages", C.c_void_p), ("max_pages", C.c_int32), ("max_len", C.c_int32),
+                ("d_out", C.c_void_p)]
 
 
 class FinchError(RuntimeError):
@@ -108,6 +141,14 @@ def load():
         "fm_embed_lookup_dev": (i, [vp, i, vp, i, vp]),
         "fm_matvec_prefill_batch_dev": (i, [vp, vp, i, vp, vp, i]),
         "fm_embed_lookup": (i, [vp, i, i, vp]),
+        "fm_gated_delta_dev": (i, [vp, vp]),
+        "fm_gated_delta_ws_bytes": (sz, [vp, vp]),
+        "fm_kv_append_dev": (i, [vp, vp]),
+        "fm_kv_read_dev": (i, [vp, vp]),
+        "fm_attn_dev": (i, [vp, vp]),
+        "fm_attn_ws_bytes": (sz, [vp, vp]),
+        "fm_logprobs_dev": (i, [vp, vp, i, i, C.c_int64, vp, i, vp, vp, vp, vp]),
+        "fm_logprobs_ws_bytes": (sz, [vp, i, i, i]),
     }
     for name, (res, args) in sig.items():
         f = getattr(L, name)
@@ -397,6 +438,88 @@ class FinchHip:
         self._chk(self.L.fm_gguf_matvec(self.h, _ptr(W), ggml_type, _ptr(x), _ptr(out), out_dim,
                                         in_dim))
         return out
+
+    # ---- token mixers: the *_args calls fill a descriptor once (pointers are integers, host arrays
+    # are kept by it), the *_dev calls submit it
+    @staticmethod
+    def _starts(seq_start, n_seq):
+        if seq_start is None:
+            return None
+        if len(seq_start) != n_seq + 1:
+            raise FinchError(ERR_ARG, "seq_start has %d entries for %d sequences" % (len(seq_start), n_seq))
+        return (C.c_int32 * (n_seq + 1))(*seq_start)
+
+    def gated_delta_args(self, n_seq, k_heads, v_heads, k_dim, v_dim, d_q, d_k, d_v, d_g, d_beta, d_state_out, d_out,
+                         d_state_in=None, seq_start=None, dtype=DTYPE_F32, l2norm=False, scale=1.0, stride=None,
+                         q_stride=None, k_stride=None, v_stride=None):
+        """Descriptor of gated_delta_dev.  stride: one row stride for q, k and v (they lie in one
+        buffer); without any stride the rows are contiguous.  d_state_in / d_state_out: a device
+        address per sequence."""
+        for states in (d_state_in, d_state_out):
+            if states is not None and len(states) != n_seq:
+                raise FinchError(ERR_ARG, "%d states for %d sequences" % (len(states), n_seq))
+        a = GatedDeltaArgs(n_seq=n_seq, k_heads=k_heads, v_heads=v_heads, k_dim=k_dim, v_dim=v_dim, dtype=dtype,
+                           flags=GDN_L2NORM if l2norm else 0, scale=scale, d_q=d_q, d_k=d_k, d_v=d_v,
+                           q_stride=q_stride or stride or k_heads * k_dim, k_stride=k_stride or stride or k_heads * k_dim,
+                           v_stride=v_stride or stride or v_heads * v_dim, d_g=d_g, d_beta=d_beta, d_out=d_out)
+        if seq_start is not None:
+            a.seq_start = self._starts(seq_start, n_seq)
+        if d_state_in is not None:
+            a.d_state_in = (C.c_void_p * n_seq)(*d_state_in)
+        if d_state_out is not None:
+            a.d_state_out = (C.c_void_p * n_seq)(*d_state_out)
+        return a
+
+    def gated_delta_dev(self, args):
+        self._chk(self.L.fm_gated_delta_dev(self.h, C.byref(args)))
+
+    def gated_delta_ws_bytes(self, args):
+        return self.L.fm_gated_delta_ws_bytes(self.h, C.byref(args))
+
+    @staticmethod
+    def kv_cache(d_k, d_v, d_k_scale, d_v_scale, n_pages, page_tokens, kv_heads, head_dim):
+        return KvCache(d_k=d_k, d_v=d_v, d_k_scale=d_k_scale, d_v_scale=d_v_scale, n_pages=n_pages,
+                       page_tokens=page_tokens, kv_heads=kv_heads, head_dim=head_dim)
+
+    def kv_args(self, cache, n_seq, d_k, d_v, d_len, d_pages, max_pages, k_stride=None, v_stride=None, seq_start=None,
+                dtype=DTYPE_F32):
+        """Descriptor of kv_append_dev and kv_read_dev."""
+        width = cache.kv_heads * cache.head_dim
+        a = KvArgs(cache=cache, n_seq=n_seq, dtype=dtype, d_k=d_k, d_v=d_v, k_stride=k_stride or width,
+                   v_stride=v_stride or width, d_len=d_len, d_pages=d_pages, max_pages=max_pages)
+        if seq_start is not None:
+            a.seq_start = self._starts(seq_start, n_seq)
+        return a
+
+    def kv_append_dev(self, args):
+        self._chk(self.L.fm_kv_append_dev(self.h, C.byref(args)))
+
+    def kv_read_dev(self, args):
+        self._chk(self.L.fm_kv_read_dev(self.h, C.byref(args)))
+
+    def attn_args(self, cache, n_seq, q_heads, d_q, d_len, d_pages, max_pages, max_len, d_out, scale, q_stride=None,
+                  seq_start=None, dtype=DTYPE_F32):
+        """Descriptor of attn_dev."""
+        a = AttnArgs(cache=cache, n_seq=n_seq, q_heads=q_heads, dtype=dtype, scale=scale, d_q=d_q,
+                     q_stride=q_stride or q_heads * cache.head_dim, d_len=d_len, d_pages=d_pages, max_pages=max_pages,
+                     max_len=max_len, d_out=d_out)
+        if seq_start is not None:
+            a.seq_start = self._starts(seq_start, n_seq)
+        return a
+
+    def attn_dev(self, args):
+        self._chk(self.L.fm_attn_dev(self.h, C.byref(args)))
+
+    def attn_ws_bytes(self, args):
+        return self.L.fm_attn_ws_bytes(self.h, C.byref(args))
+
+    def logprobs_dev(self, d_logits, rows, vocab, row_stride, d_tokens, top_n, d_logprob, d_entropy, d_top_ids,
+                     d_top_logprobs):
+        self._chk(self.L.fm_logprobs_dev(self.h, d_logits, rows, vocab, row_stride, d_tokens, top_n, d_logprob,
+                                         d_entropy, d_top_ids, d_top_logprobs))
+
+    def logprobs_ws_bytes(self, rows, vocab, top_n):
+        return self.L.fm_logprobs_ws_bytes(self.h, rows, vocab, top_n)
 
     # ---- dequant
     def dequant_expert(self, layer, expert, which):

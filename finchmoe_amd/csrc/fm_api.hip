@@ -13,6 +13,7 @@
 
 #include "fm_common.h"
 #include "fm_route.h"     // RouteArgs
+#include "fm_mix_index.h"
 
 // ---- launchers implemented in the kernel files ------------------------------
 extern "C" {
@@ -58,6 +59,14 @@ int fm_launch_widen_bf16(const uint16_t *d_src, float *d_dst, size_t n, hipStrea
 int fm_launch_layer_tail(const FmTailArgs *a, int bits, int scale_fp16, hipStream_t st);
 int fm_launch_route(const float *d_logits, int n, int K, const float *d_seg_score, int32_t *d_idx,
                     float *d_w, float *d_params, hipStream_t st);
+size_t fm_gdn_ws_bytes(const FmGdn *a, const int *start, int n_seq);
+int fm_launch_gdn(const FmGdn *a, int bf16, const int *start, int n_seq, const float *const *in,
+                  float *const *out, void *ws, int n_cu, hipStream_t st);
+int fm_launch_attn(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int bf16, void *ws, hipStream_t st);
+int fm_launch_kv(const FmKv *c, const FmKvRows *x, const FmSeqs *b, int D, int bf16, int read, hipStream_t st);
+size_t fm_logprob_ws(int rows, int vocab, int top_n);
+int fm_launch_logprob(const float *x, int rows, int vocab, int64_t stride, const int32_t *tokens, int top_n,
+                      float *logprob, float *entropy, int32_t *ids, float *top_lp, void *ws, hipStream_t st);
 }
 
 // ---- scratch of the entry point that allocates nothing (fm_moe_decode_step_noalloc_dev) ----
@@ -1644,6 +1653,98 @@ extern "C" int fm_gguf_matvec(fm_ctx *c, const void *W, int ggml_type, const flo
     if (rc) return fail(c, rc, "GGUF matvec launch failed");
     HIPCHK(c, hipMemcpyAsync(out, st + off_o, (size_t)out_dim * 4, hipMemcpyDeviceToHost, c->stream));
     HIPCHK(c, hipStreamSynchronize(c->stream));
+    return FM_OK;
+}
+
+// ============================================================================
+// token mixers
+// ============================================================================
+
+// (operands are checked by the functions of fm_mix_index.h)
+extern "C" size_t fm_gated_delta_ws_bytes(fm_ctx *c, const fm_gated_delta_args *p) {
+    FmGdn a;
+    FmWhy w;
+    if (!c || fm_gdn_check(&w, p, &a)) return 0;
+    return fm_gdn_ws_bytes(&a, p->seq_start, p->n_seq);
+}
+
+extern "C" int fm_gated_delta_dev(fm_ctx *c, const fm_gated_delta_args *p) {
+    if (!c) return FM_ERR_ARG;
+    FmGdn a;
+    FmWhy w;
+    int rc = fm_gdn_check(&w, p, &a);
+    if (rc) return fail(c, rc, "%s", w.text);
+    DeviceGuard dg(c->device);
+    const size_t ws = fm_gdn_ws_bytes(&a, p->seq_start, p->n_seq);
+    if (ws && (rc = ensure_ws(c, ws))) return rc;
+    rc = fm_launch_gdn(&a, p->dtype == FM_DTYPE_BF16, p->seq_start, p->n_seq, p->d_state_in, p->d_state_out, c->d_ws,
+                       c->n_cu, c->stream);
+    if (rc) return fail(c, rc, "gated delta launch failed: %s", hipGetErrorString(hipGetLastError()));
+    return FM_OK;
+}
+
+static int kv_rows(fm_ctx *c, const fm_kv_args *p, int read) {
+    if (!c) return FM_ERR_ARG;
+    FmKv k;
+    FmKvRows x;
+    FmSeqs b;
+    FmWhy w;
+    int rc = fm_kv_rows_check(&w, p, read, &k, &x, &b);
+    if (rc) return fail(c, rc, "%s", w.text);
+    DeviceGuard dg(c->device);
+    rc = fm_launch_kv(&k, &x, &b, p->cache.head_dim, p->dtype == FM_DTYPE_BF16, read, c->stream);
+    if (rc) return fail(c, rc, "cache launch failed: %s", hipGetErrorString(hipGetLastError()));
+    return FM_OK;
+}
+extern "C" int fm_kv_append_dev(fm_ctx *c, const fm_kv_args *p) { return kv_rows(c, p, 0); }
+extern "C" int fm_kv_read_dev(fm_ctx *c, const fm_kv_args *p) { return kv_rows(c, p, 1); }
+
+extern "C" size_t fm_attn_ws_bytes(fm_ctx *c, const fm_attn_args *p) {
+    FmKv k;
+    FmAttn a;
+    FmSeqs b;
+    FmWhy w;
+    size_t ws = 0;
+    return c && !fm_attn_check(&w, p, c->n_cu, &k, &a, &b, &ws) ? ws : 0;
+}
+
+extern "C" int fm_attn_dev(fm_ctx *c, const fm_attn_args *p) {
+    if (!c) return FM_ERR_ARG;
+    FmKv k;
+    FmAttn a;
+    FmSeqs b;
+    FmWhy w;
+    size_t ws = 0;
+    int rc = fm_attn_check(&w, p, c->n_cu, &k, &a, &b, &ws);
+    if (rc) return fail(c, rc, "%s", w.text);
+    DeviceGuard dg(c->device);
+    if (ws && (rc = ensure_ws(c, ws))) return rc;
+    rc = fm_launch_attn(&k, &a, &b, p->cache.head_dim, p->dtype == FM_DTYPE_BF16, c->d_ws, c->stream);
+    if (rc) return fail(c, rc, "attention launch failed: %s", hipGetErrorString(hipGetLastError()));
+    return FM_OK;
+}
+
+// ============================================================================
+// log probabilities
+// ============================================================================
+extern "C" size_t fm_logprobs_ws_bytes(fm_ctx *c, int rows, int vocab, int top_n) {
+    FmWhy w;
+    return c && !fm_logprob_check(&w, rows, vocab, top_n) ? fm_logprob_ws(rows, vocab, top_n) : 0;
+}
+
+extern "C" int fm_logprobs_dev(fm_ctx *c, const float *d_logits, int rows, int vocab, int64_t row_stride,
+                               const int32_t *d_tokens, int top_n, float *d_logprob, float *d_entropy,
+                               int32_t *d_top_ids, float *d_top_logprobs) {
+    if (!c) return FM_ERR_ARG;
+    FmWhy w;
+    int rc = fm_logprob_args_check(&w, d_logits, rows, vocab, row_stride, d_tokens, top_n, d_logprob, d_entropy, d_top_ids,
+                                   d_top_logprobs);
+    if (rc) return fail(c, rc, "%s", w.text);
+    DeviceGuard dg(c->device);
+    if ((rc = ensure_ws(c, fm_logprob_ws(rows, vocab, top_n)))) return rc;
+    rc = fm_launch_logprob(d_logits, rows, vocab, row_stride, d_tokens, top_n, d_logprob, d_entropy, d_top_ids,
+                           d_top_logprobs, c->d_ws, c->stream);
+    if (rc) return fail(c, rc, "log probability launch failed: %s", hipGetErrorString(hipGetLastError()));
     return FM_OK;
 }
 

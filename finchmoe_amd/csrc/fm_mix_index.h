@@ -1,0 +1,332 @@
+// fm_mix_index.h — operands of the token mixers' launches (fm_gdn.hip, fm_attn.hip), the checks
+// their entry points make and the index arithmetic of the paged cache, in code that compiles into
+// the library, into the kernels and into a plain host program: tests/host_mix/ runs the checks on every
+// refusal and walks the cache's addresses without a GPU.
+#pragma once
+
+#include <stdarg.h>
+#include <stdint.h>
+#include <stdio.h>
+#include <string.h>
+
+#include <algorithm>
+#include <utility>
+
+#include "../../include/finch_hip.h"
+#include "fm_index.h"
+
+// rows of one call of a token mixer or of the log probabilities (grid dimensions)
+#define FM_MAX_ROWS 65535
+
+// Rows of the sequences of one call.  Passed to kernels by value (kernel arguments hold 4 KB;
+// FM_MAX_SEQ + 1 starts are 1 KB), so nothing has to be copied to the device before a launch and a
+// captured graph carries its own.  one_row: sequence s is row s.
+struct FmSeqs {
+    int n_seq, one_row;
+    int start[FM_MAX_SEQ + 1];
+};
+FM_HD int fm_seq_row0(const FmSeqs &s, int i) { return s.one_row ? i : s.start[i]; }
+FM_HD int fm_seq_rows(const FmSeqs &s, int i) { return s.one_row ? 1 : s.start[i + 1] - s.start[i]; }
+
+struct FmGdn {
+    int k_heads, v_heads, k_dim, v_dim, l2norm;
+    float scale;
+    const void *q, *k, *v;
+    int64_t q_stride, k_stride, v_stride;
+    const float *g, *beta;
+    void *out;
+};
+
+// The sequences of one launch, by value: 128 of them are 2.6 KB of kernel arguments.
+#define FM_GDN_SEQS 128
+struct FmGdnSeqs {
+    int n;
+    int start[FM_GDN_SEQS + 1];
+    const float *in[FM_GDN_SEQS];
+    float *out[FM_GDN_SEQS];
+};
+
+struct FmKv {
+    int8_t *k, *v;
+    float *k_scale, *v_scale;
+    int n_pages, page_tokens, page_shift, kv_heads;
+    const int32_t *len, *pages;
+    int max_pages;
+};
+
+struct FmKvRows {
+    const void *k, *v;      // rows appended
+    float *k_out, *v_out;   // rows read back
+    int64_t k_stride, v_stride;
+};
+
+struct FmAttn {
+    const void *q;
+    int64_t q_stride;
+    void *out;
+    int q_heads, group;     // query heads per cache head
+    float scale_log2;       // scale * log2(e)
+    int max_len;            // keys from here on are not seen, at most max_pages * page_tokens
+    int chunk;              // keys of one workgroup (a multiple of 4 * FM_ATTN_KEYS)
+    int n_chunks;           // workgroups over the longest sequence
+    int n_tiles;            // column tiles of the sequence with the most rows
+    float *part_o, *part_ml;
+};
+#define FM_ATTN_KEYS 64     // keys of a wave's step
+#define FM_ATTN_COLS 16     // columns of a tile
+
+// ---- the paged cache's addresses -----------------------------------------------------------
+// the page that holds position `pos` of sequence s, or -1 for one that is not there
+FM_HD int fm_kv_page(const FmKv &c, int s, int pos) {
+    if (pos < 0) return -1;
+    const int at = pos >> c.page_shift;
+    if (at >= c.max_pages) return -1;
+    const int p = c.pages[(int64_t)s * c.max_pages + at];
+    return p >= 0 && p < c.n_pages ? p : -1;
+}
+// byte offset of a code: keys [page][head][token][dim], values [page][head][dim][token]
+FM_HD int64_t fm_kv_k_at(const FmKv &c, int D, int page, int head, int pos, int dim) {
+    return (((int64_t)page * c.kv_heads + head) * c.page_tokens + (pos & (c.page_tokens - 1))) * D + dim;
+}
+FM_HD int64_t fm_kv_v_at(const FmKv &c, int D, int page, int head, int pos, int dim) {
+    return (((int64_t)page * c.kv_heads + head) * D + dim) * c.page_tokens + (pos & (c.page_tokens - 1));
+}
+// Rows of one sequence that an append writes into its j-th page from the first one touched:
+// false if there are none.  start: the page's first position; tokens t0 .. t1 - 1 of it; row0: row
+// (of the sequence) of the page's token 0, may be negative.
+struct FmKvSpan {
+    int start, t0, t1, row0;
+};
+FM_HD bool fm_kv_span(int n, int len, int page_shift, int j, FmKvSpan *out) {
+    if (n <= 0 || len <= 0) return false;
+    const int first = len < n ? 0 : len - n, P = 1 << page_shift;
+    const int64_t start = ((int64_t)(first >> page_shift) + j) << page_shift;
+    if (start >= len) return false;
+    out->start = (int)start;
+    out->t0 = first > out->start ? first - out->start : 0;
+    out->t1 = len - out->start < P ? len - out->start : P;
+    out->row0 = n - len + out->start;
+    return true;
+}
+
+// ---- the checks ----------------------------------------------------------------------------
+struct FmWhy {
+    char text[256];
+};
+inline int fm_why(FmWhy *w, int code, const char *fmt, ...) {
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(w->text, sizeof w->text, fmt, ap);
+    va_end(ap);
+    return code;
+}
+
+// Rows of a call's sequences: the check of seq_start that every mixer makes.
+inline int fm_check_rows(FmWhy *w, const int32_t *start, int n_seq, int *rows) {
+    if (n_seq < 1 || n_seq > FM_MAX_SEQ) return fm_why(w, FM_ERR_ARG, "n_seq %d outside 1..%d", n_seq, FM_MAX_SEQ);
+    *rows = n_seq;
+    if (!start) return FM_OK;
+    if (start[0] != 0) return fm_why(w, FM_ERR_ARG, "seq_start[0] is %d, not 0", start[0]);
+    for (int i = 0; i < n_seq; i++)
+        if (start[i + 1] < start[i]) return fm_why(w, FM_ERR_ARG, "seq_start[%d] %d below its predecessor %d", i + 1, start[i + 1], start[i]);
+    *rows = start[n_seq];
+    if (*rows > FM_MAX_ROWS) return fm_why(w, FM_ERR_ARG, "%d rows, at most %d", *rows, FM_MAX_ROWS);
+    return FM_OK;
+}
+inline int fm_check_dtype(FmWhy *w, int dtype) {
+    return dtype == FM_DTYPE_F32 || dtype == FM_DTYPE_BF16 ? FM_OK : fm_why(w, FM_ERR_ARG, "dtype %d", dtype);
+}
+// a vector of rows: 16-byte aligned, its stride too, and at least a row wide
+inline int fm_check_vec(FmWhy *w, const char *what, const void *p, int64_t stride, int64_t width, int dtype) {
+    const int size = dtype == FM_DTYPE_BF16 ? 2 : 4;
+    if (!p) return fm_why(w, FM_ERR_ARG, "null pointer: %s", what);
+    if ((uintptr_t)p & 15) return fm_why(w, FM_ERR_ARG, "%s is not 16-byte aligned", what);
+    if (stride < width) return fm_why(w, FM_ERR_ARG, "row stride %lld of %s below its width %lld", (long long)stride, what, (long long)width);
+    if (stride > ((int64_t)1 << 40)) return fm_why(w, FM_ERR_ARG, "row stride %lld of %s", (long long)stride, what);
+    if (stride * size % 16) return fm_why(w, FM_ERR_ARG, "row stride %lld of %s leaves rows unaligned (16 bytes)", (long long)stride, what);
+    return FM_OK;
+}
+inline void fm_fill_seqs(FmSeqs *b, const int32_t *start, int n_seq) {
+    memset(b, 0, sizeof *b);
+    b->n_seq = n_seq;
+    b->one_row = !start;
+    if (start) memcpy(b->start, start, (size_t)(n_seq + 1) * sizeof(int));
+}
+inline int fm_gdn_check(FmWhy *w, const fm_gated_delta_args *p, FmGdn *a) {
+    if (!p) return fm_why(w, FM_ERR_ARG, "null arguments");
+    int rows, rc;
+    if ((rc = fm_check_rows(w, p->seq_start, p->n_seq, &rows))) return rc;
+    if ((rc = fm_check_dtype(w, p->dtype))) return rc;
+    if (p->flags & ~FM_GDN_L2NORM) return fm_why(w, FM_ERR_ARG, "flags 0x%x", p->flags);
+    if (p->k_heads < 1 || p->v_heads < p->k_heads || p->v_heads > 256 || p->v_heads % p->k_heads)
+        return fm_why(w, FM_ERR_ARG, "%d key heads, %d value heads", p->k_heads, p->v_heads);
+    if (p->k_dim != 64 && p->k_dim != 128) return fm_why(w, FM_ERR_UNSUPPORTED, "k_dim %d (64 or 128)", p->k_dim);
+    if (p->v_dim < 16 || p->v_dim > 256 || p->v_dim % 16)
+        return fm_why(w, FM_ERR_UNSUPPORTED, "v_dim %d (multiples of 16 up to 256)", p->v_dim);
+    const int64_t kw = (int64_t)p->k_heads * p->k_dim, vw = (int64_t)p->v_heads * p->v_dim;
+    if ((rc = fm_check_vec(w, "d_q", p->d_q, p->q_stride, kw, p->dtype))) return rc;
+    if ((rc = fm_check_vec(w, "d_k", p->d_k, p->k_stride, kw, p->dtype))) return rc;
+    if ((rc = fm_check_vec(w, "d_v", p->d_v, p->v_stride, vw, p->dtype))) return rc;
+    if ((rc = fm_check_vec(w, "d_out", p->d_out, vw, vw, p->dtype))) return rc;
+    if (!p->d_g || !p->d_beta || !p->d_state_out) return fm_why(w, FM_ERR_ARG, "null pointer");
+    if (((uintptr_t)p->d_g | (uintptr_t)p->d_beta) & 3) return fm_why(w, FM_ERR_ARG, "d_g or d_beta not 4-byte aligned");
+    const size_t state = (size_t)vw * p->k_dim * sizeof(float);
+    // Outputs in address order: neighbours must lie a state apart, and an input may only meet the output
+    // of its own sequence, exactly.
+    std::pair<uintptr_t, int> outs[FM_MAX_SEQ];
+    for (int i = 0; i < p->n_seq; i++) {
+        const void *out = p->d_state_out[i], *in = p->d_state_in ? p->d_state_in[i] : nullptr;
+        if (!out) return fm_why(w, FM_ERR_ARG, "null state output %d", i);
+        if (((uintptr_t)out | (uintptr_t)in) & 15) return fm_why(w, FM_ERR_ARG, "state %d is not 16-byte aligned", i);
+        outs[i] = {(uintptr_t)out, i};
+    }
+    std::sort(outs, outs + p->n_seq);
+    for (int i = 1; i < p->n_seq; i++)
+        if (outs[i].first - outs[i - 1].first < state)
+            return fm_why(w, FM_ERR_ARG, "state outputs %d and %d overlap", outs[i - 1].second, outs[i].second);
+    for (int i = 0; p->d_state_in && i < p->n_seq; i++) {
+        const uintptr_t in = (uintptr_t)p->d_state_in[i];
+        if (!in) continue;
+        auto it = std::lower_bound(outs, outs + p->n_seq, std::make_pair(in, -1));
+        if (it != outs + p->n_seq && it->first - in < state && !(it->first == in && it->second == i))
+            return fm_why(w, FM_ERR_ARG, "state output %d overlaps state input %d", it->second, i);
+        if (it != outs && in - (it - 1)->first < state)
+            return fm_why(w, FM_ERR_ARG, "state output %d overlaps state input %d", (it - 1)->second, i);
+    }
+    a->k_heads = p->k_heads;
+    a->v_heads = p->v_heads;
+    a->k_dim = p->k_dim;
+    a->v_dim = p->v_dim;
+    a->l2norm = (p->flags & FM_GDN_L2NORM) != 0;
+    a->scale = p->scale;
+    a->q = p->d_q;
+    a->k = p->d_k;
+    a->v = p->d_v;
+    a->q_stride = p->q_stride;
+    a->k_stride = p->k_stride;
+    a->v_stride = p->v_stride;
+    a->g = p->d_g;
+    a->beta = p->d_beta;
+    a->out = p->d_out;
+    return FM_OK;
+}
+
+inline int fm_kv_check(FmWhy *w, const fm_kv_cache *p, const int32_t *len, const int32_t *pages, int max_pages, FmKv *k) {
+    if (!p->d_k || !p->d_v || !p->d_k_scale || !p->d_v_scale || !len || !pages)
+        return fm_why(w, FM_ERR_ARG, "null pointer");
+    if (((uintptr_t)p->d_k | (uintptr_t)p->d_v) & 15) return fm_why(w, FM_ERR_ARG, "cache codes are not 16-byte aligned");
+    if (((uintptr_t)p->d_k_scale | (uintptr_t)p->d_v_scale | (uintptr_t)len | (uintptr_t)pages) & 3)
+        return fm_why(w, FM_ERR_ARG, "scales, lengths or page table not 4-byte aligned");
+    if (p->page_tokens != 16 && p->page_tokens != 32 && p->page_tokens != 64 && p->page_tokens != 128)
+        return fm_why(w, FM_ERR_UNSUPPORTED, "pages of %d tokens (16, 32, 64 or 128)", p->page_tokens);
+    if (p->head_dim != 64 && p->head_dim != 128 && p->head_dim != 256)
+        return fm_why(w, FM_ERR_UNSUPPORTED, "head_dim %d (64, 128 or 256)", p->head_dim);
+    if (p->n_pages < 1 || p->kv_heads < 1 || p->kv_heads > 256) return fm_why(w, FM_ERR_ARG, "%d pages, %d cache heads", p->n_pages, p->kv_heads);
+    if (max_pages < 1 || (int64_t)max_pages * p->page_tokens > (int64_t)1 << 30)
+        return fm_why(w, FM_ERR_ARG, "max_pages %d", max_pages);
+    k->k = (int8_t *)p->d_k;
+    k->v = (int8_t *)p->d_v;
+    k->k_scale = p->d_k_scale;
+    k->v_scale = p->d_v_scale;
+    k->n_pages = p->n_pages;
+    k->page_tokens = p->page_tokens;
+    k->page_shift = __builtin_ctz((unsigned)p->page_tokens);
+    k->kv_heads = p->kv_heads;
+    k->len = len;
+    k->pages = pages;
+    k->max_pages = max_pages;
+    return FM_OK;
+}
+
+
+// operands of fm_kv_append_dev / fm_kv_read_dev
+inline int fm_kv_rows_check(FmWhy *w, const fm_kv_args *p, int read, FmKv *k, FmKvRows *x, FmSeqs *b) {
+    if (!p) return fm_why(w, FM_ERR_ARG, "null arguments");
+    int rows, rc;
+    if ((rc = fm_check_rows(w, p->seq_start, p->n_seq, &rows))) return rc;
+    if ((rc = fm_check_dtype(w, p->dtype))) return rc;
+    if (read && p->dtype != FM_DTYPE_F32) return fm_why(w, FM_ERR_UNSUPPORTED, "rows are read back as fp32");
+    if ((rc = fm_kv_check(w, &p->cache, p->d_len, p->d_pages, p->max_pages, k))) return rc;
+    const int64_t width = (int64_t)p->cache.kv_heads * p->cache.head_dim;
+    if ((rc = fm_check_vec(w, "d_k", p->d_k, p->k_stride, width, p->dtype))) return rc;
+    if ((rc = fm_check_vec(w, "d_v", p->d_v, p->v_stride, width, p->dtype))) return rc;
+    fm_fill_seqs(b, p->seq_start, p->n_seq);
+    *x = FmKvRows{p->d_k, p->d_v, (float *)p->d_k, (float *)p->d_v, p->k_stride, p->v_stride};
+    return FM_OK;
+}
+
+// ---- how a call is cut ---------------------------------------------------------------------
+inline int fm_most_rows(const FmSeqs &b) {
+    int most = b.one_row ? 1 : 0;
+    if (!b.one_row)
+        for (int i = 0; i < b.n_seq; i++) most = b.start[i + 1] - b.start[i] > most ? b.start[i + 1] - b.start[i] : most;
+    return most;
+}
+inline int fm_all_rows(const FmSeqs &b) { return b.one_row ? b.n_seq : b.start[b.n_seq]; }
+
+// Attention: chunks of keys so that about four workgroups per CU are there.  Returns the workspace.
+inline size_t fm_attn_plan(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int n_cu) {
+    const int step = 4 * FM_ATTN_KEYS;
+    const int64_t have = (int64_t)c->max_pages * c->page_tokens;
+    if (a->max_len > have) a->max_len = (int)have;
+    a->n_tiles = (int)(((int64_t)fm_most_rows(*b) * a->group + FM_ATTN_COLS - 1) / FM_ATTN_COLS);
+    const int64_t groups = (int64_t)(a->n_tiles > 0 ? a->n_tiles : 1) * b->n_seq * c->kv_heads;
+    const int64_t want = (4 * (int64_t)n_cu + groups - 1) / groups;
+    int64_t chunk = ((int64_t)a->max_len + want - 1) / want;
+    chunk = (chunk + step - 1) / step * step;
+    if (chunk < step) chunk = step;
+    a->chunk = (int)chunk;
+    a->n_chunks = (int)(((int64_t)a->max_len + chunk - 1) / chunk);
+    if (a->n_chunks < 1) a->n_chunks = 1;
+    if (a->n_chunks == 1) return 0;
+    return (size_t)fm_all_rows(*b) * a->q_heads * a->n_chunks * (D + 2) * sizeof(float);
+}
+
+inline int fm_attn_check(FmWhy *w, const fm_attn_args *p, int n_cu, FmKv *k, FmAttn *a, FmSeqs *b, size_t *ws) {
+    if (!p) return fm_why(w, FM_ERR_ARG, "null arguments");
+    int rows, rc;
+    if ((rc = fm_check_rows(w, p->seq_start, p->n_seq, &rows))) return rc;
+    if ((rc = fm_check_dtype(w, p->dtype))) return rc;
+    if ((rc = fm_kv_check(w, &p->cache, p->d_len, p->d_pages, p->max_pages, k))) return rc;
+    if (p->q_heads < 1 || p->q_heads > 1024 || p->q_heads % p->cache.kv_heads)
+        return fm_why(w, FM_ERR_ARG, "%d query heads on %d cache heads", p->q_heads, p->cache.kv_heads);
+    if (p->max_len < 0) return fm_why(w, FM_ERR_ARG, "max_len %d", p->max_len);
+    const int64_t width = (int64_t)p->q_heads * p->cache.head_dim;
+    if ((rc = fm_check_vec(w, "d_q", p->d_q, p->q_stride, width, p->dtype))) return rc;
+    if ((rc = fm_check_vec(w, "d_out", p->d_out, width, width, p->dtype))) return rc;
+    memset(a, 0, sizeof *a);
+    a->q = p->d_q;
+    a->q_stride = p->q_stride;
+    a->out = p->d_out;
+    a->q_heads = p->q_heads;
+    a->group = p->q_heads / p->cache.kv_heads;
+    a->scale_log2 = (float)((double)p->scale * 1.4426950408889634);
+    a->max_len = p->max_len;
+    fm_fill_seqs(b, p->seq_start, p->n_seq);
+    *ws = fm_attn_plan(k, a, b, p->cache.head_dim, n_cu);
+    return FM_OK;
+}
+
+inline int fm_logprob_check(FmWhy *w, int rows, int vocab, int top_n) {
+    if (rows < 1 || rows > FM_MAX_ROWS) return fm_why(w, FM_ERR_ARG, "%d rows outside 1..%d", rows, FM_MAX_ROWS);
+    if (vocab < 1 || vocab > (1 << 30)) return fm_why(w, FM_ERR_ARG, "vocab %d", vocab);
+    if (top_n < 0 || top_n > 32 || top_n > vocab) return fm_why(w, FM_ERR_ARG, "top_n %d outside 0..min(32, vocab)", top_n);
+    return FM_OK;
+}
+
+inline int fm_logprob_args_check(FmWhy *w, const void *d_logits, int rows, int vocab, int64_t row_stride, const void *d_tokens,
+                                 int top_n, const void *d_logprob, const void *d_entropy, const void *d_top_ids,
+                                 const void *d_top_logprobs) {
+    if (!d_logits) return fm_why(w, FM_ERR_ARG, "null pointer");
+    int rc = fm_logprob_check(w, rows, vocab, top_n);
+    if (rc) return rc;
+    if (row_stride < vocab || row_stride > ((int64_t)1 << 40))
+        return fm_why(w, FM_ERR_ARG, "row stride %lld, vocab %d", (long long)row_stride, vocab);
+    if (!d_tokens != !d_logprob) return fm_why(w, FM_ERR_ARG, "tokens and their log probabilities go together");
+    if (!d_top_ids != !d_top_logprobs || !d_top_ids != !top_n)
+        return fm_why(w, FM_ERR_ARG, "top_n, top ids and top log probabilities go together");
+    if (((uintptr_t)d_logits | (uintptr_t)d_tokens | (uintptr_t)d_logprob | (uintptr_t)d_entropy | (uintptr_t)d_top_ids |
+         (uintptr_t)d_top_logprobs) & 3)
+        return fm_why(w, FM_ERR_ARG, "pointer not 4-byte aligned");
+    return FM_OK;
+}

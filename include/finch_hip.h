@@ -370,6 +370,123 @@ FM_API int fm_embed_lookup_dev(fm_ctx *ctx, fm_tensor t, const int32_t *d_token_
                         float *d_out);
 FM_API int fm_embed_lookup(fm_ctx *ctx, fm_tensor t, int token_id, float *out);
 
+/* ---------------------------------------------------------------- token mixers
+ * What stands between the quantized products of a token: the gated delta rule that the
+ * GatedDeltaNet projections feed, and attention over a cache held in 8 bits.  Vectors are fp32,
+ * or bfloat16 bits where dtype says so; sums, statistics and states are fp32 in either case.
+ * Rows (tokens) of several sequences lie one behind the other; seq_start names where each begins:
+ * n_seq + 1 ascending row numbers in HOST memory, the first of them 0 (a sequence may be empty).
+ * seq_start == NULL: one row per sequence.  It is read during the call only; the launch carries
+ * the values, so a captured graph replays them.  Row strides count elements between the rows of a
+ * vector whose heads lie side by side, so q, k and v may point into one buffer; d_q, d_k, d_v and
+ * d_out are 16-byte aligned and the strides keep every row so.  Inputs and outputs do not overlap
+ * except where it says so.  Workspace is the context's: calls of one context, and graphs captured
+ * from it, run one after another. */
+enum { FM_DTYPE_F32 = 0, FM_DTYPE_BF16 = 1 };
+#define FM_MAX_SEQ 256            /* sequences of one call */
+
+/* The gated delta rule.  Per sequence and value head h (its key head is
+ * h / (v_heads / k_heads)), with the state S [v_dim][k_dim] and for each token
+ *   S = exp(g) * S;  u = beta * (v - S k);  S = S + u k^T;  out = scale * S q
+ * FM_GDN_L2NORM: q and k are divided by sqrt(sum of squares + 1e-6) first.
+ *   d_q, d_k [rows][k_heads][k_dim], d_v [rows][v_heads][v_dim], d_out [rows][v_heads][v_dim]
+ *   contiguous, d_g (logarithm of the decay, -inf wipes the state) and d_beta
+ *   [rows][v_heads] fp32 contiguous.
+ *   d_state_in, d_state_out: HOST arrays of n_seq device pointers, each a state
+ *   [v_heads][v_dim][k_dim] fp32, 16-byte aligned.  d_state_in or an entry of it NULL: zeros.  An output may be
+ *   its own sequence's input (update in place); any other overlap, also of two outputs, is
+ *   FM_ERR_ARG.  An empty sequence's state is copied.
+ * k_dim 64 or 128, v_dim a multiple of 16 up to 256, v_heads a multiple of k_heads (up to 256).
+ * Short sequences run token by token, long ones in chunks of 64 tokens on the matrix cores; the
+ * two agree to fp32 rounding. */
+enum { FM_GDN_L2NORM = 1 };
+typedef struct {
+    int32_t n_seq, k_heads, v_heads, k_dim, v_dim, dtype, flags;
+    float scale;
+    const void *d_q, *d_k, *d_v;
+    int64_t q_stride, k_stride, v_stride;
+    const float *d_g, *d_beta;
+    const int32_t *seq_start;
+    const float *const *d_state_in;
+    float *const *d_state_out;
+    void *d_out;
+} fm_gated_delta_args;
+FM_API int fm_gated_delta_dev(fm_ctx *ctx, const fm_gated_delta_args *args);
+
+/* A cache of keys and values in 8 bits, in pages of page_tokens (16, 32, 64 or 128) tokens:
+ * codes d_k [n_pages][kv_heads][page_tokens][head_dim] and d_v
+ * [n_pages][kv_heads][head_dim][page_tokens] (transposed: the order the second product of
+ * attention reads), and one fp32 scale per page and head for each; a value is code * scale.  head_dim
+ * 64, 128 or 256.  The memory is the caller's (codes 16-byte aligned).
+ * A sequence's tokens lie in the pages that its row of the table names: d_pages
+ * [n_seq][max_pages], d_len [n_seq] the number of its tokens INCLUDING the rows of the call
+ * (both in device memory).  An entry outside 0..n_pages-1 is a page that is not there: nothing is
+ * written for its tokens, they read as zeros and attention does not see them.  Positions from
+ * max_pages * page_tokens on are not there either. */
+typedef struct {
+    void *d_k, *d_v;
+    float *d_k_scale, *d_v_scale;
+    int32_t n_pages, page_tokens, kv_heads, head_dim;
+} fm_kv_cache;
+
+/* fm_kv_append_dev: rows k, v [rows][kv_heads][head_dim] become the last tokens of their
+ * sequences (positions d_len - rows of the sequence .. d_len - 1).  A page's scale is the largest finite
+ * magnitude in it / 127; a page that already holds tokens keeps its scale unless a new token
+ * exceeds it, then the old codes are rounded to the new scale.  code = round to nearest even of value / scale,
+ * decided exactly; a NaN becomes 0, an infinity +-127.  The same rows appended again change nothing.
+ * A page that two sequences of the call append to is not defined.
+ * fm_kv_read_dev: the last rows of each sequence back as fp32 (dtype must be FM_DTYPE_F32);
+ * positions below 0 read as zeros. */
+typedef struct {
+    fm_kv_cache cache;
+    int32_t n_seq, dtype;
+    void *d_k, *d_v;                 /* fm_kv_append_dev reads them, fm_kv_read_dev writes them */
+    int64_t k_stride, v_stride;
+    const int32_t *seq_start;
+    const int32_t *d_len, *d_pages;
+    int32_t max_pages;
+} fm_kv_args;
+FM_API int fm_kv_append_dev(fm_ctx *ctx, const fm_kv_args *args);
+FM_API int fm_kv_read_dev(fm_ctx *ctx, const fm_kv_args *args);
+
+/* Attention over the cache: rows q [rows][q_heads][head_dim] are the last tokens of their
+ * sequences; row i of n sees the keys at positions 0 .. d_len - n + i.  Query head h reads cache head
+ * h / (q_heads / kv_heads).  out [rows][q_heads][head_dim] contiguous =
+ * sum softmax(scale * q.k) v; a row that sees nothing (d_len 0, pages that are not there) is
+ * zeros.  max_len: upper bound of d_len; keys from it on are not seen.  The size of the
+ * launch goes by it, so a captured graph takes the largest length it will be replayed at. */
+typedef struct {
+    fm_kv_cache cache;
+    int32_t n_seq, q_heads, dtype;
+    float scale;
+    const void *d_q;
+    int64_t q_stride;
+    const int32_t *seq_start;
+    const int32_t *d_len, *d_pages;
+    int32_t max_pages, max_len;
+    void *d_out;
+} fm_attn_args;
+FM_API int fm_attn_dev(fm_ctx *ctx, const fm_attn_args *args);
+
+/* Bytes of workspace that the call would take (for fm_reserve before a capture); 0 for
+ * arguments that the call refuses. */
+FM_API size_t fm_gated_delta_ws_bytes(fm_ctx *ctx, const fm_gated_delta_args *args);
+FM_API size_t fm_attn_ws_bytes(fm_ctx *ctx, const fm_attn_args *args);
+
+/* ---------------------------------------------------------------- log probabilities
+ * What is read off the vocabulary projection's output: for each of `rows` rows of logits
+ * (row_stride >= vocab elements apart), all outputs in device memory,
+ *   d_logprob[rows]  log softmax at d_tokens[row] (-inf for an id outside 0..vocab-1)
+ *   d_entropy[rows]  -sum p log p (a logit of -inf adds nothing)
+ *   d_top_ids, d_top_logprobs [rows][top_n]  the top_n largest, equal ones in the order of their ids
+ * Each output may be NULL (d_tokens and d_logprob go together, so do the last two).  top_n
+ * 0..32 and <= vocab.  A row of -inf alone has log probabilities -inf, entropy 0 and the ids 0..top_n-1;
+ * one that holds a NaN or +inf has NaN everywhere and ids -1.  No counterpart in the reference. */
+FM_API int fm_logprobs_dev(fm_ctx *ctx, const float *d_logits, int rows, int vocab, int64_t row_stride,
+                    const int32_t *d_tokens, int top_n, float *d_logprob, float *d_entropy,
+                    int32_t *d_top_ids, float *d_top_logprobs);
+FM_API size_t fm_logprobs_ws_bytes(fm_ctx *ctx, int rows, int vocab, int top_n);
+
 /* ---------------------------------------------------------------- dequant (bit-exact checks)
  * The reference has no such call; these expose what its kernels compute on the
  * fly — code = field of the packed word, w = (float)code * scale + bias in fp32

@@ -1,0 +1,264 @@
+// Host program over finchmoe_amd/csrc/fm_mix_index.h: every refusal of the token mixers' entry
+// points, and a walk of the paged cache's addresses — each (sequence, head, step, lane, load) of the
+// attention and of the appends, over page tables with entries that are not there, against the buffers'
+// sizes.  Built with the address and undefined-behaviour sanitizers; no GPU.
+#include <stdio.h>
+#include <stdlib.h>
+
+#include <set>
+#include <vector>
+
+#include "../../finchmoe_amd/csrc/fm_mix_index.h"
+
+static int bad = 0;
+#define CHECK(cond)                                                       \
+    do {                                                                  \
+        if (!(cond)) {                                                    \
+            printf("line %d: %s\n", __LINE__, #cond);                     \
+            bad++;                                                        \
+        }                                                                 \
+    } while (0)
+
+static unsigned rnd_state = 1;
+static int rnd(int n) {
+    rnd_state = rnd_state * 1664525u + 1013904223u;
+    return (int)((rnd_state >> 8) % (unsigned)n);
+}
+static void *at(uintptr_t a) { return (void *)a; }
+
+// ---- refusals
+static void refuse_gdn() {
+    FmWhy w;
+    FmGdn a;
+    const uintptr_t B = 1 << 20;
+    const float *in[3] = {(float *)at(B), (float *)at(2 * B), nullptr};
+    float *out[3] = {(float *)at(B), (float *)at(4 * B), (float *)at(5 * B)};
+    int start[4] = {0, 5, 5, 9};
+    fm_gated_delta_args g{};
+    g.n_seq = 3, g.k_heads = 2, g.v_heads = 4, g.k_dim = 128, g.v_dim = 64, g.scale = 1;
+    g.d_q = g.d_k = g.d_v = at(16 * B), g.d_out = at(32 * B), g.d_g = g.d_beta = (float *)at(48 * B);
+    g.q_stride = g.k_stride = g.v_stride = 256;
+    g.seq_start = start, g.d_state_in = in, g.d_state_out = out;
+    CHECK(fm_gdn_check(&w, &g, &a) == FM_OK);
+    CHECK(fm_gdn_check(&w, nullptr, &a) == FM_ERR_ARG);
+#define BAD(field, value, code)                                           \
+    do {                                                                  \
+        auto h = g;                                                       \
+        h.field = value;                                                  \
+        CHECK(fm_gdn_check(&w, &h, &a) == code);                          \
+    } while (0)
+    BAD(n_seq, 0, FM_ERR_ARG);
+    BAD(n_seq, FM_MAX_SEQ + 1, FM_ERR_ARG);
+    BAD(k_heads, 0, FM_ERR_ARG);
+    BAD(k_heads, 3, FM_ERR_ARG);
+    BAD(v_heads, 1, FM_ERR_ARG);
+    BAD(v_heads, 512, FM_ERR_ARG);
+    BAD(k_dim, 96, FM_ERR_UNSUPPORTED);
+    BAD(v_dim, 0, FM_ERR_UNSUPPORTED);
+    BAD(v_dim, 40, FM_ERR_UNSUPPORTED);
+    BAD(v_dim, 272, FM_ERR_UNSUPPORTED);
+    BAD(dtype, 2, FM_ERR_ARG);
+    BAD(flags, 2, FM_ERR_ARG);
+    BAD(d_q, nullptr, FM_ERR_ARG);
+    BAD(d_k, at(16 * B + 8), FM_ERR_ARG);
+    BAD(d_out, at(16 * B + 4), FM_ERR_ARG);
+    BAD(d_g, nullptr, FM_ERR_ARG);
+    BAD(d_beta, (float *)at(B + 2), FM_ERR_ARG);
+    BAD(q_stride, 255, FM_ERR_ARG);
+    BAD(k_stride, 258, FM_ERR_ARG);
+    BAD(v_stride, -256, FM_ERR_ARG);
+    BAD(d_state_out, nullptr, FM_ERR_ARG);
+    {
+        auto h = g;
+        h.dtype = FM_DTYPE_BF16;
+        h.q_stride = 260;      // 520 bytes: not a multiple of 16
+        CHECK(fm_gdn_check(&w, &h, &a) == FM_ERR_ARG);
+    }
+    int s1[4] = {1, 5, 5, 9}, s2[4] = {0, 5, 4, 9}, s3[4] = {0, 5, 5, 70000};
+    BAD(seq_start, s1, FM_ERR_ARG);
+    BAD(seq_start, s2, FM_ERR_ARG);
+    BAD(seq_start, s3, FM_ERR_ARG);
+    const size_t state = 4 * 64 * 128 * 4;
+    float *o1[3] = {(float *)at(B), (float *)at(B), (float *)at(5 * B)};
+    float *o2[3] = {(float *)at(4 * B), (float *)at(4 * B + state - 16), (float *)at(5 * B)};
+    float *o3[3] = {(float *)at(2 * B), (float *)at(4 * B), (float *)at(5 * B)};      // another sequence's input
+    float *o4[3] = {(float *)at(B + 16), (float *)at(4 * B), (float *)at(5 * B)};     // its own input, shifted
+    float *o5[3] = {(float *)at(B), (float *)at(4 * B), nullptr};
+    float *o6[3] = {(float *)at(B + 4), (float *)at(4 * B), (float *)at(5 * B)};
+    for (auto o : {o1, o2, o3, o4, o5, o6}) BAD(d_state_out, o, FM_ERR_ARG);
+    float *o7[3] = {(float *)at(4 * B + state), (float *)at(4 * B), (float *)at(4 * B + 2 * state)};
+    BAD(d_state_out, o7, FM_OK);
+    BAD(d_state_in, nullptr, FM_OK);
+    BAD(seq_start, nullptr, FM_OK);
+#undef BAD
+    // the overlap rule against plain pairwise comparison
+    for (int round = 0; round < 20000; round++) {
+        const int n = 1 + rnd(5);
+        const float *ri[5];
+        float *ro[5];
+        for (int i = 0; i < n; i++) {
+            ri[i] = rnd(4) ? (float *)at(B + (uintptr_t)rnd(14) * (state / 2)) : nullptr;
+            ro[i] = (float *)at(B + (uintptr_t)rnd(14) * (state / 2));
+        }
+        bool clash = false;
+        auto meet = [&](const void *x, const void *y) { return (uintptr_t)x < (uintptr_t)y + state && (uintptr_t)y < (uintptr_t)x + state; };
+        for (int i = 0; i < n; i++)
+            for (int j = 0; j < n; j++) {
+                if (j < i && meet(ro[i], ro[j])) clash = true;
+                if (ri[j] && meet(ro[i], ri[j]) && !(i == j && ro[i] == ri[j])) clash = true;
+            }
+        auto h = g;
+        h.n_seq = n, h.seq_start = nullptr, h.d_state_in = ri, h.d_state_out = ro;
+        CHECK((fm_gdn_check(&w, &h, &a) == FM_OK) == !clash);
+    }
+}
+
+static void refuse_cache() {
+    FmWhy w;
+    FmKv k;
+    FmAttn a;
+    FmSeqs b;
+    FmKvRows x;
+    size_t ws;
+    const uintptr_t B = 1 << 20;
+    fm_attn_args g{};
+    g.cache.d_k = g.cache.d_v = at(B), g.cache.d_k_scale = g.cache.d_v_scale = (float *)at(2 * B);
+    g.cache.n_pages = 4, g.cache.page_tokens = 32, g.cache.kv_heads = 2, g.cache.head_dim = 128;
+    g.n_seq = 2, g.q_heads = 6, g.scale = 1, g.d_q = at(3 * B), g.d_out = at(4 * B), g.q_stride = 768;
+    g.d_len = g.d_pages = (int32_t *)at(5 * B), g.max_pages = 3, g.max_len = 96;
+    CHECK(fm_attn_check(&w, &g, 256, &k, &a, &b, &ws) == FM_OK);
+    CHECK(fm_attn_check(&w, nullptr, 256, &k, &a, &b, &ws) == FM_ERR_ARG);
+#define BAD(field, value, code)                                           \
+    do {                                                                  \
+        auto h = g;                                                       \
+        h.field = value;                                                  \
+        CHECK(fm_attn_check(&w, &h, 256, &k, &a, &b, &ws) == code);       \
+    } while (0)
+    BAD(cache.d_k, nullptr, FM_ERR_ARG);
+    BAD(cache.d_v, at(B + 8), FM_ERR_ARG);
+    BAD(cache.d_k_scale, (float *)at(B + 2), FM_ERR_ARG);
+    BAD(cache.n_pages, 0, FM_ERR_ARG);
+    BAD(cache.page_tokens, 8, FM_ERR_UNSUPPORTED);
+    BAD(cache.page_tokens, 256, FM_ERR_UNSUPPORTED);
+    BAD(cache.head_dim, 192, FM_ERR_UNSUPPORTED);
+    BAD(cache.kv_heads, 0, FM_ERR_ARG);
+    BAD(cache.kv_heads, 4, FM_ERR_ARG);
+    BAD(q_heads, 0, FM_ERR_ARG);
+    BAD(q_heads, 2048, FM_ERR_ARG);
+    BAD(d_len, nullptr, FM_ERR_ARG);
+    BAD(d_pages, nullptr, FM_ERR_ARG);
+    BAD(max_pages, 0, FM_ERR_ARG);
+    BAD(max_pages, 1 << 26, FM_ERR_ARG);
+    BAD(max_len, -1, FM_ERR_ARG);
+    BAD(q_stride, 760, FM_ERR_ARG);
+    BAD(d_out, at(4 * B + 2), FM_ERR_ARG);
+    BAD(dtype, -1, FM_ERR_ARG);
+    BAD(n_seq, 257, FM_ERR_ARG);
+#undef BAD
+    fm_kv_args r{};
+    r.cache = g.cache, r.n_seq = 2, r.d_k = r.d_v = at(6 * B), r.k_stride = r.v_stride = 256;
+    r.d_len = r.d_pages = g.d_len, r.max_pages = 3;
+    CHECK(fm_kv_rows_check(&w, &r, 0, &k, &x, &b) == FM_OK && fm_kv_rows_check(&w, &r, 1, &k, &x, &b) == FM_OK);
+    r.dtype = FM_DTYPE_BF16;
+    CHECK(fm_kv_rows_check(&w, &r, 0, &k, &x, &b) == FM_OK && fm_kv_rows_check(&w, &r, 1, &k, &x, &b) == FM_ERR_UNSUPPORTED);
+    r.v_stride = 128;
+    CHECK(fm_kv_rows_check(&w, &r, 0, &k, &x, &b) == FM_ERR_ARG);
+    r.v_stride = 256, r.d_v = nullptr;
+    CHECK(fm_kv_rows_check(&w, &r, 0, &k, &x, &b) == FM_ERR_ARG);
+}
+
+static void refuse_logprobs() {
+    FmWhy w;
+    void *p = at(1 << 20);
+    CHECK(fm_logprob_args_check(&w, p, 3, 100, 100, p, 5, p, p, p, p) == FM_OK);
+    CHECK(fm_logprob_args_check(&w, p, 3, 100, 100, nullptr, 0, nullptr, nullptr, nullptr, nullptr) == FM_OK);
+    CHECK(fm_logprob_args_check(&w, nullptr, 3, 100, 100, p, 5, p, p, p, p) == FM_ERR_ARG);
+    CHECK(fm_logprob_args_check(&w, p, 0, 100, 100, p, 5, p, p, p, p) == FM_ERR_ARG);
+    CHECK(fm_logprob_args_check(&w, p, 65536, 100, 100, p, 5, p, p, p, p) == FM_ERR_ARG);
+    CHECK(fm_logprob_args_check(&w, p, 3, 100, 99, p, 5, p, p, p, p) == FM_ERR_ARG);
+    CHECK(fm_logprob_args_check(&w, p, 3, 100, 100, p, 33, p, p, p, p) == FM_ERR_ARG);
+    CHECK(fm_logprob_args_check(&w, p, 3, 4, 100, p, 5, p, p, p, p) == FM_ERR_ARG);
+    CHECK(fm_logprob_args_check(&w, p, 3, 100, 100, nullptr, 5, p, p, p, p) == FM_ERR_ARG);
+    CHECK(fm_logprob_args_check(&w, p, 3, 100, 100, p, 5, p, p, nullptr, p) == FM_ERR_ARG);
+    CHECK(fm_logprob_args_check(&w, p, 3, 100, 100, p, 0, p, p, p, p) == FM_ERR_ARG);
+    CHECK(fm_logprob_args_check(&w, p, 3, 100, 100, p, 5, at((1 << 20) + 2), p, p, p) == FM_ERR_ARG);
+}
+
+// ---- the cache's addresses
+static void walk(int n_seq, int kv, int D, int P, int group) {
+    const int n_pages = 1 + rnd(12), max_pages = 1 + rnd(6);
+    std::vector<int32_t> table((size_t)n_seq * max_pages), len(n_seq);
+    for (auto &t : table) t = rnd(5) ? rnd(n_pages) : rnd(2) ? -1 - rnd(5) : n_pages + rnd(3);
+    std::vector<int> start(n_seq + 1, 0);
+    for (int s = 0; s < n_seq; s++) {
+        len[s] = rnd(8) ? rnd(max_pages * P + 40) : (rnd(2) ? -3 : 0);
+        start[s + 1] = start[s] + rnd(70);
+    }
+    FmKv c{};
+    c.n_pages = n_pages, c.page_tokens = P, c.page_shift = __builtin_ctz((unsigned)P), c.kv_heads = kv;
+    c.len = len.data(), c.pages = table.data(), c.max_pages = max_pages;
+    const int64_t bytes = (int64_t)n_pages * kv * P * D;
+    FmAttn a{};
+    a.q_heads = kv * group, a.group = group, a.max_len = rnd(2) ? max_pages * P + 100 : 1 + rnd(max_pages * P);
+    FmSeqs b{};
+    b.n_seq = n_seq;
+    for (int s = 0; s <= n_seq; s++) b.start[s] = start[s];
+    const size_t ws = fm_attn_plan(&c, &a, &b, D, 1 + rnd(64));
+    CHECK(a.max_len <= max_pages * P && a.chunk % (4 * FM_ATTN_KEYS) == 0 && a.n_chunks >= 1);
+    CHECK((int64_t)a.chunk * a.n_chunks >= a.max_len);
+    CHECK(a.n_chunks == 1 || ws == (size_t)start[n_seq] * a.q_heads * a.n_chunks * (D + 2) * 4);
+    for (int s = 0; s < n_seq; s++)
+        for (int h = 0; h < kv; h++)
+            // (every step, also behind the length: a tile's last column may see more than its lane's own)
+            for (int pos0 = 0; pos0 < a.chunk * a.n_chunks; pos0 += FM_ATTN_KEYS)
+                for (int lane = 0; lane < 64; lane++) {
+                    const int g = lane >> 4, r = lane & 15;
+                    const int kp = fm_kv_page(c, s, pos0 + 16 * (r >> 2)), vp = fm_kv_page(c, s, pos0 + 16 * g);
+                    CHECK(kp < n_pages && vp < n_pages);
+                    const int64_t kb = fm_kv_k_at(c, D, kp < 0 ? 0 : kp, h, pos0 + 16 * (r >> 2) + (r & 3), 16 * g);
+                    const int64_t vb = fm_kv_v_at(c, D, vp < 0 ? 0 : vp, h, pos0 + 16 * g, r);
+                    for (int d = 0; d < D / 64; d++)
+                        for (int t = 0; t < 4; t++) CHECK(kb + 4 * t * D + 64 * d >= 0 && kb + 4 * t * D + 64 * d + 16 <= bytes);
+                    for (int d = 0; d < D / 16; d++) CHECK(vb + (int64_t)16 * d * P >= 0 && vb + (int64_t)16 * d * P + 16 <= bytes);
+                    CHECK(kb % 16 == 0 && vb % 16 == 0);
+                }
+    // appends: every row of a sequence that has a place is written once, to its own place
+    const int most = fm_most_rows(b);
+    for (int s = 0; s < n_seq; s++) {
+        const int n = start[s + 1] - start[s];
+        std::set<int> seen;
+        for (int j = 0; j < (most + P - 2) / P + 1; j++) {
+            FmKvSpan sp;
+            if (!fm_kv_span(n, len[s], c.page_shift, j, &sp)) continue;
+            CHECK(sp.t0 >= 0 && sp.t0 < sp.t1 && sp.t1 <= P);
+            const int page = fm_kv_page(c, s, sp.start);
+            for (int t = sp.t0; t < sp.t1; t++) {
+                CHECK(sp.row0 + t >= 0 && sp.row0 + t < n && sp.start + t == len[s] - n + sp.row0 + t);
+                CHECK(seen.insert(sp.start + t).second);
+                if (page < 0) continue;
+                for (int d = 0; d < D; d += D - 1) {
+                    const int64_t ka = fm_kv_k_at(c, D, page, kv - 1, t, d), va = fm_kv_v_at(c, D, page, kv - 1, t, d);
+                    CHECK(ka >= 0 && ka < bytes && va >= 0 && va < bytes);
+                }
+            }
+        }
+        CHECK((int)seen.size() == (len[s] <= 0 ? 0 : n < len[s] ? n : len[s]));
+    }
+}
+
+int main() {
+    refuse_gdn();
+    refuse_cache();
+    refuse_logprobs();
+    for (int round = 0; round < 60; round++)
+        for (int P : {16, 32, 64, 128}) walk(1 + rnd(4), 1 + rnd(3), 64 << rnd(3), P, 1 + rnd(9));
+    // far offsets: past 32 bits
+    FmKv c{};
+    c.n_pages = 1 << 20, c.page_tokens = 128, c.page_shift = 7, c.kv_heads = 8;
+    CHECK(fm_kv_k_at(c, 256, (1 << 20) - 1, 7, 127, 255) == ((int64_t)(1 << 20) * 8 * 128 * 256) - 1);
+    CHECK(fm_kv_v_at(c, 256, (1 << 20) - 1, 7, 127, 255) == ((int64_t)(1 << 20) * 8 * 128 * 256) - 1);
+    FmKvSpan sp;
+    CHECK(fm_kv_span(3, 2147483647, 4, 0, &sp) && !fm_kv_span(3, 2147483647, 4, 1 << 28, &sp));
+    if (!bad) printf("all refusals and addresses hold\n");
+    return bad ? 1 : 0;
+}
