@@ -10,6 +10,18 @@
 // so the sums of a token (these three and, normalised, |k|^2 and |q|^2) do not wait for each
 // other.  The state is read and written once per call and lives in registers in between: a call
 // of one token per sequence is bound by that traffic, a longer one by the chain of its sums.
+//
+// Longer sequences run in chunks of C = 64 tokens.  With G_i the sum of the chunk's g up to token i,
+// E_ij = e^(G_i - G_j) for j <= i and a chunk's rows K, Q, V, the u of all its tokens solve a triangular system,
+//   u_i + beta_i sum_{j<i} E_ij (k_i.k_j) u_j = beta_i (v_i - e^G_i S k_i)    =:  (1 + A) u = R
+//   o_i = scale (e^G_i S q_i + sum_{j<=i} E_ij (q_i.k_j) u_j)
+//   S <- e^G_C S + sum_i e^(G_C - G_i) u_i k_i^T
+// Everything that does not need the state — the inverse T of 1 + A, P = scale tril(E . Q K^T), K^T and the
+// factors of a token — is computed for all chunks at once by fm_gdn_prep; fm_gdn_scan walks the chunks in
+// order, sixteen state rows (value dims) a workgroup, with five small products a chunk.  Both use
+// the fp32 matrix instruction v_mfma_f32_16x16x4_f32: the state is an fp32 result, which 16-bit
+// operands would have to be split in three pieces (six products) to keep.
+// G is summed in fp64: E_ij is a difference of sums that may be hundreds while it is small itself.
 #include "fm_mix.h"
 
 namespace {
@@ -42,7 +54,7 @@ __global__ __launch_bounds__(256) void fm_gdn_steps(FmGdn a, FmGdnSeqs b) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15;
     const int s = blockIdx.z, h = blockIdx.y, hk = h / (a.v_heads / a.k_heads);
     const int v0 = (blockIdx.x * 4 + wave) * 4 * R + (lane >> 4);   // rows v0, v0 + 4, ...
-    const int t0 = b.start[s], T = b.start[s + 1] - t0;
+    const int t0 = b.row[s], T = b.rows[s];
     const int64_t head = (int64_t)h * a.v_dim * DK;
     const float *in = b.in[s];
     RowPart<DK> st[R];
@@ -109,35 +121,276 @@ __global__ __launch_bounds__(256) void fm_gdn_steps(FmGdn a, FmGdnSeqs b) {
                 *(fm_v4f *)(out + head + (int64_t)(v0 + 4 * r) * DK + 64 * n + 4 * li) = st[r].p[n];
 }
 
+__device__ __forceinline__ fm_v4f mfma4(float x, float y, fm_v4f c) {
+    return __builtin_amdgcn_mfma_f32_16x16x4f32(x, y, c, 0, 0, 0);
+}
+// c += sum over the 4 k of a float4 pair: lane group g supplies k = 4 g + e of each
+__device__ __forceinline__ fm_v4f mfma16(fm_v4f x, fm_v4f y, fm_v4f c) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) c = mfma4(x[e], y[e], c);
+    return c;
+}
+
+// Per (chunk, key head): K K^T and Q K^T of the chunk's rows, then per value head of the key head the
+// decay factors, P, and the inverse of 1 + A by forward substitution, a column of it per lane.
 template <int DK, bool BF16>
-void launch_steps(const FmGdn &a, const FmGdnSeqs &b, hipStream_t st) {
-    hipLaunchKernelGGL((fm_gdn_steps<DK, BF16, 1>), dim3(a.v_dim / 16, a.v_heads, b.n), dim3(256), 0, st, a, b);
+__global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *ws) {
+    constexpr int LD = DK + 4, LA = 68;      // rows 4 banks apart: 16 lanes' 16-byte reads do not collide
+    // K and Q [64][LD]; once their products are taken, A of each wave's head [4][64][LA]
+    constexpr int ROWS = 2 * 64 * LD > 4 * 64 * LA ? 2 * 64 * LD : 4 * 64 * LA;
+    __shared__ __attribute__((aligned(16))) float rows[ROWS], kk[64 * LA], qk[64 * LA], norm[2][64];
+    float *sk = rows, *sq = sk + 64 * LD;
+    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, r = lane & 15;
+    const int c = blockIdx.x, hk = blockIdx.y, s = fm_gdn_seq_of(b, c);
+    const int first = (c - b.chunk0[s]) * 64, n = min(64, b.rows[s] - first);
+    const int64_t row0 = b.row[s] + first;
+    const FmGdnWs w = fm_gdn_ws(a);
+    float *out = ws + (int64_t)c * w.floats;
+    for (int e = tid; e < 64 * (DK / 4); e += 256) {
+        const int i = e / (DK / 4), d = 4 * (e % (DK / 4));
+        fm_v4f k = {0.f, 0.f, 0.f, 0.f}, q = k;
+        if (i < n) {
+            k = fm_ld4<BF16>(a.k, (row0 + i) * a.k_stride + (int64_t)hk * DK + d);
+            q = fm_ld4<BF16>(a.q, (row0 + i) * a.q_stride + (int64_t)hk * DK + d);
+        }
+        *(fm_v4f *)(sk + i * LD + d) = k;
+        *(fm_v4f *)(sq + i * LD + d) = q;
+    }
+    __syncthreads();
+    // the 10 lower tiles of each product, five a wave
+    for (int t = wave * 5; t < wave * 5 + 5; t++) {
+        const int u = t % 10, i = u < 1 ? 0 : u < 3 ? 1 : u < 6 ? 2 : 3, j = u - i * (i + 1) / 2;
+        const float *x = (t < 10 ? sk : sq) + (16 * i + r) * LD + 4 * g, *y = sk + (16 * j + r) * LD + 4 * g;
+        fm_v4f c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
+#pragma unroll
+        for (int d = 0; d < DK; d += 32) {
+            c0 = mfma16(*(const fm_v4f *)(x + d), *(const fm_v4f *)(y + d), c0);
+            c1 = mfma16(*(const fm_v4f *)(x + d + 16), *(const fm_v4f *)(y + d + 16), c1);
+        }
+        float *z = (t < 10 ? kk : qk) + (16 * i + 4 * g) * LA + 16 * j + r;
+#pragma unroll
+        for (int e = 0; e < 4; e++) z[e * LA] = c0[e] + c1[e];
+    }
+    // K^T, four tokens of a dim per thread
+    float *kt = out + w.kt + (int64_t)hk * DK * 64;
+    for (int e = tid; e < DK * 16; e += 256) {
+        const int d = e / 16, i = 4 * (e % 16);
+        *(fm_v4f *)(kt + d * 64 + i) = fm_v4f{sk[i * LD + d], sk[(i + 1) * LD + d], sk[(i + 2) * LD + d], sk[(i + 3) * LD + d]};
+    }
+    // 1 / |k| and scale / |q|: two lanes a row and vector
+    {
+        const float *x = (tid < 128 ? sk : sq) + (tid & 127) / 2 * LD + (tid & 1) * (DK / 2);
+        float sum = 0.0f;
+        for (int d = 0; d < DK / 2; d += 4) {
+            const fm_v4f y = *(const fm_v4f *)(x + d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) sum = fmaf(y[e], y[e], sum);
+        }
+        sum = fm_group_sum<2>(sum);
+        const float inv = a.l2norm ? 1.0f / sqrtf(sum + 1e-6f) : 1.0f;
+        if (!(tid & 1)) norm[tid >> 7][(tid & 127) >> 1] = tid < 128 ? inv : a.scale * inv;
+    }
+    __syncthreads();
+    const int rep = a.v_heads / a.k_heads;
+    for (int hh = wave; hh < rep; hh += 4) {
+        const int h = hk * rep + hh;
+        float *am = rows + wave * 64 * LA;
+        const bool live = lane < n;
+        float gate = live ? a.g[(row0 + lane) * a.v_heads + h] : 0.0f;
+        const float beta = live ? a.beta[(row0 + lane) * a.v_heads + h] : 0.0f;
+        // e^-104 is 0 in fp32: a stronger decay, -inf included, is the same factor with finite sums
+        if (gate < -104.0f) gate = -104.0f;
+        double G = gate;
+        for (int o = 1; o < 64; o <<= 1) {
+            const double up = __shfl_up(G, o);
+            if (lane >= o) G += up;
+        }
+        const double end = __shfl(G, 63);
+        const float rk = norm[0][lane], rq = norm[1][lane];
+        // factors of a token: of v, of (K S), of u in the state's update, of (Q S)
+        float *sc = out + w.sc + (int64_t)h * 256;
+        const float eg = expf((float)G);
+        sc[lane] = beta;
+        sc[64 + lane] = beta * eg * rk;
+        sc[128 + lane] = live ? expf((float)(end - G)) * rk : 0.0f;
+        sc[192 + lane] = rq * eg;
+        if (lane == 63) out[w.end + h] = eg;
+        // row i of A and P, a column per lane
+        float *pm = out + w.p + (int64_t)h * 4096;
+        for (int i = 0; i < 64; i++) {
+            const float e = lane <= i ? expf((float)(__shfl(G, i) - G)) : 0.0f;
+            const float bi = __shfl(beta, i), ki = __shfl(rk, i), qi = __shfl(rq, i);
+            am[i * LA + lane] = lane < i ? bi * e * (kk[i * LA + lane] * (ki * rk)) : 0.0f;
+            pm[i * 64 + lane] = lane <= i ? e * (qk[i * LA + lane] * (qi * rk)) : 0.0f;
+        }
+        __builtin_amdgcn_wave_barrier();       // (one wave: its LDS accesses run in order)
+        float *tm = out + w.tm + (int64_t)h * 4096;
+        float t[64];
+#pragma unroll
+        for (int i = 0; i < 64; i++) {
+            float x = lane == i ? 1.0f : 0.0f, y = 0.0f;
+#pragma unroll
+            for (int m = 0; m < i; m += 4) {
+                const fm_v4f ai = *(const fm_v4f *)(am + i * LA + m);
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (m + e < i) (e & 1 ? y : x) = fmaf(-ai[e], t[m + e], e & 1 ? y : x);
+            }
+            t[i] = x + y;
+            tm[i * 64 + lane] = t[i];
+        }
+    }
+}
+
+// The chunks of a sequence in order, 16 value dims of one head per workgroup.  Wave w has the chunk's tokens
+// 16 w .. 16 w + 15 and, of the state [k_dim][16], the k rows (k_dim / 4) w ..; S, R and u pass
+// through LDS as [column][k or token], so that both the writers (four consecutive rows of a
+// result) and the readers (four consecutive k of an operand) move 16 bytes.
+template <int DK, bool BF16>
+__global__ __launch_bounds__(256, 1) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, const float *ws) {
+    constexpr int LS = DK + 4, LU = 68, ST = DK / 64;    // ST: state tiles of a wave
+    __shared__ __attribute__((aligned(16))) float ss[16 * LS], sr[16 * LU], su[16 * LU], sw[16 * LU];
+    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    const int h = blockIdx.x % a.v_heads, v0 = 16 * (blockIdx.x / a.v_heads), s = blockIdx.y;
+    const int hk = h / (a.v_heads / a.k_heads);
+    const FmGdnWs w = fm_gdn_ws(a);
+    const int T = b.rows[s], chunks = (T + 63) / 64;
+    // the state's rows [v_dim][k_dim] are the columns here
+    const int64_t st_at = ((int64_t)h * a.v_dim + v0 + r) * DK;
+    fm_v4f st[ST];
+#pragma unroll
+    for (int t = 0; t < ST; t++) {
+        const int k = (wave * ST + t) * 16 + 4 * g;
+        st[t] = b.in[s] ? *(const fm_v4f *)(b.in[s] + st_at + k) : fm_v4f{0.f, 0.f, 0.f, 0.f};
+        *(fm_v4f *)(ss + r * LS + k) = st[t];
+    }
+    struct Ops {
+        fm_v4f k[DK / 16], q[DK / 16], kt[ST][4], tm[4], p[4], beta, fk, fu, fq;
+        float v[4], decay;
+    };
+    auto load = [&](int c, Ops &o) {
+        const int n = min(64, T - 64 * c);
+        const int64_t row0 = b.row[s] + 64 * (int64_t)c;
+        const float *in = ws + (int64_t)(b.chunk0[s] + c) * w.floats;
+        const int tok = 16 * wave + r;
+#pragma unroll
+        for (int d = 0; d < DK / 16; d++) {
+            o.k[d] = o.q[d] = fm_v4f{0.f, 0.f, 0.f, 0.f};
+            if (tok < n) {
+                o.k[d] = fm_ld4<BF16>(a.k, (row0 + tok) * a.k_stride + (int64_t)hk * DK + 16 * d + 4 * g);
+                o.q[d] = fm_ld4<BF16>(a.q, (row0 + tok) * a.q_stride + (int64_t)hk * DK + 16 * d + 4 * g);
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < ST; t++)
+#pragma unroll
+            for (int j = 0; j < 4; j++)
+                o.kt[t][j] = *(const fm_v4f *)(in + w.kt + ((int64_t)hk * DK + (wave * ST + t) * 16 + r) * 64 + 16 * j + 4 * g);
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (j <= wave) {       // (lower triangular: later tokens' tiles are zero)
+                o.tm[j] = *(const fm_v4f *)(in + w.tm + (int64_t)h * 4096 + tok * 64 + 16 * j + 4 * g);
+                o.p[j] = *(const fm_v4f *)(in + w.p + (int64_t)h * 4096 + tok * 64 + 16 * j + 4 * g);
+            }
+        const float *sc = in + w.sc + (int64_t)h * 256 + 16 * wave + 4 * g;
+        o.beta = *(const fm_v4f *)sc;
+        o.fk = *(const fm_v4f *)(sc + 64);
+        o.fu = *(const fm_v4f *)(sc + 128);
+        o.fq = *(const fm_v4f *)(sc + 192);
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const int t = 16 * wave + 4 * g + i;
+            o.v[i] = t < n ? fm_ld1<BF16>(a.v, (row0 + t) * a.v_stride + (int64_t)h * a.v_dim + v0 + r) : 0.0f;
+        }
+        o.decay = in[w.end + h];
+    };
+    Ops o, nx;
+    if (chunks > 0) load(0, o);
+    for (int c = 0; c < chunks; c++) {
+        const int n = min(64, T - 64 * c);
+        if (c + 1 < chunks) load(c + 1, nx);
+        const fm_v4f zero = {0.f, 0.f, 0.f, 0.f};
+        fm_v4f ks0 = zero, ks1 = zero, qs0 = zero, qs1 = zero;
+        __syncthreads();                                   // S is there
+#pragma unroll
+        for (int d = 0; d < DK / 16; d += 2) {
+            const fm_v4f s0 = *(const fm_v4f *)(ss + r * LS + 16 * d + 4 * g), s1 = *(const fm_v4f *)(ss + r * LS + 16 * d + 16 + 4 * g);
+            ks0 = mfma16(o.k[d], s0, ks0);
+            qs0 = mfma16(o.q[d], s0, qs0);
+            ks1 = mfma16(o.k[d + 1], s1, ks1);
+            qs1 = mfma16(o.q[d + 1], s1, qs1);
+        }
+        fm_v4f x;
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = o.beta[i] * o.v[i] - o.fk[i] * (ks0[i] + ks1[i]);
+        *(fm_v4f *)(sr + r * LU + 16 * wave + 4 * g) = x;
+        __syncthreads();                                   // R is there, S has been read
+        fm_v4f u0 = zero, u1 = zero;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (j <= wave) {
+                const fm_v4f y = *(const fm_v4f *)(sr + r * LU + 16 * j + 4 * g);
+                if (j & 1) u1 = mfma16(o.tm[j], y, u1);
+                else u0 = mfma16(o.tm[j], y, u0);
+            }
+        u0 += u1;
+        *(fm_v4f *)(su + r * LU + 16 * wave + 4 * g) = u0;
+        *(fm_v4f *)(sw + r * LU + 16 * wave + 4 * g) = u0 * o.fu;
+        __syncthreads();                                   // u is there
+#pragma unroll
+        for (int t = 0; t < ST; t++) {
+            fm_v4f z0 = st[t] * o.decay, z1 = zero;
+#pragma unroll
+            for (int j = 0; j < 4; j += 2) {
+                z0 = mfma16(o.kt[t][j], *(const fm_v4f *)(sw + r * LU + 16 * j + 4 * g), z0);
+                z1 = mfma16(o.kt[t][j + 1], *(const fm_v4f *)(sw + r * LU + 16 * j + 16 + 4 * g), z1);
+            }
+            st[t] = z0 + z1;
+            *(fm_v4f *)(ss + r * LS + (wave * ST + t) * 16 + 4 * g) = st[t];
+        }
+        fm_v4f y0 = o.fq * (qs0 + qs1), y1 = zero;
+#pragma unroll
+        for (int j = 0; j < 4; j++)
+            if (j <= wave) {
+                const fm_v4f y = *(const fm_v4f *)(su + r * LU + 16 * j + 4 * g);
+                if (j & 1) y1 = mfma16(o.p[j], y, y1);
+                else y0 = mfma16(o.p[j], y, y0);
+            }
+        y0 += y1;
+        const int64_t row0 = b.row[s] + 64 * (int64_t)c + 16 * wave + 4 * g;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+            if (16 * wave + 4 * g + i < n) fm_st1<BF16>(a.out, ((row0 + i) * a.v_heads + h) * a.v_dim + v0 + r, y0[i]);
+        if (c + 1 < chunks) o = nx;
+    }
+#pragma unroll
+    for (int t = 0; t < ST; t++) *(fm_v4f *)(b.out[s] + st_at + (wave * ST + t) * 16 + 4 * g) = st[t];
+}
+
+template <int DK, bool BF16>
+int launch_seqs(const FmGdn &a, const FmGdnSeqs &b, int chunked, float *ws, hipStream_t st) {
+    if (!chunked) {
+        hipLaunchKernelGGL((fm_gdn_steps<DK, BF16, 1>), dim3(a.v_dim / 16, a.v_heads, b.n), dim3(256), 0, st, a, b);
+    } else {
+        hipLaunchKernelGGL((fm_gdn_prep<DK, BF16>), dim3(b.chunk0[b.n], a.k_heads), dim3(256), 0, st, a, b, ws);
+        hipLaunchKernelGGL((fm_gdn_scan<DK, BF16>), dim3(a.v_heads * (a.v_dim / 16), b.n), dim3(256), 0, st, a, b, ws);
+    }
+    return hipGetLastError() == hipSuccess ? FM_OK : FM_ERR_HIP;
 }
 
 }  // namespace
 
-extern "C" size_t fm_gdn_ws_bytes(const FmGdn *, const int *, int) { return 0; }
-
 // start: n_seq + 1 row numbers (null: one row per sequence); in, out: n_seq state pointers
 extern "C" int fm_launch_gdn(const FmGdn *a, int bf16, const int *start, int n_seq, const float *const *in,
-                             float *const *out, void *ws, int n_cu, hipStream_t st) {
-    (void)ws; (void)n_cu;
-    for (int first = 0; first < n_seq; first += FM_GDN_SEQS) {
-        FmGdnSeqs b;
-        b.n = n_seq - first < FM_GDN_SEQS ? n_seq - first : FM_GDN_SEQS;
-        for (int i = 0; i <= b.n; i++) b.start[i] = start ? start[first + i] : first + i;
-        for (int i = 0; i < b.n; i++) {
-            b.in[i] = in ? in[first + i] : nullptr;
-            b.out[i] = out[first + i];
-        }
-        if (a->k_dim == 128) {
-            if (bf16) launch_steps<128, true>(*a, b, st);
-            else launch_steps<128, false>(*a, b, st);
-        } else {
-            if (bf16) launch_steps<64, true>(*a, b, st);
-            else launch_steps<64, false>(*a, b, st);
-        }
-        if (hipGetLastError() != hipSuccess) return FM_ERR_HIP;
+                             float *const *out, void *ws, hipStream_t st) {
+    FmGdnPlan plan{a, start, n_seq, in, out};
+    FmGdnSeqs b;
+    int chunked;
+    while (plan.next(&b, &chunked)) {
+        int rc;
+        if (a->k_dim == 128) rc = bf16 ? launch_seqs<128, true>(*a, b, chunked, (float *)ws, st) : launch_seqs<128, false>(*a, b, chunked, (float *)ws, st);
+        else rc = bf16 ? launch_seqs<64, true>(*a, b, chunked, (float *)ws, st) : launch_seqs<64, false>(*a, b, chunked, (float *)ws, st);
+        if (rc) return rc;
     }
     return FM_OK;
 }

@@ -37,14 +37,115 @@ struct FmGdn {
     void *out;
 };
 
-// The sequences of one launch, by value: 128 of them are 2.6 KB of kernel arguments.
+// The sequences of one launch, by value: 128 of them are 3.6 KB of kernel arguments.  The launch
+// runs rows row[i] .. row[i] + rows[i] - 1; chunk0[i]: chunks of the sequences before (chunked form).
 #define FM_GDN_SEQS 128
 struct FmGdnSeqs {
     int n;
-    int start[FM_GDN_SEQS + 1];
+    int row[FM_GDN_SEQS], rows[FM_GDN_SEQS], chunk0[FM_GDN_SEQS + 1];
     const float *in[FM_GDN_SEQS];
     float *out[FM_GDN_SEQS];
 };
+// the sequence that chunk `c` of the launch belongs to
+FM_HD int fm_gdn_seq_of(const FmGdnSeqs &b, int c) {
+    int lo = 0, hi = b.n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (b.chunk0[mid] <= c) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+#define FM_GDN_CHUNK 64
+// Sequences of fewer rows run token by token.
+#define FM_GDN_MIN_CHUNKED 24
+// What the chunked form keeps per chunk between its two kernels, in floats:
+//   kt [k_heads][k_dim][64] | tm [v_heads][64][64] | p [v_heads][64][64] | sc [v_heads][4][64] |
+//   end [v_heads], to a multiple of 64
+struct FmGdnWs {
+    int64_t kt, tm, p, sc, end, floats;
+};
+FM_HD FmGdnWs fm_gdn_ws(const FmGdn &a) {
+    FmGdnWs w;
+    w.kt = 0;
+    w.tm = (int64_t)a.k_heads * a.k_dim * 64;
+    w.p = w.tm + (int64_t)a.v_heads * 4096;
+    w.sc = w.p + (int64_t)a.v_heads * 4096;
+    w.end = w.sc + (int64_t)a.v_heads * 256;
+    w.floats = w.end + (a.v_heads + 63) / 64 * 64;
+    return w;
+}
+// Chunks of one pass over the sequences: as many of each as keep the workspace near 192 MB, where
+// the last-level cache still holds it between the two kernels.
+inline int fm_gdn_window(const FmGdn &a, int n_seq) {
+    const int64_t per = fm_gdn_ws(a).floats * 4;
+    const int64_t n = ((int64_t)192 << 20) / per / (n_seq < 1 ? 1 : n_seq);
+    return n < 1 ? 1 : n > 1024 ? 1024 : (int)n;
+}
+// The launches of a call, in order: plan(i, &seqs) fills the i-th, false when there are no more.  The first
+// are those of the short sequences.
+struct FmGdnPlan {
+    const FmGdn *a;
+    const int *start;
+    int n_seq;
+    const float *const *in;
+    float *const *out;
+    int at = 0;          // next sequence to look at
+    int pass = 0;        // 0: short sequences, 1: chunked
+    int done = 0;        // chunks of the group in hand that have run
+    int group0 = 0;      // its first sequence
+    int rows(int i) const { return start ? start[i + 1] - start[i] : 1; }
+    bool next(FmGdnSeqs *b, int *chunked) {
+        b->n = 0;
+        if (pass == 0) {
+            for (; at < n_seq && b->n < FM_GDN_SEQS; at++)
+                if (rows(at) < FM_GDN_MIN_CHUNKED) put(b, at, 0, rows(at), true);
+            *chunked = 0;
+            if (b->n) return true;
+            pass = 1;
+            at = 0;
+        }
+        *chunked = 1;
+        for (;;) {
+            // a group: up to FM_GDN_SEQS long sequences, run window by window
+            int n_long = 0, end = group0;
+            for (; end < n_seq && n_long < FM_GDN_SEQS; end++) n_long += rows(end) >= FM_GDN_MIN_CHUNKED;
+            if (!n_long) return false;
+            const int win = fm_gdn_window(*a, n_long) * FM_GDN_CHUNK;
+            b->n = 0;
+            for (int i = group0; i < end; i++) {
+                const int left = rows(i) - done;
+                if (rows(i) >= FM_GDN_MIN_CHUNKED && left > 0) put(b, i, done, left < win ? left : win, done == 0);
+            }
+            if (b->n) {
+                done += win;
+                return true;
+            }
+            group0 = end;
+            done = 0;
+        }
+    }
+    void put(FmGdnSeqs *b, int i, int first, int n, bool fresh) {
+        const int k = b->n++;
+        b->row[k] = (start ? start[i] : i) + first;
+        b->rows[k] = n;
+        if (!k) b->chunk0[0] = 0;
+        b->chunk0[k + 1] = b->chunk0[k] + (n + FM_GDN_CHUNK - 1) / FM_GDN_CHUNK;
+        b->in[k] = fresh ? (in ? in[i] : nullptr) : out[i];
+        b->out[k] = out[i];
+    }
+};
+// workspace of a call: that of its largest launch
+inline size_t fm_gdn_ws_bytes(const FmGdn *a, const int *start, int n_seq) {
+    float *none[FM_MAX_SEQ] = {};
+    FmGdnPlan plan{a, start, n_seq, nullptr, none};
+    FmGdnSeqs b;
+    int chunked, most = 0;
+    while (plan.next(&b, &chunked))
+        if (chunked && b.chunk0[b.n] > most) most = b.chunk0[b.n];
+    return (size_t)most * fm_gdn_ws(*a).floats * sizeof(float);
+}
 
 struct FmKv {
     int8_t *k, *v;

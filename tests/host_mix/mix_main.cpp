@@ -246,7 +246,46 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
     }
 }
 
+// ---- the gated delta rule's launches: every row runs once, in order, and the workspace holds a launch
+static void plan_gdn() {
+    for (int round = 0; round < 3000; round++) {
+        FmGdn a{};
+        a.k_heads = 1 + rnd(16), a.v_heads = a.k_heads * (1 + rnd(3)), a.k_dim = rnd(2) ? 64 : 128, a.v_dim = 128;
+        const int n = 1 + rnd(rnd(4) ? 6 : FM_MAX_SEQ);
+        std::vector<int> start(n + 1, 0);
+        for (int i = 0; i < n; i++) start[i + 1] = start[i] + (rnd(3) ? rnd(60) : rnd(65536 / n));
+        std::vector<float *> in(n), out(n);
+        std::vector<int> next(n, 0);
+        for (int i = 0; i < n; i++) in[i] = (float *)at(4096 + 64 * i), out[i] = (float *)at(1 << 20 | 64 * i);
+        FmGdnPlan plan{&a, start.data(), n, in.data(), out.data()};
+        FmGdnSeqs b;
+        int chunked;
+        const size_t ws = fm_gdn_ws_bytes(&a, start.data(), n);
+        while (plan.next(&b, &chunked)) {
+            CHECK(b.n >= 1 && b.n <= FM_GDN_SEQS);
+            for (int k = 0; k < b.n; k++) {
+                const int i = (int)(((uintptr_t)b.out[k] & ((1 << 20) - 1)) / 64);
+                CHECK(b.row[k] == start[i] + next[i] && b.in[k] == (next[i] ? out[i] : in[i]));
+                CHECK(b.row[k] + b.rows[k] <= start[i + 1]);
+                CHECK(chunked == (start[i + 1] - start[i] >= FM_GDN_MIN_CHUNKED));
+                CHECK(!chunked || b.rows[k] % FM_GDN_CHUNK == 0 || b.row[k] + b.rows[k] == start[i + 1]);
+                next[i] += b.rows[k] ? b.rows[k] : -1;      // (an empty sequence runs once, its state is copied)
+                for (int c = b.chunk0[k]; c < b.chunk0[k + 1]; c++) CHECK(fm_gdn_seq_of(b, c) == k);
+            }
+            if (chunked) CHECK((size_t)b.chunk0[b.n] * fm_gdn_ws(a).floats * 4 <= ws);
+        }
+        for (int i = 0; i < n; i++) CHECK(next[i] == (start[i + 1] > start[i] ? start[i + 1] - start[i] : -1));
+    }
+    FmGdn a{};
+    a.k_heads = 16, a.v_heads = 32, a.k_dim = a.v_dim = 128;
+    CHECK(fm_gdn_ws_bytes(&a, nullptr, 200) == 0);
+    const FmGdnWs w = fm_gdn_ws(a);
+    CHECK(w.tm % 4 == 0 && w.p % 4 == 0 && w.sc % 4 == 0 && w.floats % 4 == 0 && w.end + a.v_heads <= w.floats);
+    CHECK(sizeof(FmGdnSeqs) + sizeof(FmGdn) + 8 <= 4096 && sizeof(FmSeqs) + sizeof(FmKv) + sizeof(FmAttn) <= 4096);
+}
+
 int main() {
+    plan_gdn();
     refuse_gdn();
     refuse_cache();
     refuse_logprobs();

@@ -68,7 +68,7 @@ SHAPES = [(1, 1, 64, 16), (2, 4, 128, 128), (1, 3, 64, 80), (2, 2, 128, 256), (4
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
 @pytest.mark.parametrize("hk,hv,dk,dv", SHAPES)
-@pytest.mark.parametrize("lens", [[1], [1, 1, 1], [2], [5, 0, 1], [63], [64], [65], [130, 17], [200]])
+@pytest.mark.parametrize("lens", [[1], [1, 1, 1], [2], [5, 0, 1], [23], [24], [63], [64], [65], [130, 17], [200]])
 def test_against_the_recurrence(hip, lens, hk, hv, dk, dv, dtype):
     import torch
     dt = getattr(torch, dtype)
@@ -181,6 +181,20 @@ def test_many_sequences_in_several_launches(hip):
     ref, ref_s = R.gated_delta(q, k, v, gate, beta, state, lens, 1.0, True)
     got, new = _call(hip, rows, gate, beta, state, lens, hk, hv, dk, dv, True, 1.0)
     _check(got, new, ref, ref_s, lens, dk, False, "256 sequences")
+
+
+def test_windows_of_chunks(hip):
+    """more chunks than one pass over the workspace holds: 40 sequences of 32 heads, three chunks each a pass"""
+    import torch
+    hk, hv, dk, dv = 16, 32, 128, 16
+    lens = [100 + 5 * i for i in range(38)] + [7, 64]
+    rows, gate, beta, state = _inputs(16, lens, hk, hv, dk, dv, torch.float32)
+    q, k, v = _split(rows, hk, hv, dk, dv)
+    ref, ref_s = R.gated_delta(q, k, v, gate, beta, state, lens, 1.0, True)
+    got, new = _call(hip, rows, gate, beta, state, lens, hk, hv, dk, dv, True, 1.0)
+    _check(got, new, ref, ref_s, lens, dk, False, "windows")
+    got, new = _call(hip, rows, gate, beta, state, lens, hk, hv, dk, dv, True, 1.0, in_place=True)
+    _check(got, new, ref, ref_s, lens, dk, False, "windows, in place")
 
 
 def test_step_after_step_equals_the_prompt(hip):
