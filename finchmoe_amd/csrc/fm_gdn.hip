@@ -131,52 +131,59 @@ __device__ __forceinline__ fm_v4f mfma16(fm_v4f x, fm_v4f y, fm_v4f c) {
     return c;
 }
 
+// Barrier behind this wave's LDS writes that leaves loads from memory in flight.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+}
+
+__device__ __forceinline__ double lane_of(double v, int lane) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ float lane_of(float v, int lane) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
+}
+
 // Per (chunk, key head): K K^T and Q K^T of the chunk's rows, then per value head of the key head the
-// decay factors, P, and the inverse of 1 + A by forward substitution, a column of it per lane.
+// decay factors, P, and T = (1 + A)^-1.  T in 16 x 16 blocks: the diagonal ones by forward substitution,
+// a column per lane; below them, block column by block column,
+//   T_ij = -T_ii sum_{j <= m < i} A_im T_mj,
+// where a product's result registers are the next one's right operand as they are (lane 16 g + c has
+// rows 4 g .. 4 g + 3 of column c in both), so a block column never leaves its wave's registers.
 template <int DK, bool BF16>
 __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *ws) {
     constexpr int LD = DK + 4, LA = 68;      // rows 4 banks apart: 16 lanes' 16-byte reads do not collide
-    // K and Q [64][LD]; once their products are taken, A of each wave's head [4][64][LA]
+    // K and Q [64][LD], then K K^T, Q K^T, A (T in its place) and P [64][LA]
     constexpr int ROWS = 2 * 64 * LD > 4 * 64 * LA ? 2 * 64 * LD : 4 * 64 * LA;
-    __shared__ __attribute__((aligned(16))) float rows[ROWS], kk[64 * LA], qk[64 * LA], norm[2][64];
-    float *sk = rows, *sq = sk + 64 * LD;
-    const int tid = threadIdx.x, wave = tid >> 6, lane = tid & 63, g = lane >> 4, r = lane & 15;
+    __shared__ __attribute__((aligned(16))) float lds[ROWS];
+    __shared__ float norm[2][64];
+    float *sk = lds, *sq = lds + 64 * LD, *kk = lds, *qk = lds + 64 * LA, *am = lds + 2 * 64 * LA, *pm = lds + 3 * 64 * LA;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, g = lane >> 4, r = lane & 15;
     const int c = blockIdx.x, hk = blockIdx.y, s = fm_gdn_seq_of(b, c);
     const int first = (c - b.chunk0[s]) * 64, n = min(64, b.rows[s] - first);
     const int64_t row0 = b.row[s] + first;
     const FmGdnWs w = fm_gdn_ws(a);
     float *out = ws + (int64_t)c * w.floats;
-    for (int e = tid; e < 64 * (DK / 4); e += 256) {
-        const int i = e / (DK / 4), d = 4 * (e % (DK / 4));
-        fm_v4f k = {0.f, 0.f, 0.f, 0.f}, q = k;
-        if (i < n) {
-            k = fm_ld4<BF16>(a.k, (row0 + i) * a.k_stride + (int64_t)hk * DK + d);
-            q = fm_ld4<BF16>(a.q, (row0 + i) * a.q_stride + (int64_t)hk * DK + d);
+    {
+        constexpr int PER = DK / 16;         // float4 of K (and of Q) a thread
+        fm_v4f x[2][PER];
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            const int e = tid + 256 * u, i = e / (DK / 4), d = 4 * (e % (DK / 4));
+            const int64_t row = row0 + min(i, n - 1);
+            x[0][u] = fm_ld4<BF16>(a.k, row * a.k_stride + (int64_t)hk * DK + d);
+            x[1][u] = fm_ld4<BF16>(a.q, row * a.q_stride + (int64_t)hk * DK + d);
         }
-        *(fm_v4f *)(sk + i * LD + d) = k;
-        *(fm_v4f *)(sq + i * LD + d) = q;
+#pragma unroll
+        for (int u = 0; u < PER; u++) {
+            const int e = tid + 256 * u, i = e / (DK / 4), d = 4 * (e % (DK / 4));
+            const fm_v4f zero = {0.f, 0.f, 0.f, 0.f};
+            *(fm_v4f *)(sk + i * LD + d) = i < n ? x[0][u] : zero;
+            *(fm_v4f *)(sq + i * LD + d) = i < n ? x[1][u] : zero;
+        }
     }
     __syncthreads();
-    // the 10 lower tiles of each product, five a wave
-    for (int t = wave * 5; t < wave * 5 + 5; t++) {
-        const int u = t % 10, i = u < 1 ? 0 : u < 3 ? 1 : u < 6 ? 2 : 3, j = u - i * (i + 1) / 2;
-        const float *x = (t < 10 ? sk : sq) + (16 * i + r) * LD + 4 * g, *y = sk + (16 * j + r) * LD + 4 * g;
-        fm_v4f c0 = {0.f, 0.f, 0.f, 0.f}, c1 = c0;
-#pragma unroll
-        for (int d = 0; d < DK; d += 32) {
-            c0 = mfma16(*(const fm_v4f *)(x + d), *(const fm_v4f *)(y + d), c0);
-            c1 = mfma16(*(const fm_v4f *)(x + d + 16), *(const fm_v4f *)(y + d + 16), c1);
-        }
-        float *z = (t < 10 ? kk : qk) + (16 * i + 4 * g) * LA + 16 * j + r;
-#pragma unroll
-        for (int e = 0; e < 4; e++) z[e * LA] = c0[e] + c1[e];
-    }
-    // K^T, four tokens of a dim per thread
-    float *kt = out + w.kt + (int64_t)hk * DK * 64;
-    for (int e = tid; e < DK * 16; e += 256) {
-        const int d = e / 16, i = 4 * (e % 16);
-        *(fm_v4f *)(kt + d * 64 + i) = fm_v4f{sk[i * LD + d], sk[(i + 1) * LD + d], sk[(i + 2) * LD + d], sk[(i + 3) * LD + d]};
-    }
     // 1 / |k| and scale / |q|: two lanes a row and vector
     {
         const float *x = (tid < 128 ? sk : sq) + (tid & 127) / 2 * LD + (tid & 1) * (DK / 2);
@@ -190,54 +197,132 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
         const float inv = a.l2norm ? 1.0f / sqrtf(sum + 1e-6f) : 1.0f;
         if (!(tid & 1)) norm[tid >> 7][(tid & 127) >> 1] = tid < 128 ? inv : a.scale * inv;
     }
+    // the 10 lower tiles of each product, five a wave
+    fm_v4f prod[5];
+#pragma unroll
+    for (int t = 0; t < 5; t++) {
+        const int u = (wave * 5 + t) % 10, i = u < 1 ? 0 : u < 3 ? 1 : u < 6 ? 2 : 3, j = u - i * (i + 1) / 2;
+        const float *x = (wave < 2 ? sk : sq) + (16 * i + r) * LD + 4 * g, *y = sk + (16 * j + r) * LD + 4 * g;
+        fm_v4f z[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) z[e] = fm_v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int d = 0; d < DK; d += 16) {
+            const fm_v4f p = *(const fm_v4f *)(x + d), q = *(const fm_v4f *)(y + d);
+#pragma unroll
+            for (int e = 0; e < 4; e++) z[e] = mfma4(p[e], q[e], z[e]);
+        }
+        prod[t] = (z[0] + z[1]) + (z[2] + z[3]);
+    }
+    // K, Q and K^T in the order of the second kernel
+    {
+        float *k = out + w.k + (int64_t)hk * DK * 64, *q = out + w.q + (int64_t)hk * DK * 64, *kt = out + w.kt + (int64_t)hk * DK * 64;
+#pragma unroll
+        for (int d = 0; d < DK / 16; d++) {
+            const int at = (wave * (DK / 16) + d) * FM_GDN_TILE + 4 * lane;
+            *(fm_v4f *)(k + at) = *(const fm_v4f *)(sk + (16 * wave + r) * LD + 16 * d + 4 * g);
+            *(fm_v4f *)(q + at) = *(const fm_v4f *)(sq + (16 * wave + r) * LD + 16 * d + 4 * g);
+        }
+#pragma unroll
+        for (int u = 0; u < DK / 16; u++) {      // tile u * 4 + wave: k rows 16 u .., tokens 16 wave ..
+            const float *x = sk + (16 * wave + 4 * g) * LD + 16 * u + r;
+            *(fm_v4f *)(kt + (u * 4 + wave) * FM_GDN_TILE + 4 * lane) = fm_v4f{x[0], x[LD], x[2 * LD], x[3 * LD]};
+        }
+    }
     __syncthreads();
+#pragma unroll
+    for (int t = 0; t < 5; t++) {
+        const int u = (wave * 5 + t) % 10, i = u < 1 ? 0 : u < 3 ? 1 : u < 6 ? 2 : 3, j = u - i * (i + 1) / 2;
+        float *z = (wave < 2 ? kk : qk) + (16 * i + 4 * g) * LA + 16 * j + r;
+#pragma unroll
+        for (int e = 0; e < 4; e++) z[e * LA] = prod[t][e];
+    }
+    const float rk = norm[0][lane], rq = norm[1][lane];
     const int rep = a.v_heads / a.k_heads;
-    for (int hh = wave; hh < rep; hh += 4) {
+    for (int hh = 0; hh < rep; hh++) {
         const int h = hk * rep + hh;
-        float *am = rows + wave * 64 * LA;
-        const bool live = lane < n;
-        float gate = live ? a.g[(row0 + lane) * a.v_heads + h] : 0.0f;
-        const float beta = live ? a.beta[(row0 + lane) * a.v_heads + h] : 0.0f;
+        const int64_t at = (row0 + min(lane, n - 1)) * a.v_heads + h;
+        float gate = a.g[at], beta = a.beta[at];
+        if (lane >= n) gate = beta = 0.0f;
         // e^-104 is 0 in fp32: a stronger decay, -inf included, is the same factor with finite sums
         if (gate < -104.0f) gate = -104.0f;
         double G = gate;
+#pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const double up = __shfl_up(G, o);
             if (lane >= o) G += up;
         }
-        const double end = __shfl(G, 63);
-        const float rk = norm[0][lane], rq = norm[1][lane];
-        // factors of a token: of v, of (K S), of u in the state's update, of (Q S)
-        float *sc = out + w.sc + (int64_t)h * 256;
-        const float eg = expf((float)G);
-        sc[lane] = beta;
-        sc[64 + lane] = beta * eg * rk;
-        sc[128 + lane] = live ? expf((float)(end - G)) * rk : 0.0f;
-        sc[192 + lane] = rq * eg;
-        if (lane == 63) out[w.end + h] = eg;
-        // row i of A and P, a column per lane
-        float *pm = out + w.p + (int64_t)h * 4096;
-        for (int i = 0; i < 64; i++) {
-            const float e = lane <= i ? expf((float)(__shfl(G, i) - G)) : 0.0f;
-            const float bi = __shfl(beta, i), ki = __shfl(rk, i), qi = __shfl(rq, i);
-            am[i * LA + lane] = lane < i ? bi * e * (kk[i * LA + lane] * (ki * rk)) : 0.0f;
-            pm[i * 64 + lane] = lane <= i ? e * (qk[i * LA + lane] * (qi * rk)) : 0.0f;
+        if (wave == 0) {
+            // factors of a token: of v, of (K S), of u in the state's update, of (Q S)
+            float *sc = out + w.sc + (int64_t)h * 256;
+            const float eg = expf((float)G);
+            sc[lane] = beta;
+            sc[64 + lane] = beta * eg * rk;
+            sc[128 + lane] = lane < n ? expf((float)(lane_of(G, 63) - G)) * rk : 0.0f;
+            sc[192 + lane] = rq * eg;
+            if (lane == 63) out[w.end + h] = eg;
         }
-        __builtin_amdgcn_wave_barrier();       // (one wave: its LDS accesses run in order)
-        float *tm = out + w.tm + (int64_t)h * 4096;
-        float t[64];
+        __syncthreads();                       // the products are there; the last head's T and P are out
+        // rows 16 wave .. of A and P, a column per lane
+        for (int ii = 0; ii < 16; ii++) {
+            const int i = 16 * wave + ii;
+            const float e = lane <= i ? expf((float)(lane_of(G, i) - G)) : 0.0f;
+            const float bi = lane_of(beta, i), ki = lane_of(rk, i), qi = lane_of(rq, i);
+            am[i * LA + lane] = lane < i ? bi * e * (kk[i * LA + lane] * (ki * rk)) : 0.0f;
+            pm[i * LA + lane] = lane <= i ? e * (qk[i * LA + lane] * (qi * rk)) : 0.0f;
+        }
+        __syncthreads();
+        if (wave == 3) {
+            // diagonal blocks: lane 16 g + r solves column r of block g
+            float *d = am + 16 * g * LA + 16 * g;
+            float t[16];
 #pragma unroll
-        for (int i = 0; i < 64; i++) {
-            float x = lane == i ? 1.0f : 0.0f, y = 0.0f;
+            for (int i = 0; i < 16; i++) {
+                float x = r == i ? 1.0f : 0.0f;
 #pragma unroll
-            for (int m = 0; m < i; m += 4) {
-                const fm_v4f ai = *(const fm_v4f *)(am + i * LA + m);
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (m + e < i) (e & 1 ? y : x) = fmaf(-ai[e], t[m + e], e & 1 ? y : x);
+                for (int m = 0; m < i; m++) x = fmaf(-d[i * LA + m], t[m], x);
+                t[i] = x;
             }
-            t[i] = x + y;
-            tm[i * 64 + lane] = t[i];
+            __builtin_amdgcn_wave_barrier();   // (one wave: its LDS accesses run in order)
+#pragma unroll
+            for (int i = 0; i < 16; i++) d[i * LA + r] = t[i];
+        }
+        __syncthreads();
+        if (wave < 3) {
+            // block column `wave`
+            fm_v4f t[4];
+            const float *d = am + (16 * wave + 4 * g) * LA + 16 * wave + r;
+#pragma unroll
+            for (int i = 0; i < 4; i++) t[i] = fm_v4f{0.f, 0.f, 0.f, 0.f};
+            const fm_v4f diag = {d[0], d[LA], d[2 * LA], d[3 * LA]};
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (i == wave) t[i] = diag;
+                if (i <= wave) continue;
+                fm_v4f x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int m = 0; m < i; m++)
+                    if (m >= wave) x = mfma16(*(const fm_v4f *)(am + (16 * i + r) * LA + 16 * m + 4 * g), t[m], x);
+                t[i] = -mfma16(*(const fm_v4f *)(am + (16 * i + r) * LA + 16 * i + 4 * g), x, fm_v4f{0.f, 0.f, 0.f, 0.f});
+            }
+            lds_barrier();                     // every wave has read A
+#pragma unroll
+            for (int i = 1; i < 4; i++)
+                if (i > wave) {
+                    float *z = am + (16 * i + 4 * g) * LA + 16 * wave + r;
+#pragma unroll
+                    for (int e = 0; e < 4; e++) z[e * LA] = t[i][e];
+                }
+        } else {
+            lds_barrier();
+        }
+        __syncthreads();
+        float *tm = out + w.tm + (int64_t)h * 10 * FM_GDN_TILE, *po = out + w.p + (int64_t)h * 10 * FM_GDN_TILE;
+#pragma unroll
+        for (int u = 0; u < 5; u++) {
+            const int t = wave + 4 * u, v = t % 10, i = v < 1 ? 0 : v < 3 ? 1 : v < 6 ? 2 : 3, j = v - i * (i + 1) / 2;
+            *(fm_v4f *)((t < 10 ? tm : po) + v * FM_GDN_TILE + 4 * lane) =
+                *(const fm_v4f *)((t < 10 ? am : pm) + (16 * i + r) * LA + 16 * j + 4 * g);
         }
     }
 }
@@ -250,7 +335,7 @@ template <int DK, bool BF16>
 __global__ __launch_bounds__(256, 1) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, const float *ws) {
     constexpr int LS = DK + 4, LU = 68, ST = DK / 64;    // ST: state tiles of a wave
     __shared__ __attribute__((aligned(16))) float ss[16 * LS], sr[16 * LU], su[16 * LU], sw[16 * LU];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const int h = blockIdx.x % a.v_heads, v0 = 16 * (blockIdx.x / a.v_heads), s = blockIdx.y;
     const int hk = h / (a.v_heads / a.k_heads);
     const FmGdnWs w = fm_gdn_ws(a);
@@ -268,100 +353,115 @@ __global__ __launch_bounds__(256, 1) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, cons
         fm_v4f k[DK / 16], q[DK / 16], kt[ST][4], tm[4], p[4], beta, fk, fu, fq;
         float v[4], decay;
     };
+    // Every load of a chunk is issued on every path (rows behind the last one as that one, tiles above
+    // the diagonal as that one: what they give is dropped): a load that some path skips would make
+    // the compiler wait for all of them.
     auto load = [&](int c, Ops &o) {
         const int n = min(64, T - 64 * c);
         const int64_t row0 = b.row[s] + 64 * (int64_t)c;
         const float *in = ws + (int64_t)(b.chunk0[s] + c) * w.floats;
-        const int tok = 16 * wave + r;
+        const float *k = in + (int64_t)hk * DK * 64 + wave * (DK / 16) * FM_GDN_TILE + 4 * lane;
 #pragma unroll
         for (int d = 0; d < DK / 16; d++) {
-            o.k[d] = o.q[d] = fm_v4f{0.f, 0.f, 0.f, 0.f};
-            if (tok < n) {
-                o.k[d] = fm_ld4<BF16>(a.k, (row0 + tok) * a.k_stride + (int64_t)hk * DK + 16 * d + 4 * g);
-                o.q[d] = fm_ld4<BF16>(a.q, (row0 + tok) * a.q_stride + (int64_t)hk * DK + 16 * d + 4 * g);
-            }
+            o.k[d] = *(const fm_v4f *)(k + w.k + d * FM_GDN_TILE);
+            o.q[d] = *(const fm_v4f *)(k + w.q + d * FM_GDN_TILE);
         }
+        const float *kt = in + w.kt + (int64_t)hk * DK * 64 + wave * ST * 4 * FM_GDN_TILE + 4 * lane;
 #pragma unroll
         for (int t = 0; t < ST; t++)
 #pragma unroll
-            for (int j = 0; j < 4; j++)
-                o.kt[t][j] = *(const fm_v4f *)(in + w.kt + ((int64_t)hk * DK + (wave * ST + t) * 16 + r) * 64 + 16 * j + 4 * g);
+            for (int j = 0; j < 4; j++) o.kt[t][j] = *(const fm_v4f *)(kt + (t * 4 + j) * FM_GDN_TILE);
+        const float *low = in + (int64_t)h * 10 * FM_GDN_TILE + fm_gdn_lower(wave, 0) + 4 * lane;
 #pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (j <= wave) {       // (lower triangular: later tokens' tiles are zero)
-                o.tm[j] = *(const fm_v4f *)(in + w.tm + (int64_t)h * 4096 + tok * 64 + 16 * j + 4 * g);
-                o.p[j] = *(const fm_v4f *)(in + w.p + (int64_t)h * 4096 + tok * 64 + 16 * j + 4 * g);
-            }
-        const float *sc = in + w.sc + (int64_t)h * 256 + 16 * wave + 4 * g;
+        for (int j = 0; j < 4; j++) {
+            o.tm[j] = *(const fm_v4f *)(low + w.tm + min(j, wave) * FM_GDN_TILE);
+            o.p[j] = *(const fm_v4f *)(low + w.p + min(j, wave) * FM_GDN_TILE);
+        }
+        const float *sc = in + w.sc + h * 256 + 16 * wave + 4 * g;
         o.beta = *(const fm_v4f *)sc;
         o.fk = *(const fm_v4f *)(sc + 64);
         o.fu = *(const fm_v4f *)(sc + 128);
         o.fq = *(const fm_v4f *)(sc + 192);
 #pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const int t = 16 * wave + 4 * g + i;
-            o.v[i] = t < n ? fm_ld1<BF16>(a.v, (row0 + t) * a.v_stride + (int64_t)h * a.v_dim + v0 + r) : 0.0f;
-        }
+        for (int i = 0; i < 4; i++)
+            o.v[i] = fm_ld1<BF16>(a.v, (row0 + min(16 * wave + 4 * g + i, n - 1)) * a.v_stride + (int64_t)h * a.v_dim + v0 + r);
         o.decay = in[w.end + h];
     };
-    Ops o, nx;
-    if (chunks > 0) load(0, o);
-    for (int c = 0; c < chunks; c++) {
+    // chunk c from o, while chunk c + 1 is fetched into nx
+    auto step = [&](int c, const Ops &o, Ops &nx) {
         const int n = min(64, T - 64 * c);
-        if (c + 1 < chunks) load(c + 1, nx);
+        load(min(c + 1, chunks - 1), nx);
         const fm_v4f zero = {0.f, 0.f, 0.f, 0.f};
         fm_v4f ks0 = zero, ks1 = zero, qs0 = zero, qs1 = zero;
-        __syncthreads();                                   // S is there
+        lds_barrier();                                     // S is there
 #pragma unroll
         for (int d = 0; d < DK / 16; d += 2) {
             const fm_v4f s0 = *(const fm_v4f *)(ss + r * LS + 16 * d + 4 * g), s1 = *(const fm_v4f *)(ss + r * LS + 16 * d + 16 + 4 * g);
-            ks0 = mfma16(o.k[d], s0, ks0);
-            qs0 = mfma16(o.q[d], s0, qs0);
-            ks1 = mfma16(o.k[d + 1], s1, ks1);
-            qs1 = mfma16(o.q[d + 1], s1, qs1);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                ks0 = mfma4(o.k[d][e], s0[e], ks0);
+                qs0 = mfma4(o.q[d][e], s0[e], qs0);
+                ks1 = mfma4(o.k[d + 1][e], s1[e], ks1);
+                qs1 = mfma4(o.q[d + 1][e], s1[e], qs1);
+            }
         }
         fm_v4f x;
 #pragma unroll
-        for (int i = 0; i < 4; i++) x[i] = o.beta[i] * o.v[i] - o.fk[i] * (ks0[i] + ks1[i]);
+        for (int i = 0; i < 4; i++)
+            x[i] = 16 * wave + 4 * g + i < n ? o.beta[i] * o.v[i] - o.fk[i] * (ks0[i] + ks1[i]) : 0.0f;
         *(fm_v4f *)(sr + r * LU + 16 * wave + 4 * g) = x;
-        __syncthreads();                                   // R is there, S has been read
-        fm_v4f u0 = zero, u1 = zero;
+        lds_barrier();                                     // R is there, S has been read
+        fm_v4f u[4] = {zero, zero, zero, zero};
 #pragma unroll
         for (int j = 0; j < 4; j++)
             if (j <= wave) {
                 const fm_v4f y = *(const fm_v4f *)(sr + r * LU + 16 * j + 4 * g);
-                if (j & 1) u1 = mfma16(o.tm[j], y, u1);
-                else u0 = mfma16(o.tm[j], y, u0);
+#pragma unroll
+                for (int e = 0; e < 4; e++) u[e] = mfma4(o.tm[j][e], y[e], u[e]);
             }
-        u0 += u1;
+        const fm_v4f u0 = (u[0] + u[1]) + (u[2] + u[3]);
         *(fm_v4f *)(su + r * LU + 16 * wave + 4 * g) = u0;
         *(fm_v4f *)(sw + r * LU + 16 * wave + 4 * g) = u0 * o.fu;
-        __syncthreads();                                   // u is there
+        lds_barrier();                                     // u is there
+        fm_v4f z[ST][2];
+#pragma unroll
+        for (int t = 0; t < ST; t++) z[t][0] = st[t] * o.decay, z[t][1] = zero;
+#pragma unroll
+        for (int j = 0; j < 4; j += 2) {
+            const fm_v4f y0 = *(const fm_v4f *)(sw + r * LU + 16 * j + 4 * g), y1 = *(const fm_v4f *)(sw + r * LU + 16 * j + 16 + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+#pragma unroll
+                for (int t = 0; t < ST; t++) {
+                    z[t][0] = mfma4(o.kt[t][j][e], y0[e], z[t][0]);
+                    z[t][1] = mfma4(o.kt[t][j + 1][e], y1[e], z[t][1]);
+                }
+        }
 #pragma unroll
         for (int t = 0; t < ST; t++) {
-            fm_v4f z0 = st[t] * o.decay, z1 = zero;
-#pragma unroll
-            for (int j = 0; j < 4; j += 2) {
-                z0 = mfma16(o.kt[t][j], *(const fm_v4f *)(sw + r * LU + 16 * j + 4 * g), z0);
-                z1 = mfma16(o.kt[t][j + 1], *(const fm_v4f *)(sw + r * LU + 16 * j + 16 + 4 * g), z1);
-            }
-            st[t] = z0 + z1;
+            st[t] = z[t][0] + z[t][1];
             *(fm_v4f *)(ss + r * LS + (wave * ST + t) * 16 + 4 * g) = st[t];
         }
-        fm_v4f y0 = o.fq * (qs0 + qs1), y1 = zero;
+        fm_v4f y[4] = {o.fq * (qs0 + qs1), zero, zero, zero};
 #pragma unroll
         for (int j = 0; j < 4; j++)
             if (j <= wave) {
-                const fm_v4f y = *(const fm_v4f *)(su + r * LU + 16 * j + 4 * g);
-                if (j & 1) y1 = mfma16(o.p[j], y, y1);
-                else y0 = mfma16(o.p[j], y, y0);
+                const fm_v4f x = *(const fm_v4f *)(su + r * LU + 16 * j + 4 * g);
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = mfma4(o.p[j][e], x[e], y[e]);
             }
-        y0 += y1;
+        const fm_v4f y0 = (y[0] + y[1]) + (y[2] + y[3]);
         const int64_t row0 = b.row[s] + 64 * (int64_t)c + 16 * wave + 4 * g;
 #pragma unroll
         for (int i = 0; i < 4; i++)
             if (16 * wave + 4 * g + i < n) fm_st1<BF16>(a.out, ((row0 + i) * a.v_heads + h) * a.v_dim + v0 + r, y0[i]);
-        if (c + 1 < chunks) o = nx;
+    };
+    // (two sets of operands that take turns: a copy from one to the other would wait for the loads)
+    Ops o0, o1;
+    load(0, o0);
+    for (int c = 0; c < chunks; c += 2) {
+        step(c, o0, o1);
+        if (c + 1 < chunks) step(c + 1, o1, o0);
     }
 #pragma unroll
     for (int t = 0; t < ST; t++) *(fm_v4f *)(b.out[s] + st_at + (wave * ST + t) * 16 + 4 * g) = st[t];

@@ -60,18 +60,25 @@ FM_HD int fm_gdn_seq_of(const FmGdnSeqs &b, int c) {
 #define FM_GDN_CHUNK 64
 // Sequences of fewer rows run token by token.
 #define FM_GDN_MIN_CHUNKED 24
-// What the chunked form keeps per chunk between its two kernels, in floats:
-//   kt [k_heads][k_dim][64] | tm [v_heads][64][64] | p [v_heads][64][64] | sc [v_heads][4][64] |
-//   end [v_heads], to a multiple of 64
+// What the chunked form keeps per chunk between its two kernels, in floats: K, Q and K^T of a key head,
+// the lower tiles of T and P of a value head, each in the order the second kernel's lanes take them — tiles of 16
+// x 16 in 64 groups of four floats, lane 16 g + r has columns 4 g .. 4 g + 3 of row r — then four
+// factors per token (sc) and one per chunk (end) of a value head.
 struct FmGdnWs {
-    int64_t kt, tm, p, sc, end, floats;
+    int64_t k, q, kt, tm, p, sc, end, floats;
 };
+#define FM_GDN_TILE 256     // floats
+// tile (i, j <= i) of the lower tiles of a 64 x 64 matrix
+FM_HDC int fm_gdn_lower(int i, int j) { return (i * (i + 1) / 2 + j) * FM_GDN_TILE; }
 FM_HD FmGdnWs fm_gdn_ws(const FmGdn &a) {
     FmGdnWs w;
-    w.kt = 0;
-    w.tm = (int64_t)a.k_heads * a.k_dim * 64;
-    w.p = w.tm + (int64_t)a.v_heads * 4096;
-    w.sc = w.p + (int64_t)a.v_heads * 4096;
+    const int64_t rows = (int64_t)a.k_heads * a.k_dim * 64, low = (int64_t)a.v_heads * 10 * FM_GDN_TILE;
+    w.k = 0;
+    w.q = rows;
+    w.kt = 2 * rows;
+    w.tm = 3 * rows;
+    w.p = w.tm + low;
+    w.sc = w.p + low;
     w.end = w.sc + (int64_t)a.v_heads * 256;
     w.floats = w.end + (a.v_heads + 63) / 64 * 64;
     return w;
