@@ -327,144 +327,157 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
     }
 }
 
-// The chunks of a sequence in order, 16 value dims of one head per workgroup.  Wave w has the chunk's tokens
-// 16 w .. 16 w + 15 and, of the state [k_dim][16], the k rows (k_dim / 4) w ..; S, R and u pass
-// through LDS as [column][k or token], so that both the writers (four consecutive rows of a
-// result) and the readers (four consecutive k of an operand) move 16 bytes.
+// The chunks of a sequence in order, 16 value dims of one head per workgroup: eight waves, two per
+// token tile of 16.  Of the state [k_dim][16] a wave keeps a tile of 16 k in registers (k_dim 64: the
+// second four keep none).  S, R and u pass through LDS as [column][k or token], so that both the
+// writers (four consecutive rows of a result) and the readers (four consecutive k of an operand) move
+// 16 bytes.  A chunk is three phases between barriers,
+//   1  waves 0-3: R = beta V - f K S                waves 4-7: half of Q S
+//   2  waves 0-3: u = T R                                      the other half
+//   3  waves 0-3: S += K^T u, k 0-63                waves 4-7: S += K^T u, k 64-127; P u, the output
+// which keep a SIMD's matrix core fed by one wave while the other is at a barrier or moves data.
+// Operands are fetched for the next chunk right behind their use, into the registers that become free: the
+// loads are spread between the products (issued in one go they hold a wave up for as long as the products
+// take) and have a chunk's time to arrive.  Every load is issued on every path (rows behind the last
+// one as that one, tiles above the diagonal as the diagonal's, what they give is dropped): one that some path
+// skips would make the compiler wait for all.
 template <int DK, bool BF16>
-__global__ __launch_bounds__(256, 1) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, const float *ws) {
-    constexpr int LS = DK + 4, LU = 68, ST = DK / 64;    // ST: state tiles of a wave
-    __shared__ __attribute__((aligned(16))) float ss[16 * LS], sr[16 * LU], su[16 * LU], sw[16 * LU];
-    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+__global__ __launch_bounds__(512, 2) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, const float *ws) {
+    constexpr int LS = DK + 4, LU = 68, ND = DK / 16;
+    __shared__ __attribute__((aligned(16))) float ss[16 * LS], sr[16 * LU], su[16 * LU], sw[16 * LU], none[4];
+    const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wv & 3, lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    const bool second = wv >= 4;
     const int h = blockIdx.x % a.v_heads, v0 = 16 * (blockIdx.x / a.v_heads), s = blockIdx.y;
     const int hk = h / (a.v_heads / a.k_heads);
     const FmGdnWs w = fm_gdn_ws(a);
     const int T = b.rows[s], chunks = (T + 63) / 64;
+    const fm_v4f zero = {0.f, 0.f, 0.f, 0.f};
     // the state's rows [v_dim][k_dim] are the columns here
-    const int64_t st_at = ((int64_t)h * a.v_dim + v0 + r) * DK;
-    fm_v4f st[ST];
-#pragma unroll
-    for (int t = 0; t < ST; t++) {
-        const int k = (wave * ST + t) * 16 + 4 * g;
-        st[t] = b.in[s] ? *(const fm_v4f *)(b.in[s] + st_at + k) : fm_v4f{0.f, 0.f, 0.f, 0.f};
-        *(fm_v4f *)(ss + r * LS + k) = st[t];
+    const bool keeps = !second || DK == 128;
+    const int k_at = wv * 16 + 4 * g;
+    const int64_t st_at = ((int64_t)h * a.v_dim + v0 + r) * DK + k_at;
+    fm_v4f st = zero;
+    if (keeps) {
+        if (b.in[s]) st = *(const fm_v4f *)(b.in[s] + st_at);
+        *(fm_v4f *)(ss + r * LS + k_at) = st;
     }
-    struct Ops {
-        fm_v4f k[DK / 16], q[DK / 16], kt[ST][4], tm[4], p[4], beta, fk, fu, fq;
-        float v[4], decay;
+    if (threadIdx.x < 4) none[threadIdx.x] = 0.0f;
+    const float *in;
+    int n_in;
+    int64_t row_in;
+    auto at_chunk = [&](int c) {
+        n_in = min(64, T - 64 * c);
+        row_in = b.row[s] + 64 * (int64_t)c;
+        in = ws + (int64_t)(b.chunk0[s] + c) * w.floats;
     };
-    // Every load of a chunk is issued on every path (rows behind the last one as that one, tiles above
-    // the diagonal as that one: what they give is dropped): a load that some path skips would make
-    // the compiler wait for all of them.
-    auto load = [&](int c, Ops &o) {
-        const int n = min(64, T - 64 * c);
-        const int64_t row0 = b.row[s] + 64 * (int64_t)c;
-        const float *in = ws + (int64_t)(b.chunk0[s] + c) * w.floats;
-        const float *k = in + (int64_t)hk * DK * 64 + wave * (DK / 16) * FM_GDN_TILE + 4 * lane;
+    // uniform base, lane offset
+    const unsigned lane4 = 4 * lane;
+    const int64_t row_at = (second ? w.q : w.k) + ((int64_t)hk * DK * 64 + wave * ND * FM_GDN_TILE);
+    const int64_t low_at = (second ? w.p : w.tm) + (int64_t)h * 10 * FM_GDN_TILE + fm_gdn_lower(wave, 0);
+    const int64_t kt_at = w.kt + (int64_t)hk * DK * 64 + (keeps ? wv : 0) * 4 * FM_GDN_TILE;
+    const unsigned sc_lane = 16 * wave + 4 * g;
+    auto ld = [&](int64_t at) { return *(const fm_v4f *)(in + at + lane4); };
+    fm_v4f rows[ND], low[4], kt[4], beta = zero, f0 = zero, f1 = zero;   // K or Q, T or P, K^T, factors
+    float v[4] = {0.f, 0.f, 0.f, 0.f}, decay;
+    auto load_kt = [&](int j) { kt[j] = ld(kt_at + j * FM_GDN_TILE); };
+    auto load_low = [&](int j) { low[j] = ld(low_at + min(j, wave) * FM_GDN_TILE); };
+    auto load_rows = [&](int d) { rows[d] = ld(row_at + d * FM_GDN_TILE); };
+    auto load_v = [&]() {
+        const float *sc = in + w.sc + h * 256;
+        beta = *(const fm_v4f *)(sc + sc_lane);
+        f0 = *(const fm_v4f *)(sc + 64 + sc_lane);
 #pragma unroll
-        for (int d = 0; d < DK / 16; d++) {
-            o.k[d] = *(const fm_v4f *)(k + w.k + d * FM_GDN_TILE);
-            o.q[d] = *(const fm_v4f *)(k + w.q + d * FM_GDN_TILE);
-        }
-        const float *kt = in + w.kt + (int64_t)hk * DK * 64 + wave * ST * 4 * FM_GDN_TILE + 4 * lane;
-#pragma unroll
-        for (int t = 0; t < ST; t++)
-#pragma unroll
-            for (int j = 0; j < 4; j++) o.kt[t][j] = *(const fm_v4f *)(kt + (t * 4 + j) * FM_GDN_TILE);
-        const float *low = in + (int64_t)h * 10 * FM_GDN_TILE + fm_gdn_lower(wave, 0) + 4 * lane;
+        for (int i = 0; i < 4; i++)
+            v[i] = fm_ld1<BF16>(a.v, (row_in + min((int)sc_lane + i, n_in - 1)) * a.v_stride + (int64_t)h * a.v_dim + v0 + r);
+    };
+    auto load_f1 = [&]() { f1 = *(const fm_v4f *)(in + w.sc + h * 256 + (second ? 192 : 128) + sc_lane); };
+    auto load_decay = [&]() { decay = in[w.end + h]; };
+    // sum over the tiles j <= wave of the lower tiles; the operand of the others is zero
+    auto lower = [&](const float *x, fm_v4f first) {
+        fm_v4f u[4] = {first, zero, zero, zero};
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-            o.tm[j] = *(const fm_v4f *)(low + w.tm + min(j, wave) * FM_GDN_TILE);
-            o.p[j] = *(const fm_v4f *)(low + w.p + min(j, wave) * FM_GDN_TILE);
-        }
-        const float *sc = in + w.sc + h * 256 + 16 * wave + 4 * g;
-        o.beta = *(const fm_v4f *)sc;
-        o.fk = *(const fm_v4f *)(sc + 64);
-        o.fu = *(const fm_v4f *)(sc + 128);
-        o.fq = *(const fm_v4f *)(sc + 192);
+            const fm_v4f y = *(const fm_v4f *)(j <= wave ? x + r * LU + 16 * j + 4 * g : none);
 #pragma unroll
-        for (int i = 0; i < 4; i++)
-            o.v[i] = fm_ld1<BF16>(a.v, (row0 + min(16 * wave + 4 * g + i, n - 1)) * a.v_stride + (int64_t)h * a.v_dim + v0 + r);
-        o.decay = in[w.end + h];
+            for (int e = 0; e < 4; e++) u[e] = mfma4(low[j][e], y[e], u[e]);
+            load_low(j);
+        }
+        return (u[0] + u[1]) + (u[2] + u[3]);
     };
-    // chunk c from o, while chunk c + 1 is fetched into nx
-    auto step = [&](int c, const Ops &o, Ops &nx) {
-        const int n = min(64, T - 64 * c);
-        load(min(c + 1, chunks - 1), nx);
-        const fm_v4f zero = {0.f, 0.f, 0.f, 0.f};
-        fm_v4f ks0 = zero, ks1 = zero, qs0 = zero, qs1 = zero;
-        lds_barrier();                                     // S is there
+    auto times_s = [&](int d0, int d1, fm_v4f *x) {
 #pragma unroll
-        for (int d = 0; d < DK / 16; d += 2) {
-            const fm_v4f s0 = *(const fm_v4f *)(ss + r * LS + 16 * d + 4 * g), s1 = *(const fm_v4f *)(ss + r * LS + 16 * d + 16 + 4 * g);
+        for (int d = 0; d < ND; d++)
+            if (d >= d0 && d < d1) {
+                const fm_v4f y = *(const fm_v4f *)(ss + r * LS + 16 * d + 4 * g);
 #pragma unroll
-            for (int e = 0; e < 4; e++) {
-                ks0 = mfma4(o.k[d][e], s0[e], ks0);
-                qs0 = mfma4(o.q[d][e], s0[e], qs0);
-                ks1 = mfma4(o.k[d + 1][e], s1[e], ks1);
-                qs1 = mfma4(o.q[d + 1][e], s1[e], qs1);
+                for (int e = 0; e < 4; e++) x[e] = mfma4(rows[d][e], y[e], x[e]);
+                load_rows(d);
             }
-        }
-        fm_v4f x;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            x[i] = 16 * wave + 4 * g + i < n ? o.beta[i] * o.v[i] - o.fk[i] * (ks0[i] + ks1[i]) : 0.0f;
-        *(fm_v4f *)(sr + r * LU + 16 * wave + 4 * g) = x;
-        lds_barrier();                                     // R is there, S has been read
-        fm_v4f u[4] = {zero, zero, zero, zero};
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (j <= wave) {
-                const fm_v4f y = *(const fm_v4f *)(sr + r * LU + 16 * j + 4 * g);
-#pragma unroll
-                for (int e = 0; e < 4; e++) u[e] = mfma4(o.tm[j][e], y[e], u[e]);
-            }
-        const fm_v4f u0 = (u[0] + u[1]) + (u[2] + u[3]);
-        *(fm_v4f *)(su + r * LU + 16 * wave + 4 * g) = u0;
-        *(fm_v4f *)(sw + r * LU + 16 * wave + 4 * g) = u0 * o.fu;
-        lds_barrier();                                     // u is there
-        fm_v4f z[ST][2];
-#pragma unroll
-        for (int t = 0; t < ST; t++) z[t][0] = st[t] * o.decay, z[t][1] = zero;
-#pragma unroll
-        for (int j = 0; j < 4; j += 2) {
-            const fm_v4f y0 = *(const fm_v4f *)(sw + r * LU + 16 * j + 4 * g), y1 = *(const fm_v4f *)(sw + r * LU + 16 * j + 16 + 4 * g);
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-#pragma unroll
-                for (int t = 0; t < ST; t++) {
-                    z[t][0] = mfma4(o.kt[t][j][e], y0[e], z[t][0]);
-                    z[t][1] = mfma4(o.kt[t][j + 1][e], y1[e], z[t][1]);
-                }
-        }
-#pragma unroll
-        for (int t = 0; t < ST; t++) {
-            st[t] = z[t][0] + z[t][1];
-            *(fm_v4f *)(ss + r * LS + (wave * ST + t) * 16 + 4 * g) = st[t];
-        }
-        fm_v4f y[4] = {o.fq * (qs0 + qs1), zero, zero, zero};
-#pragma unroll
-        for (int j = 0; j < 4; j++)
-            if (j <= wave) {
-                const fm_v4f x = *(const fm_v4f *)(su + r * LU + 16 * j + 4 * g);
-#pragma unroll
-                for (int e = 0; e < 4; e++) y[e] = mfma4(o.p[j][e], x[e], y[e]);
-            }
-        const fm_v4f y0 = (y[0] + y[1]) + (y[2] + y[3]);
-        const int64_t row0 = b.row[s] + 64 * (int64_t)c + 16 * wave + 4 * g;
-#pragma unroll
-        for (int i = 0; i < 4; i++)
-            if (16 * wave + 4 * g + i < n) fm_st1<BF16>(a.out, ((row0 + i) * a.v_heads + h) * a.v_dim + v0 + r, y0[i]);
     };
-    // (two sets of operands that take turns: a copy from one to the other would wait for the loads)
-    Ops o0, o1;
-    load(0, o0);
-    for (int c = 0; c < chunks; c += 2) {
-        step(c, o0, o1);
-        if (c + 1 < chunks) step(c + 1, o1, o0);
+    auto update = [&]() {
+        fm_v4f z[4] = {st * decay, zero, zero, zero};
+        load_decay();
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const fm_v4f y = *(const fm_v4f *)(sw + r * LU + 16 * j + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; e++) z[e] = mfma4(kt[j][e], y[e], z[e]);
+            load_kt(j);
+        }
+        st = (z[0] + z[1]) + (z[2] + z[3]);
+        *(fm_v4f *)(ss + r * LS + k_at) = st;
+    };
+    at_chunk(0);
+#pragma unroll
+    for (int d = 0; d < ND; d++) load_rows(d);
+    load_f1();
+    load_decay();
+#pragma unroll
+    for (int j = 0; j < 4; j++) load_low(j), load_kt(j);
+    if (!second) load_v();
+    // (the first chunk's operands arrive before the loop: its waits then go by the loop's own order of loads)
+    __builtin_amdgcn_s_waitcnt(0x0F70);                    // vmcnt(0)
+    if (!second) {
+        for (int c = 0; c < chunks; c++) {
+            const int n = n_in;
+            at_chunk(min(c + 1, chunks - 1));
+            fm_v4f x[4] = {zero, zero, zero, zero};
+            lds_barrier();                                 // S is there
+            times_s(0, ND, x);
+            const fm_v4f ks = (x[0] + x[1]) + (x[2] + x[3]);
+            fm_v4f rr;
+#pragma unroll
+            for (int i = 0; i < 4; i++) rr[i] = (int)sc_lane + i < n ? beta[i] * v[i] - f0[i] * ks[i] : 0.0f;
+            *(fm_v4f *)(sr + r * LU + sc_lane) = rr;
+            load_v();
+            lds_barrier();                                 // R is there
+            const fm_v4f u = lower(sr, zero);
+            *(fm_v4f *)(su + r * LU + sc_lane) = u;
+            *(fm_v4f *)(sw + r * LU + sc_lane) = u * f1;
+            load_f1();
+            lds_barrier();                                 // u is there, S has been read
+            update();
+        }
+    } else {
+        for (int c = 0; c < chunks; c++) {
+            const int n = n_in;
+            const int64_t row0 = row_in + sc_lane;
+            at_chunk(min(c + 1, chunks - 1));
+            fm_v4f x[4] = {zero, zero, zero, zero};
+            lds_barrier();
+            times_s(0, ND / 2, x);
+            lds_barrier();
+            times_s(ND / 2, ND, x);
+            lds_barrier();
+            if (keeps) update();
+            const fm_v4f y = lower(su, f1 * ((x[0] + x[1]) + (x[2] + x[3])));
+            load_f1();
+#pragma unroll
+            for (int i = 0; i < 4; i++)
+                if ((int)sc_lane + i < n) fm_st1<BF16>(a.out, ((row0 + i) * a.v_heads + h) * a.v_dim + v0 + r, y[i]);
+        }
     }
-#pragma unroll
-    for (int t = 0; t < ST; t++) *(fm_v4f *)(b.out[s] + st_at + (wave * ST + t) * 16 + 4 * g) = st[t];
+    if (keeps) *(fm_v4f *)(b.out[s] + st_at) = st;
 }
 
 template <int DK, bool BF16>
@@ -473,7 +486,7 @@ int launch_seqs(const FmGdn &a, const FmGdnSeqs &b, int chunked, float *ws, hipS
         hipLaunchKernelGGL((fm_gdn_steps<DK, BF16, 1>), dim3(a.v_dim / 16, a.v_heads, b.n), dim3(256), 0, st, a, b);
     } else {
         hipLaunchKernelGGL((fm_gdn_prep<DK, BF16>), dim3(b.chunk0[b.n], a.k_heads), dim3(256), 0, st, a, b, ws);
-        hipLaunchKernelGGL((fm_gdn_scan<DK, BF16>), dim3(a.v_heads * (a.v_dim / 16), b.n), dim3(256), 0, st, a, b, ws);
+        hipLaunchKernelGGL((fm_gdn_scan<DK, BF16>), dim3(a.v_heads * (a.v_dim / 16), b.n), dim3(512), 0, st, a, b, ws);
     }
     return hipGetLastError() == hipSuccess ? FM_OK : FM_ERR_HIP;
 }
