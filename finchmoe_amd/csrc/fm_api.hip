@@ -65,7 +65,7 @@ int fm_launch_attn(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int bf16, v
 int fm_launch_kv(const FmKv *c, const FmKvRows *x, const FmSeqs *b, int D, int bf16, int read, hipStream_t st);
 size_t fm_logprob_ws(int rows, int vocab, int top_n);
 int fm_launch_logprob(const float *x, int rows, int vocab, int64_t stride, const int32_t *tokens, int top_n,
-                      float *logprob, float *entropy, int32_t *ids, float *top_lp, void *ws, hipStream_t st);
+                      float *logprob, float *entropy, int32_t *ids, float *top_lp, void *ws, int n_cu, hipStream_t st);
 }
 
 // ---- scratch of the entry point that allocates nothing (fm_moe_decode_step_noalloc_dev) ----
@@ -1742,7 +1742,7 @@ extern "C" int fm_logprobs_dev(fm_ctx *c, const float *d_logits, int rows, int v
     DeviceGuard dg(c->device);
     if ((rc = ensure_ws(c, fm_logprob_ws(rows, vocab, top_n)))) return rc;
     rc = fm_launch_logprob(d_logits, rows, vocab, row_stride, d_tokens, top_n, d_logprob, d_entropy, d_top_ids,
-                           d_top_logprobs, c->d_ws, c->stream);
+                           d_top_logprobs, c->d_ws, c->n_cu, c->stream);
     if (rc) return fail(c, rc, "log probability launch failed: %s", hipGetErrorString(hipGetLastError()));
     return FM_OK;
 }

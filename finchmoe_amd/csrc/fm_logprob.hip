@@ -1,40 +1,50 @@
 // fm_logprob.hip — log probability of a given token, entropy and the largest alternatives of rows
 // of logits (include/finch_hip.h, fm_logprobs_dev), in one pass over the logits.
 //
-// A row is cut into segments of FM_LP_SEG elements, one workgroup each, sixteen elements a thread in
-// registers.  With d_i = x_i - m, m the row's maximum and the (first) maximum's own term e^0 = 1
-// kept apart,
+// A row is cut into segments, one workgroup each, E elements a thread in registers.  With d_i = x_i - m,
+// m the row's maximum and the (first) maximum's own term e^0 = 1 kept apart,
 //   Z' = sum over the others of e^d,  log p_i = d_i - log1p(Z'),  H = log1p(Z') - sum e^d d / (1 + Z')
 // so that neither loses its digits when one token holds nearly all the probability.  A segment
 // gives (m, Z', sum e^d d) for its own maximum, and its top_n largest elements.
 //
 // Order: an element's key is its value, made an unsigned number of the same order, above the complement
 // of its index: keys of a row are distinct, and the larger key is the larger value or, of equal
-// ones, the lower index.  The top_n keys of a segment: the top_n-th largest of the threads'
-// maxima bounds the top_n-th largest key from below, and at most 16 top_n keys (those of top_n threads)
-// are not below it; they are ranked by counting.  The second kernel joins a row's segments the same way.
+// ones, the lower index.  The top_n keys of a segment: the top_n-th largest of a wave's 64 lane
+// maxima (to 16 bits, found bit by bit with ballots) bounds the segment's top_n-th value from below, so
+// does the largest of the waves' bounds; the elements that reach it, few more than top_n, are
+// collected and ranked by counting.  (Equal values, or many of the largest in one lane, may be more than
+// there is room for: then the maximum is taken top_n times instead.)  A second kernel joins a row's
+// segments the same way.
+//
+// 257 rows of 248320: bound by the loads and, close behind, by the vector ALU (ten instruction slots an
+// element, four of them the exponential's).
 #include "fm_common.h"
 
 namespace {
 
-constexpr int LP_T = 256, LP_E = 16;           // threads, elements per thread
-constexpr int LP_SEG = LP_T * LP_E;
+constexpr int LP_T = 256;            // threads
 constexpr int LP_TOP = 32;
+constexpr int LP_CAND = 512;
 
 typedef unsigned long long LpKey;
+typedef float fm_v4 __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ uint32_t order_bits(float x) {      // unsigned order of the floats
-    const uint32_t b = __float_as_uint(x);
-    return b & 0x80000000u ? ~b : b | 0x80000000u;
+    // (-0 and +0 are equal values: both take the place of +0)
+    const uint32_t b = __float_as_uint(x == 0.0f ? 0.0f : x);
+    return b ^ ((uint32_t)((int32_t)b >> 31) | 0x80000000u);
 }
 __device__ __forceinline__ float from_order(uint32_t o) {
     return __uint_as_float(o & 0x80000000u ? o & 0x7FFFFFFFu : ~o);
 }
-// -0 and +0 are equal values: both take the key of +0
 __device__ __forceinline__ LpKey make_key(float x, uint32_t idx) {
-    return (LpKey)order_bits(x == 0.0f ? 0.0f : x) << 32 | (0xFFFFFFFFu - idx);
+    return (LpKey)order_bits(x) << 32 | (0xFFFFFFFFu - idx);
 }
 __device__ __forceinline__ LpKey key_max(LpKey a, LpKey b) { return a > b ? a : b; }
+__device__ __forceinline__ LpKey wave_key_max(LpKey k) {
+    for (int o = 32; o; o >>= 1) k = key_max(k, (LpKey)__shfl_xor(k, o));
+    return k;
+}
 
 struct Part {             // what a segment leaves: statistics relative to its own maximum
     float m, z, ed;       // maximum, sum of e^d without the maximum's own term, sum of e^d d
@@ -42,80 +52,136 @@ struct Part {             // what a segment leaves: statistics relative to its o
 };
 
 struct Shared {
-    LpKey keys[LP_T];
-    LpKey cand[LP_E * LP_TOP];
-    LpKey bound;
+    LpKey cand[LP_CAND], bound[LP_T / 64];
     float red[2][LP_T / 64];
     int n_cand;
 };
 
-// The n largest of the block's keys (E per thread; key 0 = none) into dst[0..n), largest first,
-// 0 where there are fewer.  mine: the thread's largest key.
-template <int E>
-__device__ __forceinline__ void block_top(const LpKey *k, LpKey mine, int n, Shared &sh, LpKey *dst) {
+// The largest t with zero low half that at least n of the wave's lanes reach; 0 if fewer than n lanes have one.
+__device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
+    uint32_t t = 0;
+#pragma unroll
+    for (int b = 31; b >= 16; b--) {
+        const uint32_t trial = t | 1u << b;
+        if (__popcll(__ballot(v >= trial)) >= n) t = trial;
+    }
+    return t;
+}
+
+// The n largest of the block's keys into dst[0..n), largest first, 0 where there are fewer.  key(e), e < E:
+// the thread's e-th (0 = none); reaches(e, bound): whether its value's order bits may reach the bound;
+// big: the largest of those.
+template <int E, class Key, class Reaches>
+__device__ __forceinline__ void block_top(Key key, Reaches reaches, uint32_t big, int n, Shared &sh, LpKey *dst) {
     const int t = threadIdx.x;
-    sh.keys[t] = mine;
-    if (t == 0) sh.n_cand = 0, sh.bound = 0;
+    const uint32_t of_wave = nth_largest(big, n);
+    if ((t & 63) == 0) sh.bound[t >> 6] = of_wave;
+    if (t == 0) sh.n_cand = 0;
     __syncthreads();
-    // the thread's place among the threads' maxima: the first n threads hold all candidates
-    int place = 0;
-    for (int j = 0; j < LP_T; j++) place += sh.keys[j] > mine;
-    // (keys are distinct but for the empty key 0; with fewer than n keys the bound stays 0)
-    if (place == n - 1) sh.bound = mine;
-    __syncthreads();
-    const LpKey bound = sh.bound;
-    if (mine >= bound && mine) {
+    uint32_t bound = 1;      // (order bits are never 0 for a number: 0 marks "none")
+#pragma unroll
+    for (int w = 0; w < LP_T / 64; w++) bound = max(bound, (uint32_t)sh.bound[w]);
+    if (big >= bound) {
 #pragma unroll
         for (int e = 0; e < E; e++)
-            if (k[e] >= bound && k[e]) {
+            if (reaches(e, bound)) {
+                const LpKey k = key(e);
+                if (!k) continue;
                 const int at = atomicAdd(&sh.n_cand, 1);
-                if (at < LP_E * LP_TOP) sh.cand[at] = k[e];
+                if (at < LP_CAND) sh.cand[at] = k;
             }
     }
     __syncthreads();
-    const int c = min(sh.n_cand, LP_E * LP_TOP);
-    for (int i = t; i < c; i += LP_T) {
-        const LpKey v = sh.cand[i];
-        int rank = 0;
-        for (int j = 0; j < c; j++) rank += sh.cand[j] > v;
-        if (rank < n) dst[rank] = v;
+    const int c = sh.n_cand;
+    if (c <= LP_CAND) {
+        for (int i = t; i < c; i += LP_T) {
+            const LpKey v = sh.cand[i];
+            int rank = 0;
+            for (int j = 0; j < c; j++) rank += sh.cand[j] > v;
+            if (rank < n) dst[rank] = v;
+        }
+        for (int i = c + t; i < n; i += LP_T) dst[i] = 0;
+        return;
     }
-    for (int i = c + t; i < n; i += LP_T) dst[i] = 0;
+    LpKey below = ~0ull;
+    for (int i = 0; i < n; i++) {
+        LpKey best = 0;
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            const LpKey k = key(e);
+            if (k < below) best = key_max(best, k);
+        }
+        best = wave_key_max(best);
+        __syncthreads();                       // (the last round's values have been read)
+        if ((t & 63) == 0) sh.bound[t >> 6] = best;
+        __syncthreads();
+        below = 0;
+#pragma unroll
+        for (int w = 0; w < LP_T / 64; w++) below = key_max(below, sh.bound[w]);
+        if (t == 0) dst[i] = below;
+    }
 }
 
+// V4: rows are 16-byte aligned, a thread takes four elements side by side
+template <int E, bool V4>
 __global__ __launch_bounds__(LP_T) void fm_logprob_seg(const float *x, int vocab, int64_t stride, int n_seg, int top_n,
                                                        Part *parts, LpKey *tops) {
     __shared__ Shared sh;
-    __shared__ LpKey wmax[LP_T / 64];
     const int row = blockIdx.y, seg = blockIdx.x, t = threadIdx.x;
     const float *r = x + (int64_t)row * stride;
-    const int base = seg * LP_SEG;
-    float v[LP_E];
-    LpKey k[LP_E], mine = 0;
-    int bad = 0;
+    const int base = seg * (LP_T * E);
+    auto index = [&](int e) { return V4 ? base + (e >> 2) * (4 * LP_T) + 4 * t + (e & 3) : base + e * LP_T + t; };
+    float v[E];
+    if (base + LP_T * E <= vocab) {
 #pragma unroll
-    for (int e = 0; e < LP_E; e++) {
-        const int i = base + e * LP_T + t;
-        v[e] = i < vocab ? r[i] : -INFINITY;
-        k[e] = i < vocab ? make_key(v[e], (uint32_t)i) : 0;
-        bad |= i < vocab && !(v[e] < INFINITY);
-        mine = key_max(mine, k[e]);
-    }
-    LpKey top = mine;
-    for (int o = 32; o; o >>= 1) top = key_max(top, (LpKey)__shfl_xor((unsigned long long)top, o));
-    if ((t & 63) == 0) wmax[t >> 6] = top;
-    bad = __syncthreads_or(bad);
-    for (int w = 0; w < LP_T / 64; w++) top = key_max(top, wmax[w]);
-    const float m = from_order((uint32_t)(top >> 32));
-    float z = 0.0f, ed = 0.0f;
-    if (!bad && m > -INFINITY) {
-#pragma unroll
-        for (int e = 0; e < LP_E; e++) {
-            const float d = v[e] - m, p = expf(d);
-            if (k[e] != top && p > 0.0f) {     // (0 * -inf must not come in)
-                z += p;
-                ed = fmaf(p, d, ed);
+        for (int e = 0; e < E; e += V4 ? 4 : 1) {
+            if constexpr (V4) {
+                const fm_v4 w = __builtin_nontemporal_load((const fm_v4 *)(r + index(e)));
+                v[e] = w[0], v[e + 1] = w[1], v[e + 2] = w[2], v[e + 3] = w[3];
+            } else {
+                v[e] = __builtin_nontemporal_load(r + index(e));
             }
+        }
+    } else {               // the row's last segment
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = r[min(index(e), vocab - 1)];
+#pragma unroll
+        for (int e = 0; e < E; e++) v[e] = index(e) < vocab ? v[e] : -INFINITY;
+    }
+    float big = -INFINITY;
+    bool bad = false;
+#pragma unroll
+    for (int e = 0; e < E; e++) bad |= !(v[e] < INFINITY), big = fmaxf(big, v[e]);
+    float m = big;
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
+    if ((t & 63) == 0) sh.red[0][t >> 6] = m;
+    const bool any_bad = __syncthreads_or(bad);
+    m = fmaxf(fmaxf(sh.red[0][0], sh.red[0][1]), fmaxf(sh.red[0][2], sh.red[0][3]));
+    __syncthreads();
+    // The maximum's own term is left out: of the first thread's first element that has it.  (Which of equal ones
+    // does not matter: their terms are the same.)
+    const unsigned long long have = __ballot(big == m);
+    int owner = have ? __ffsll(have) - 1 + (t & ~63) : LP_T;
+    if ((t & 63) == 0) sh.red[1][t >> 6] = __int_as_float(owner);
+    __syncthreads();
+    owner = min(min(__float_as_int(sh.red[1][0]), __float_as_int(sh.red[1][1])), min(__float_as_int(sh.red[1][2]), __float_as_int(sh.red[1][3])));
+    __syncthreads();
+    float z = 0.0f, ed = 0.0f;
+    if (!any_bad && m > -INFINITY) {
+        bool out = t == owner;
+        const bool mine = __ballot(out) != 0;     // (this wave holds the owner)
+#pragma unroll
+        for (int e = 0; e < E; e++) {
+            // e^-200 is 0 in fp32, and 0 * -inf must not come in
+            const float d = fmaxf(v[e] - m, -200.0f);
+            float p = __expf(d);
+            if (mine) {
+                const bool drop = out && d == 0.0f;
+                p = drop ? 0.0f : p;
+                out = out && !drop;
+            }
+            z += p;
+            ed = fmaf(p, d, ed);
         }
     }
     z = fm_group_sum<64>(z);
@@ -127,11 +193,18 @@ __global__ __launch_bounds__(LP_T) void fm_logprob_seg(const float *x, int vocab
         p.m = m;
         p.z = ((sh.red[0][0] + sh.red[0][1]) + sh.red[0][2]) + sh.red[0][3];
         p.ed = ((sh.red[1][0] + sh.red[1][1]) + sh.red[1][2]) + sh.red[1][3];
-        p.bad = bad;
+        p.bad = any_bad;
         parts[(size_t)row * n_seg + seg] = p;
     }
-    if (top_n) block_top<LP_E>(k, mine, top_n, sh, tops + ((size_t)row * n_seg + seg) * top_n);
+    if (top_n) {
+        // (compared as numbers: bounds below -inf stand for everything)
+        auto reaches = [&](int e, uint32_t bound) { return v[e] >= (bound > 0x007FFFFFu ? from_order(bound) : -INFINITY); };
+        block_top<E>([&](int e) { return index(e) < vocab ? make_key(v[e], (uint32_t)index(e)) : (LpKey)0; }, reaches,
+                     index(0) < vocab ? order_bits(big) : 0u, top_n, sh, tops + ((size_t)row * n_seg + seg) * top_n);
+    }
 }
+
+constexpr int JOIN_E = 8;
 
 // joins a row's segments; one workgroup per row
 __global__ __launch_bounds__(LP_T) void fm_logprob_join(const float *x, int vocab, int64_t stride, int n_seg, int top_n,
@@ -143,17 +216,34 @@ __global__ __launch_bounds__(LP_T) void fm_logprob_join(const float *x, int voca
     __shared__ float s_m, s_logz;
     const int row = blockIdx.x, t = threadIdx.x, lane = t & 63, wave = t >> 6;
     const Part *p = parts + (size_t)row * n_seg;
-    float m = -INFINITY;
-    int bad = 0;
-    for (int i = t; i < n_seg; i += LP_T) m = fmaxf(m, p[i].m), bad |= p[i].bad;
+    const LpKey *src = tops + (size_t)row * n_seg * top_n;
+    const int total = n_seg * top_n;
+    // what most rows need (256 segments, a round of keys, the token's logit) is requested at once
+    const Part none = {-INFINITY, 0.0f, 0.0f, 0};
+    const Part p0 = t < n_seg ? p[t] : none;
+    LpKey k[JOIN_E];
+    if (t < LP_TOP) best[t] = 0;
+    auto fetch = [&](int at) {
+#pragma unroll
+        for (int e = 0; e < JOIN_E; e++) {
+            const int i = at + e * LP_T + t - LP_TOP;
+            k[e] = e * LP_T + t >= LP_TOP && i < total ? src[i] : 0;
+        }
+    };
+    if (top_n) fetch(0);
+    const int id = logprob ? tokens[row] : 0;
+    const float given = logprob && id >= 0 && id < vocab ? x[(int64_t)row * stride + id] : -INFINITY;
+    float m = p0.m;
+    int bad = p0.bad;
+    for (int i = t + LP_T; i < n_seg; i += LP_T) m = fmaxf(m, p[i].m), bad |= p[i].bad;
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     if (lane == 0) stat[wave] = m;
     bad = __syncthreads_or(bad);
     m = fmaxf(fmaxf(stat[0], stat[1]), fmaxf(stat[2], stat[3]));
     __syncthreads();
     // the first segment that holds the maximum keeps its own 1 apart, the others' ones count
-    int first = n_seg;
-    for (int i = t; i < n_seg; i += LP_T)
+    int first = p0.m == m ? t : n_seg;
+    for (int i = t + LP_T; i < n_seg; i += LP_T)
         if (p[i].m == m) first = min(first, i);
     for (int o = 32; o; o >>= 1) first = min(first, __shfl_xor(first, o));
     if (lane == 0) stat[wave] = __int_as_float(first);
@@ -162,12 +252,13 @@ __global__ __launch_bounds__(LP_T) void fm_logprob_join(const float *x, int voca
     float z = 0.0f, ed = 0.0f;
     if (!bad && m > -INFINITY)
         for (int i = t; i < n_seg; i += LP_T) {
-            const float d = p[i].m - m, one = i == first ? 0.0f : 1.0f;
+            const Part q = i == t ? p0 : p[i];
+            const float d = q.m - m, one = i == first ? 0.0f : 1.0f;
             const float e = expf(d);
             if (!(e > 0.0f)) continue;         // (0 * -inf must not come in)
-            z = fmaf(e, p[i].z + one, z);
+            z = fmaf(e, q.z + one, z);
             // sum e^(d_i + d) (d_i + d) over the segment's elements
-            ed += e * (p[i].ed + d * (p[i].z + one));
+            ed += e * (q.ed + d * (q.z + one));
         }
     z = fm_group_sum<64>(z);
     ed = fm_group_sum<64>(ed);
@@ -177,40 +268,29 @@ __global__ __launch_bounds__(LP_T) void fm_logprob_join(const float *x, int voca
         z = ((sh.red[0][0] + sh.red[0][1]) + sh.red[0][2]) + sh.red[0][3];
         ed = ((sh.red[1][0] + sh.red[1][1]) + sh.red[1][2]) + sh.red[1][3];
         const float logz = log1pf(z);
-        const bool none = !(m > -INFINITY);
-        if (entropy) entropy[row] = bad ? NAN : none ? 0.0f : logz - ed / (1.0f + z);
+        const bool none_seen = !(m > -INFINITY);
+        if (entropy) entropy[row] = bad ? NAN : none_seen ? 0.0f : logz - ed / (1.0f + z);
         if (logprob) {
-            const int id = tokens[row];
             float lp = -INFINITY;
             if (bad) lp = NAN;
-            else if (id >= 0 && id < vocab && !none) lp = (x[(int64_t)row * stride + id] - m) - logz;
+            else if (!none_seen) lp = (given - m) - logz;
             logprob[row] = lp;
         }
-        s_m = none ? 0.0f : m;
+        s_m = none_seen ? 0.0f : m;
         s_logz = logz;
     }
-    __syncthreads();
     if (!top_n) return;
-    // the segments' lists: few enough keys for one thread to keep its own (vocab < 2^31)
-    const LpKey *src = tops + (size_t)row * n_seg * top_n;
-    const int total = n_seg * top_n;
-    LpKey bound_keys[LP_E];
-    // rounds of LP_SEG keys, the best so far riding along
-    for (int i = t; i < LP_TOP; i += LP_T) best[i] = 0;
+    // the segments' lists in rounds, the best so far riding along in the first threads' first place
     __syncthreads();
-    for (int at = 0; at < total; at += LP_SEG - LP_TOP) {
+    for (int at = 0; at < total; at += LP_T * JOIN_E - LP_TOP) {
+        if (at) fetch(at);
+        if (t < LP_TOP) k[0] = t < top_n ? best[t] : 0;
         LpKey mine = 0;
 #pragma unroll
-        for (int e = 0; e < LP_E; e++) {
-            const int i = e * LP_T + t;
-            LpKey kk = 0;
-            if (i < LP_TOP) kk = i < top_n ? best[i] : 0;
-            else if (at + i - LP_TOP < total) kk = src[at + i - LP_TOP];
-            bound_keys[e] = kk;
-            mine = key_max(mine, kk);
-        }
+        for (int e = 0; e < JOIN_E; e++) mine = key_max(mine, k[e]);
         __syncthreads();
-        block_top<LP_E>(bound_keys, mine, top_n, sh, best);
+        block_top<JOIN_E>([&](int e) { return k[e]; }, [&](int e, uint32_t bound) { return (uint32_t)(k[e] >> 32) >= bound; }, (uint32_t)(mine >> 32), top_n,
+                          sh, best);
         __syncthreads();
     }
     if (t < top_n) {
@@ -221,19 +301,34 @@ __global__ __launch_bounds__(LP_T) void fm_logprob_join(const float *x, int voca
     }
 }
 
+// Elements per thread: 32 when that still gives every CU two workgroups (the selection of the
+// largest runs once per segment), 16 otherwise.
+int per_thread(int rows, int vocab, int n_cu) {
+    const int64_t segs = ((int64_t)vocab + LP_T * 32 - 1) / (LP_T * 32);
+    return rows * segs >= 2 * n_cu ? 32 : 16;
+}
+
 }  // namespace
 
 extern "C" size_t fm_logprob_ws(int rows, int vocab, int top_n) {
-    const size_t n_seg = ((size_t)vocab + LP_SEG - 1) / LP_SEG;
+    const size_t n_seg = ((size_t)vocab + LP_T * 16 - 1) / (LP_T * 16);
     return (size_t)rows * n_seg * (sizeof(Part) + (size_t)top_n * sizeof(LpKey));
 }
 
 extern "C" int fm_launch_logprob(const float *x, int rows, int vocab, int64_t stride, const int32_t *tokens, int top_n,
-                                 float *logprob, float *entropy, int32_t *ids, float *top_lp, void *ws, hipStream_t st) {
-    const int n_seg = (int)(((int64_t)vocab + LP_SEG - 1) / LP_SEG);
+                                 float *logprob, float *entropy, int32_t *ids, float *top_lp, void *ws, int n_cu, hipStream_t st) {
+    const int E = per_thread(rows, vocab, n_cu);
+    const int n_seg = (vocab + LP_T * E - 1) / (LP_T * E);
     LpKey *tops = (LpKey *)ws;
     Part *parts = (Part *)(tops + (size_t)rows * n_seg * top_n);
-    hipLaunchKernelGGL(fm_logprob_seg, dim3(n_seg, rows), dim3(LP_T), 0, st, x, vocab, stride, n_seg, top_n, parts, tops);
+    const bool v4 = ((uintptr_t)x & 15) == 0 && (stride & 3) == 0;
+#define FM_LP(EE, VV) \
+    hipLaunchKernelGGL((fm_logprob_seg<EE, VV>), dim3(n_seg, rows), dim3(LP_T), 0, st, x, vocab, stride, n_seg, top_n, parts, tops)
+    if (E == 32 && v4) FM_LP(32, true);
+    else if (E == 32) FM_LP(32, false);
+    else if (v4) FM_LP(16, true);
+    else FM_LP(16, false);
+#undef FM_LP
     hipLaunchKernelGGL(fm_logprob_join, dim3(rows), dim3(LP_T), 0, st, x, vocab, stride, n_seg, top_n, parts, tops, tokens,
                        logprob, entropy, ids, top_lp);
     return hipGetLastError() == hipSuccess ? FM_OK : FM_ERR_HIP;

@@ -417,7 +417,7 @@ inline int fm_attn_check(FmWhy *w, const fm_attn_args *p, int n_cu, FmKv *k, FmA
 
 inline int fm_logprob_check(FmWhy *w, int rows, int vocab, int top_n) {
     if (rows < 1 || rows > FM_MAX_ROWS) return fm_why(w, FM_ERR_ARG, "%d rows outside 1..%d", rows, FM_MAX_ROWS);
-    if (vocab < 1 || vocab > (1 << 30)) return fm_why(w, FM_ERR_ARG, "vocab %d", vocab);
+    if (vocab < 1 || vocab > (1 << 24)) return fm_why(w, FM_ERR_ARG, "vocab %d", vocab);
     if (top_n < 0 || top_n > 32 || top_n > vocab) return fm_why(w, FM_ERR_ARG, "top_n %d outside 0..min(32, vocab)", top_n);
     return FM_OK;
 }

@@ -480,7 +480,7 @@ FM_API size_t fm_attn_ws_bytes(fm_ctx *ctx, const fm_attn_args *args);
  *   d_entropy[rows]  -sum p log p (a logit of -inf adds nothing)
  *   d_top_ids, d_top_logprobs [rows][top_n]  the top_n largest, equal ones in the order of their ids
  * Each output may be NULL (d_tokens and d_logprob go together, so do the last two).  top_n
- * 0..32 and <= vocab.  A row of -inf alone has log probabilities -inf, entropy 0 and the ids 0..top_n-1;
+ * 0..32 and <= vocab, vocab up to 2^24.  A row of -inf alone has log probabilities -inf, entropy 0 and the ids 0..top_n-1;
  * one that holds a NaN or +inf has NaN everywhere and ids -1.  No counterpart in the reference. */
 FM_API int fm_logprobs_dev(fm_ctx *ctx, const float *d_logits, int rows, int vocab, int64_t row_stride,
                     const int32_t *d_tokens, int top_n, float *d_logprob, float *d_entropy,
