@@ -286,52 +286,99 @@ __device__ __forceinline__ int quantise(double x, float scale) {
     return q > 127.0 ? 127 : q < -127.0 ? -127 : (int)q;
 }
 
+// The same decision in fp32, for a scale well inside the range: the candidate from x * (1 / scale) is off by
+// at most one code, and the sign of x - (code +- 1/2) scale, one fma, tells (an fma's sign is that of the
+// exact value while nothing underflows).
+__device__ __forceinline__ int quantise_fast(float x, float scale, float inv) {
+    float c = rintf(x * inv);
+    const float up = fmaf(-(c + 0.5f), scale, x), down = fmaf(-(c - 0.5f), scale, x);
+    const bool odd = (int)c & 1;
+    if (up > 0.0f || (up == 0.0f && odd)) c += 1.0f;
+    else if (down < 0.0f || (down == 0.0f && odd)) c -= 1.0f;
+    c = fminf(fmaxf(c, -127.0f), 127.0f);
+    return fabsf(x) < INFINITY ? (int)c : x > 0.0f ? 127 : x < 0.0f ? -127 : 0;
+}
+
+constexpr int KV_T = 1024, KV_E = 128 * 256 / 4 / KV_T;    // threads; float4 a thread of the largest page
+
 // One workgroup: the rows that fall into one page of one sequence, for one head, keys (z even) or
-// values.  First their largest magnitude, then the codes; the rows come out of the caches the second time.
+// values.  The rows are read once, into registers: their largest magnitude, then the codes.  Values
+// are turned through LDS, so that both the rows and the page move in whole lines: a page that gets a
+// run of tokens is rewritten (its other bytes as they are); fewer than 16 tokens go byte by byte.
 template <bool BF16>
-__global__ __launch_bounds__(256) void fm_kv_append(FmKv c, FmKvRows x, int D, FmSeqs b) {
-    __shared__ float red[4];
-    const int s = blockIdx.z >> 1, h = blockIdx.y;
+__global__ __launch_bounds__(KV_T) void fm_kv_append(FmKv c, FmKvRows x, int D, FmSeqs b) {
+    __shared__ float red[KV_T / 64];
+    __shared__ __attribute__((aligned(16))) int8_t turn[256 * (128 + 4)];   // [dim][token], rows a bank apart
+    const int s = blockIdx.z >> 1, h = blockIdx.y, tid = threadIdx.x;
     const bool value = blockIdx.z & 1;
-    const int P = c.page_tokens;
+    const int P = c.page_tokens, ps = c.page_shift, LD = P + 4, s4 = 31 - __builtin_clz(D) - 2, d4 = 1 << s4;
     FmKvSpan sp;
     if (!fm_kv_span(fm_seq_rows(b, s), c.len[s], c.page_shift, blockIdx.x, &sp)) return;
     const int page = fm_kv_page(c, s, sp.start);
     if (page < 0) return;
-    const int t0 = sp.t0, t1 = sp.t1;                                  // tokens written, in the page
-    const int64_t row0 = (int64_t)fm_seq_row0(b, s) + sp.row0;       // row of the page's token 0
+    const int t0 = sp.t0, n = sp.t1 - sp.t0;                          // tokens written, in the page
+    const int64_t row0 = (int64_t)fm_seq_row0(b, s) + sp.row0 + t0;  // the first one's row
     const void *src = value ? x.v : x.k;
     const int64_t stride = value ? x.v_stride : x.k_stride;
-    float big = 0.0f;
-    for (int e = threadIdx.x; e < (t1 - t0) * (D / 4); e += 256) {
-        const int t = t0 + e / (D / 4), d = 4 * (e % (D / 4));
-        const fm_v4f w = fm_ld4<BF16>(src, (row0 + t) * stride + (int64_t)h * D + d);
-#pragma unroll
-        for (int i = 0; i < 4; i++) {
-            const float m = fabsf(w[i]);
-            if (m < INFINITY) big = fmaxf(big, m);
-        }
-    }
-    for (int o = 32; o; o >>= 1) big = fmaxf(big, __shfl_xor(big, o));
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = big;
-    __syncthreads();
-    big = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
     float *scale_at = (value ? c.v_scale : c.k_scale) + (int64_t)page * c.kv_heads + h;
     const float old = t0 > 0 ? *scale_at : 0.0f;
+    fm_v4f w[KV_E];
+    float big = 0.0f;
+#pragma unroll
+    for (int u = 0; u < KV_E; u++) {
+        const int e = tid + u * KV_T;
+        if (e < n * d4) w[u] = fm_ld4<BF16>(src, (row0 + (e >> s4)) * stride + (int64_t)h * D + 4 * (e & (d4 - 1)));
+    }
+#pragma unroll
+    for (int u = 0; u < KV_E; u++)
+        if (tid + u * KV_T < n * d4)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const float m = fabsf(w[u][i]);
+                if (m < INFINITY) big = fmaxf(big, m);
+            }
+    for (int o = 32; o; o >>= 1) big = fmaxf(big, __shfl_xor(big, o));
+    if ((tid & 63) == 0) red[tid >> 6] = big;
+    __syncthreads();                                             // (everybody has read the old scale, too)
+#pragma unroll
+    for (int i = 0; i < KV_T / 64; i++) big = fmaxf(big, red[i]);
     const float scale = fmaxf(old, __fdiv_rn(big, 127.0f));
-    __syncthreads();                                             // everybody has read the old scale
-    if (threadIdx.x == 0) *scale_at = scale;
-    int8_t *codes = value ? c.v : c.k;
-    const bool again = t0 > 0 && scale != old;                  // the old codes go to the new scale
-    const int from = again ? 0 : t0;
-    for (int e = threadIdx.x; e < (t1 - from) * D; e += 256) {
-        // keys: dims side by side; values too while reading the rows (a token's bytes lie page_tokens apart)
-        const int t = from + e / D, d = e % D;
-        int8_t *at = codes + (value ? fm_kv_v_at(c, D, page, h, t, d) : fm_kv_k_at(c, D, page, h, t, d));
-        double w;
-        if (t < t0) w = (double)*at * (double)old;
-        else w = (double)fm_ld1<BF16>(src, (row0 + t) * stride + (int64_t)h * D + d);
-        *at = (int8_t)quantise(w, scale);
+    if (tid == 0) *scale_at = scale;
+    int8_t *codes = value ? c.v + fm_kv_v_at(c, D, page, h, 0, 0) : c.k + fm_kv_k_at(c, D, page, h, 0, 0);
+    if (t0 > 0 && scale != old) {                               // the old codes go to the new scale
+        for (int e = tid; e < t0 * D; e += KV_T) {
+            int8_t *at = codes + (value ? (e & (D - 1)) * P + (e >> (s4 + 2)) : e);
+            *at = (int8_t)quantise((double)*at * (double)old, scale);
+        }
+    }
+    const bool fast = scale > 0x1p-100f && scale < 0x1p100f, whole = value && n >= 16;
+    const float inv = 1.0f / scale;
+    if (whole) {                                                // the page as it is
+        __syncthreads();
+        for (int e = 4 * tid; e < P * D; e += 4 * KV_T) *(uint32_t *)(turn + (e >> ps) * LD + (e & (P - 1))) = *(const uint32_t *)(codes + e);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < KV_E; u++) {
+        const int e = tid + u * KV_T;
+        if (e >= n * d4) continue;
+        const int t = t0 + (e >> s4), d = 4 * (e & (d4 - 1));
+        int q[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) q[i] = fast ? quantise_fast(w[u][i], scale, inv) : quantise((double)w[u][i], scale);
+        if (value) {
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                if (whole) turn[(d + i) * LD + t] = (int8_t)q[i];
+                else codes[(d + i) * P + t] = (int8_t)q[i];
+            }
+        } else {
+            *(uint32_t *)(codes + t * D + d) = (q[0] & 255) | (q[1] & 255) << 8 | (q[2] & 255) << 16 | (uint32_t)q[3] << 24;
+        }
+    }
+    if (whole) {
+        __syncthreads();
+        for (int e = 4 * tid; e < P * D; e += 4 * KV_T) *(uint32_t *)(codes + e) = *(const uint32_t *)(turn + (e >> ps) * LD + (e & (P - 1)));
     }
 }
 
@@ -385,8 +432,8 @@ extern "C" int fm_launch_kv(const FmKv *c, const FmKvRows *x, const FmSeqs *b, i
         hipLaunchKernelGGL(fm_kv_read, dim3(wg < 1024 ? wg : 1024, c->kv_heads, b->n_seq), dim3(256), 0, st, *c, *x, D, *b);
     } else {
         const dim3 grid((most + c->page_tokens - 2) / c->page_tokens + 1, c->kv_heads, 2 * b->n_seq);
-        if (bf16) hipLaunchKernelGGL(fm_kv_append<true>, grid, dim3(256), 0, st, *c, *x, D, *b);
-        else hipLaunchKernelGGL(fm_kv_append<false>, grid, dim3(256), 0, st, *c, *x, D, *b);
+        if (bf16) hipLaunchKernelGGL(fm_kv_append<true>, grid, dim3(KV_T), 0, st, *c, *x, D, *b);
+        else hipLaunchKernelGGL(fm_kv_append<false>, grid, dim3(KV_T), 0, st, *c, *x, D, *b);
     }
     return hipGetLastError() == hipSuccess ? FM_OK : FM_ERR_HIP;
 }
