@@ -45,48 +45,93 @@ __device__ __forceinline__ fm_v8h codes_f16(uint32_t lo, uint32_t hi) {
     return r.h;
 }
 
-// A wave's columns: running maximum (of scores in units of log2), sum and output, and the step that
-// adds 64 keys.
-template <int D, int NP>
+// The pages of a lane's two runs of 16 keys: that of the tile rows it loads (run r / 4) and that of its
+// scores and of V (run g).  The table is read on every path and a step ahead, its entry judged when it
+// is used: whoever looks at a load's result waits for all that were issued before it.
+struct Runs {
+    int k, v;        // table entries
+    __device__ __forceinline__ void load(const FmKv &c, const int32_t *table, int pos0) {
+        const int lane = threadIdx.x & 63;
+        k = table[min((pos0 + 16 * ((lane & 15) >> 2)) >> c.page_shift, c.max_pages - 1)];
+        v = table[min((pos0 + 16 * (lane >> 4)) >> c.page_shift, c.max_pages - 1)];
+    }
+    // page, or -1 for one that is not there
+    static __device__ __forceinline__ int judge(const FmKv &c, int entry, int pos) {
+        return (pos >> c.page_shift) < c.max_pages && entry >= 0 && entry < c.n_pages ? entry : -1;
+    }
+    __device__ __forceinline__ int k_page(const FmKv &c, int pos0) const { return judge(c, k, pos0 + 16 * ((threadIdx.x & 15) >> 2)); }
+    __device__ __forceinline__ int v_page(const FmKv &c, int pos0) const { return judge(c, v, pos0 + 16 * ((threadIdx.x & 63) >> 4)); }
+};
+
+// A wave's columns: running maximum (of scores in units of log2), sum and output, the codes of the step
+// in hand, and the step.  The queries lie in LDS as operands [piece][k step][lane], the same for the
+// workgroup's waves: registers go to the codes in flight.
+template <int D, int NP, bool ONCE>
 struct Columns {
     static constexpr int KS = D / 32, DT = D / 16;
-    fm_v8h q[NP][KS];
     fm_v4f o[DT];
     float m, l, qscale;      // qscale: takes a score back from the power of two in q
     int ref;                 // o is held in units of 2^ref, a power of two above every value scale seen
+    fm_v4u kc[D / 64][4], vc[DT];
+    float ks, vs;
 
-    // lane 16 g + column: dims 64 c + 16 g + 8 hh + j are element j of k step 2 c + hh
+    // (codes that nobody else reads are not kept in the caches)
+    static __device__ __forceinline__ fm_v4u ld(const int8_t *p) {
+        if constexpr (ONCE) return __builtin_nontemporal_load((const fm_v4u *)p);
+        else return *(const fm_v4u *)p;
+    }
+
+    // Lane 16 g + column: dims 64 c + 16 g + 8 hh + j are element j of k step 2 c + hh.  Each wave fetches and
+    // writes a quarter of the k steps (D 64: the first two waves a half); the columns' largest elements meet in LDS.
+    // (A column that is not there holds the first row's: nothing of it is used.)
+    static constexpr int MY = (KS + 3) / 4;
+    fm_v4f x[MY][2];
     template <bool BF16>
-    __device__ __forceinline__ void load_q(const void *base, int64_t at, bool there, float scale_log2) {
-        const int g = (threadIdx.x & 63) >> 4;
-        fm_v4f x[KS][2];
-        float big = 0.0f;
+    __device__ __forceinline__ void fetch_q(const void *base, int64_t at) {
+        const int g = (threadIdx.x & 63) >> 4, wave = threadIdx.x >> 6;
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+        for (int u = 0; u < MY; u++)
 #pragma unroll
             for (int h = 0; h < 2; h++) {
-                x[s][h] = there ? fm_ld4<BF16>(base, at + 64 * (s >> 1) + 16 * g + 8 * (s & 1) + 4 * h) : fm_v4f{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int i = 0; i < 4; i++) big = fmaxf(big, fabsf(x[s][h][i]));
+                const int s = min(wave * MY + u, KS - 1);
+                x[u][h] = fm_ld4<BF16>(base, at + 64 * (s >> 1) + 16 * g + 8 * (s & 1) + 4 * h);
             }
+    }
+    __device__ __forceinline__ void put_q(float scale_log2, int wave, fm_v8h *q, float (*s_big)[16]) {
+        const int lane = threadIdx.x & 63, col = lane & 15;
+        float big = 0.0f;
+#pragma unroll
+        for (int u = 0; u < MY; u++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) big = fmaxf(big, fabsf(x[u][h][i]));
         big = fmaxf(big, __shfl_xor(big, 16));
         big = fmaxf(big, __shfl_xor(big, 32));
+        if (lane < 16) s_big[wave][col] = big;
+        lds_barrier();
+        big = fmaxf(fmaxf(s_big[0][col], s_big[1][col]), fmaxf(s_big[2][col], s_big[3][col]));
         int e = (int)(__float_as_uint(big) >> 23 & 255) - 127;
         e = e > 100 ? 100 : e < -100 ? -100 : e;      // (zeros, infinities: any power will do)
         const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
         qscale = __uint_as_float((uint32_t)(127 - 8 + e) << 23) * scale_log2;
 #pragma unroll
-        for (int s = 0; s < KS; s++)
+        for (int u = 0; u < MY; u++) {
+            fm_v8h v[NP];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                float f = x[s][j >> 2][j & 3] * up;
+                float f = x[u][j >> 2][j & 3] * up;
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
                     const _Float16 hv = (_Float16)f;
-                    q[p][s][j] = hv;
+                    v[p][j] = hv;
                     f -= (float)hv;
                 }
             }
+            const int s = min(wave * MY + u, KS - 1);
+#pragma unroll
+            for (int p = 0; p < NP; p++) q[(p * KS + s) * 64 + lane] = v[p];
+        }
         m = -INFINITY;
         l = 0.0f;
         ref = -100;
@@ -94,37 +139,72 @@ struct Columns {
         for (int d = 0; d < DT; d++) o[d] = fm_v4f{0.f, 0.f, 0.f, 0.f};
     }
 
-    // 64 keys from position pos0; the column sees keys below `limit`
-    __device__ __forceinline__ void step(const FmKv &c, int s, int h, int pos0, int limit) {
+    // (a page that is not there is read as page 0 and masked)
+    __device__ __forceinline__ const int8_t *k_base(const FmKv &c, const Runs &p, int h, int pos0) const {
         const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-        // keys of tile rows: run r / 4 of 16 keys; of scores and of V: run g
-        const int kpos = pos0 + 16 * (r >> 2), vpos = pos0 + 16 * g;
-        const int kp = fm_kv_page(c, s, kpos), vp = fm_kv_page(c, s, vpos);
-        // (a page that is not there is read as page 0 and masked)
-        const int8_t *kb = c.k + fm_kv_k_at(c, D, kp < 0 ? 0 : kp, h, kpos + (r & 3), 16 * g);
-        const int8_t *vb = c.v + fm_kv_v_at(c, D, vp < 0 ? 0 : vp, h, vpos, r);
-        const bool live = vp >= 0 && vpos < limit;
-        float ks = 0.0f, vs = 0.0f;
-        if (live) {
-            ks = c.k_scale[(int64_t)vp * c.kv_heads + h];
-            vs = c.v_scale[(int64_t)vp * c.kv_heads + h];
-        }
-        fm_v4f sc[4];
-#pragma unroll
-        for (int t = 0; t < 4; t++) sc[t] = fm_v4f{0.f, 0.f, 0.f, 0.f};
+        return c.k + fm_kv_k_at(c, D, max(p.k_page(c, pos0), 0), h, pos0 + 16 * (r >> 2) + (r & 3), 16 * g);
+    }
+    __device__ __forceinline__ const int8_t *v_base(const FmKv &c, const Runs &p, int h, int pos0) const {
+        const int lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+        return c.v + fm_kv_v_at(c, D, max(p.v_page(c, pos0), 0), h, pos0 + 16 * g, r);
+    }
+    __device__ __forceinline__ void load_k(const int8_t *kb, int d, int t) { kc[d][t] = ld(kb + 4 * t * D + 64 * d); }
+    __device__ __forceinline__ void load_v(const FmKv &c, const int8_t *vb, int d) { vc[d] = ld(vb + 16 * d * c.page_tokens); }
+    __device__ __forceinline__ void load_scales(const FmKv &c, const Runs &p, int h, int pos0) {
+        const int64_t at = (int64_t)max(p.v_page(c, pos0), 0) * c.kv_heads + h;
+        ks = c.k_scale[at];
+        vs = c.v_scale[at];
+    }
+    __device__ __forceinline__ void first(const FmKv &c, const Runs &p, int h, int pos0, bool any) {
+        if (!any) return;
+        const int8_t *kb = k_base(c, p, h, pos0), *vb = v_base(c, p, h, pos0);
 #pragma unroll
         for (int d = 0; d < D / 64; d++)
 #pragma unroll
+            for (int t = 0; t < 4; t++) load_k(kb, d, t);
+        load_scales(c, p, h, pos0);
+#pragma unroll
+        for (int d = 0; d < DT; d++) load_v(c, vb, d);
+    }
+
+    // 64 keys from position pos0, in the pages `now`; the column sees keys below `limit`.  MORE: each code register
+    // takes the next step's (positions pos1, pages `next`) as soon as it is used.
+    template <bool MORE>
+    __device__ __forceinline__ void step(const FmKv &c, int h, int pos0, int limit, const Runs &now, int pos1, const Runs &next,
+                                         const fm_v8h *q) {
+        const int g = (threadIdx.x & 63) >> 4;
+        const int vpos = pos0 + 16 * g;
+        const int8_t *kb = k_base(c, next, h, pos1), *vb = v_base(c, next, h, pos1);
+        fm_v4f sc[4];
+#pragma unroll
+        for (int t = 0; t < 4; t++) sc[t] = fm_v4f{0.f, 0.f, 0.f, 0.f};
+        // (the scheduler may not move loads ahead of the uses whose registers they take: it would need both)
+#pragma unroll
+        for (int d = 0; d < D / 64; d++) {
+            fm_v8h b0[NP], b1[NP];
+#pragma unroll
+            for (int p = 0; p < NP; p++) b0[p] = q[(p * KS + 2 * d) * 64], b1[p] = q[(p * KS + 2 * d + 1) * 64];
+#pragma unroll
             for (int t = 0; t < 4; t++) {
-                const uint4 w = *(const uint4 *)(kb + 4 * t * D + 64 * d);
-                const fm_v8h a0 = codes_f16(w.x, w.y), a1 = codes_f16(w.z, w.w);
+                const fm_v8h a0 = codes_f16(kc[d][t][0], kc[d][t][1]), a1 = codes_f16(kc[d][t][2], kc[d][t][3]);
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
-                    sc[t] = mfma(a0, q[p][2 * d], sc[t]);
-                    sc[t] = mfma(a1, q[p][2 * d + 1], sc[t]);
+                    sc[t] = mfma(a0, b0[p], sc[t]);
+                    sc[t] = mfma(a1, b1[p], sc[t]);
                 }
             }
-        const float f = ks * qscale;
+            if constexpr (MORE) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int t = 0; t < 4; t++) load_k(kb, d, t);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+        // (scales behind the last key may be anything)
+        const bool live = now.v_page(c, pos0) >= 0 && vpos < limit;
+        const float f = (live ? ks : 0.0f) * qscale;
+        float v_scale = live ? vs : 0.0f;
+        if constexpr (MORE) load_scales(c, next, h, pos1);
         float top = -INFINITY;
 #pragma unroll
         for (int t = 0; t < 4; t++)
@@ -141,13 +221,13 @@ struct Columns {
         const float keep = exp2f(m - base);
         m = m1;
         l *= keep;
-        int up = live ? (int)(__float_as_uint(vs) >> 23 & 255) - 126 : -100;
+        int up = live ? (int)(__float_as_uint(v_scale) >> 23 & 255) - 126 : -100;
         up = max(ref, min(up, 100));
         up = max(up, __shfl_xor(up, 16));
         up = max(up, __shfl_xor(up, 32));
         const float keep_o = ldexpf(keep, ref - up);
         ref = up;
-        vs = ldexpf(vs, -up);
+        v_scale = ldexpf(v_scale, -up);
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] *= keep_o;
         fm_v8h p8[NP][2];
@@ -157,8 +237,7 @@ struct Columns {
             for (int i = 0; i < 4; i++) {
                 const float e = exp2f(sc[t][i] - base + P_SHIFT);
                 l += e;
-                // (a scale behind the last key may be anything: 0 * NaN must not come in)
-                float pv = e == 0.0f ? 0.0f : e * vs;
+                float pv = e * v_scale;
                 const int j = 4 * (t & 1) + i;
 #pragma unroll
                 for (int p = 0; p < NP; p++) {
@@ -168,111 +247,201 @@ struct Columns {
                 }
             }
 #pragma unroll
-        for (int d = 0; d < DT; d++) {
-            const uint4 w = *(const uint4 *)(vb + (int64_t)16 * d * c.page_tokens);
-            const fm_v8h a0 = codes_f16(w.x, w.y), a1 = codes_f16(w.z, w.w);
+        for (int d0 = 0; d0 < DT; d0 += 4) {
 #pragma unroll
-            for (int p = 0; p < NP; p++) {
-                o[d] = mfma(a0, p8[p][0], o[d]);
-                o[d] = mfma(a1, p8[p][1], o[d]);
+            for (int d = d0; d < d0 + 4; d++) {
+                const fm_v8h a0 = codes_f16(vc[d][0], vc[d][1]), a1 = codes_f16(vc[d][2], vc[d][3]);
+#pragma unroll
+                for (int p = 0; p < NP; p++) {
+                    o[d] = mfma(a0, p8[p][0], o[d]);
+                    o[d] = mfma(a1, p8[p][1], o[d]);
+                }
+            }
+            if constexpr (MORE) {
+                __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                for (int d = d0; d < d0 + 4; d++) load_v(c, vb, d);
+                __builtin_amdgcn_sched_barrier(0);
             }
         }
     }
 };
 
-// One workgroup: a chunk of the keys, 16 columns of one (sequence, cache head).  Its four waves take
-// steps of 64 keys in turn and are joined through LDS.
-template <int D, bool BF16>
-__global__ __launch_bounds__(256) void fm_attn_cols(FmKv c, FmAttn a, FmSeqs b) {
+// The steps of all sequences, heads and tiles are numbered through and shared out evenly: sequences
+// of a batch differ in length by any factor, and only the device knows the lengths.  Every workgroup adds
+// them up itself.  first[s]: steps before sequence s.  256 threads.
+struct Shares {
+    int first[FM_MAX_SEQ + 1], len[FM_MAX_SEQ];
+    int of_wave[4];
+};
+__device__ __forceinline__ void add_steps(const FmKv &c, const FmAttn &a, const FmSeqs &b, Shares &sh) {
+    const int t = threadIdx.x, lane = t & 63;
+    int n = 0;
+    if (t < b.n_seq) {
+        const int len = c.len[t];
+        sh.len[t] = len;
+        n = c.kv_heads * fm_attn_head_steps(fm_seq_rows(b, t), a.group, len, a.max_len);
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const int up = __shfl_up(n, o);
+        if (lane >= o) n += up;
+    }
+    if (lane == 63) sh.of_wave[t >> 6] = n;
+    __syncthreads();
+    for (int w = 0; w < t >> 6; w++) n += sh.of_wave[w];
+    if (t < b.n_seq) sh.first[t + 1] = n;
+    if (t == 0) sh.first[0] = 0;
+    __syncthreads();
+}
+
+// One workgroup: its share of the steps, tile by tile.  The four waves take a tile's steps in turn and are
+// joined through LDS.
+template <int D, bool BF16, bool ONCE>
+__global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_cols(FmKv c, FmAttn a, FmSeqs b) {
     constexpr int NP = BF16 ? 1 : 2, DT = D / 16;
     __shared__ float s_o[3][DT][64][4];
     __shared__ float s_m[4][16], s_l[4][16];
-    const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
-    const int s = blockIdx.z, h = blockIdx.y, chunk = blockIdx.x % a.n_chunks, tile = blockIdx.x / a.n_chunks;
-    const int n = fm_seq_rows(b, s), n_cols = n * a.group;
-    if (tile * COLS >= n_cols) return;
-    const int cc = tile * COLS + col;
-    const bool there = cc < n_cols;
-    const int i = there ? cc / a.group : 0, qh = h * a.group + (there ? cc % a.group : 0);
-    const int len = c.len[s];
-    const int seen = min(len, a.max_len);
-    const int limit = there ? min(seen, len - n + i + 1) : 0;
-    // the tile's last column sees the most
-    const int last = min(n_cols - 1, tile * COLS + COLS - 1) / a.group;
-    const int end = min(seen, len - n + last + 1);
-    const int k0 = chunk * a.chunk, k1 = min(end, k0 + a.chunk);
-    if (k0 >= end && chunk) return;
-
-    const int64_t row = fm_seq_row0(b, s) + i;
-    Columns<D, NP> w;
-    w.template load_q<BF16>(a.q, row * a.q_stride + (int64_t)qh * D, there, a.scale_log2);
-    for (int pos = k0 + wave * BK; pos < k1; pos += 4 * BK) w.step(c, s, h, pos, limit);
-    w.l += __shfl_xor(w.l, 16);
-    w.l += __shfl_xor(w.l, 32);
-
-    // join the waves: wave 0 takes the others' sums at the common maximum
-    if (g == 0) s_m[wave][col] = w.m, s_l[wave][col] = w.l;
-    __syncthreads();
-    const float m = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
-    const float base = m == -INFINITY ? 0.0f : m;
-    const float f = ldexpf(exp2f(w.m - base), w.ref);
-#pragma unroll
-    for (int d = 0; d < DT; d++) w.o[d] *= f;
-    if (wave) {
-#pragma unroll
-        for (int d = 0; d < DT; d++) *(fm_v4f *)s_o[wave - 1][d][lane] = w.o[d];
+    __shared__ fm_v8h s_q[NP * (D / 32) * 64];
+    __shared__ Shares sh;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
+    add_steps(c, a, b, sh);
+    const int total = sh.first[b.n_seq], share = fm_attn_share(total, a.groups);
+    if (blockIdx.x == 0)                                         // for the join
+        for (int i = threadIdx.x; i <= b.n_seq; i += 256) a.first[i] = sh.first[i];
+    int at = blockIdx.x * share;
+    const int stop = min(total, at + share);
+    if (at >= stop) return;
+    int s = 0;
+    for (int hi = b.n_seq; hi - s > 1;) {
+        const int mid = (s + hi) / 2;
+        if (sh.first[mid] <= at) s = mid;
+        else hi = mid;
     }
-    __syncthreads();
-    if (wave || !there) return;
-    float l = 0.0f;
+    while (at < stop) {
+        while (sh.first[s + 1] <= at) s++;                       // (sequences without rows have no steps)
+        const int n = fm_seq_rows(b, s), len = __builtin_amdgcn_readfirstlane(sh.len[s]), per_head = (sh.first[s + 1] - sh.first[s]) / c.kv_heads;
+        const int h = (at - sh.first[s]) / per_head;
+        int off = (at - sh.first[s]) - h * per_head, tile = 0, steps;
+        while (off >= (steps = fm_attn_steps(n, a.group, len, a.max_len, tile))) off -= steps, tile++;
+        const int s0 = off, s1 = min(steps, off + stop - at);    // this workgroup's steps of the tile
+        at += s1 - s0;
+
+        const int n_cols = n * a.group, cc = tile * COLS + col;
+        const bool there = cc < n_cols;
+        const int i = there ? cc / a.group : 0, qh = h * a.group + (there ? cc % a.group : 0);
+        const int limit = there ? min(min(len, a.max_len), len - n + i + 1) : 0;
+        const int64_t row = fm_seq_row0(b, s) + i;
+        const int32_t *table = c.pages + (int64_t)s * c.max_pages;
+        Columns<D, NP, ONCE> w;
+        Runs now, next;
+        int pos = (s0 + wave) * BK;
+        const int end = s1 * BK;
+        const bool any = pos < end;
+        now.load(c, table, any ? pos : 0);
+        next.load(c, table, pos + 4 * BK < end ? pos + 4 * BK : 0);
+        // (the queries first: who looks at a load's result waits for all that were issued before it)
+        w.template fetch_q<BF16>(a.q, row * a.q_stride + (int64_t)qh * D);
+        w.first(c, now, h, any ? pos : 0, any);
+        w.put_q(a.scale_log2, wave, s_q, s_m);
+        lds_barrier();
+        const fm_v8h *q = s_q + lane;
+        if (any) {
+            for (; pos + 4 * BK < end; pos += 4 * BK) {
+                Runs later;
+                later.load(c, table, min(pos + 8 * BK, end - BK));
+                w.template step<true>(c, h, pos, limit, now, pos + 4 * BK, next, q);
+                now = next;
+                next = later;
+            }
+            w.template step<false>(c, h, pos, limit, now, pos, now, q);
+        }
+        w.l += __shfl_xor(w.l, 16);
+        w.l += __shfl_xor(w.l, 32);
+
+        // join the waves: wave 0 takes the others' sums at the common maximum
+        __syncthreads();                                          // (the last tile's sums have been read)
+        if (g == 0) s_m[wave][col] = w.m, s_l[wave][col] = w.l;
+        __syncthreads();
+        const float m = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
+        const float base = m == -INFINITY ? 0.0f : m;
+        const float f = ldexpf(exp2f(w.m - base), w.ref);
 #pragma unroll
-    for (int v = 0; v < 4; v++) l = fmaf(s_l[v][col], exp2f(s_m[v][col] - base), l);
+        for (int d = 0; d < DT; d++) w.o[d] *= f;
+        if (wave) {
 #pragma unroll
-    for (int d = 0; d < DT; d++)
+            for (int d = 0; d < DT; d++) *(fm_v4f *)s_o[wave - 1][d][lane] = w.o[d];
+        }
+        __syncthreads();
+        if (wave) continue;
+        float l = 0.0f;
 #pragma unroll
-        for (int v = 0; v < 3; v++) w.o[d] += *(const fm_v4f *)s_o[v][d][lane];
-    // register i of tile d: dim 16 d + 4 g + i
-    if (a.n_chunks == 1) {
-        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        const int64_t at = (row * a.q_heads + qh) * D + 4 * g;
+        for (int v = 0; v < 4; v++) l = fmaf(s_l[v][col], exp2f(s_m[v][col] - base), l);
 #pragma unroll
-        for (int d = 0; d < DT; d++) fm_st4<BF16>(a.out, at + 16 * d, w.o[d] * inv);
-    } else {
-        const int64_t at = ((row * a.q_heads + qh) * a.n_chunks + chunk);
+        for (int d = 0; d < DT; d++)
 #pragma unroll
-        for (int d = 0; d < DT; d++) *(fm_v4f *)(a.part_o + at * D + 16 * d + 4 * g) = w.o[d];
-        if (g == 0) a.part_ml[2 * at] = m, a.part_ml[2 * at + 1] = l;
+            for (int v = 0; v < 3; v++) w.o[d] += *(const fm_v4f *)s_o[v][d][lane];
+        // register i of tile d: dim 16 d + 4 g + i
+        if (s0 == 0 && s1 == steps) {
+            if (!there) continue;
+            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+            const int64_t to = (row * a.q_heads + qh) * D + 4 * g;
+#pragma unroll
+            for (int d = 0; d < DT; d++) fm_st4<BF16>(a.out, to + 16 * d, w.o[d] * inv);
+        } else {
+            const int64_t to = (int64_t)fm_attn_slot(blockIdx.x, s0) * COLS + col;
+#pragma unroll
+            for (int d = 0; d < DT; d++) *(fm_v4f *)(a.part_o + to * D + 16 * d + 4 * g) = w.o[d];
+            if (g == 0) a.part_ml[2 * to] = m, a.part_ml[2 * to + 1] = l;
+        }
     }
 }
 
-// joins the chunks of one (row, query head); one wave each, D / 64 dims a lane
+// Joins the parts of one tile that several workgroups took: a wave per column (four workgroups a tile),
+// D / 64 dims a lane.
 template <int D, bool BF16>
-__global__ __launch_bounds__(64) void fm_attn_join(FmKv c, FmAttn a, FmSeqs b) {
-    const int s = blockIdx.z, i = blockIdx.y, qh = blockIdx.x, lane = threadIdx.x;
+__global__ __launch_bounds__(256) void fm_attn_join(FmKv c, FmAttn a, FmSeqs b) {
+    const int s = blockIdx.z, h = blockIdx.y, tile = blockIdx.x >> 2, lane = threadIdx.x & 63;
     const int n = fm_seq_rows(b, s);
-    if (i >= n) return;
-    const int len = c.len[s];
-    // the chunks that the row's column tile ran
-    const int tile = (i * a.group + qh % a.group) / COLS;
-    const int last = min(n * a.group - 1, tile * COLS + COLS - 1) / a.group;
-    const int end = min(min(len, a.max_len), len - n + last + 1);
-    const int chunks = end <= 0 ? 1 : (end + a.chunk - 1) / a.chunk;
-    const int64_t row = fm_seq_row0(b, s) + i, at = (row * a.q_heads + qh) * a.n_chunks;
+    if (tile >= fm_attn_tiles(n, a.group)) return;
+    const int len = c.len[s], from = a.first[s], per_head = (a.first[s + 1] - from) / c.kv_heads;
+    const int share = fm_attn_share(a.first[b.n_seq], a.groups), steps = fm_attn_steps(n, a.group, len, a.max_len, tile);
+    int at = from + h * per_head;
+    for (int t = 0; t < tile; t++) at += fm_attn_steps(n, a.group, len, a.max_len, t);
+    const int g0 = at / share, g1 = (at + steps - 1) / share;
+    if (g0 == g1) return;
+    const int col = 4 * (blockIdx.x & 3) + (threadIdx.x >> 6), cc = tile * COLS + col;
+    if (cc >= n * a.group) return;
+    const int64_t row = fm_seq_row0(b, s) + cc / a.group;
+    auto slot = [&](int g) { return (int64_t)fm_attn_slot(g, g * share - at) * COLS + col; };
+    // a lane per part: its weight e^(m - base)
     float m = -INFINITY;
-    for (int k = 0; k < chunks; k++) m = fmaxf(m, a.part_ml[2 * (at + k)]);
+    for (int g = g0 + lane; g <= g1; g += 64) m = fmaxf(m, a.part_ml[2 * slot(g)]);
+    for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     const float base = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, o[D / 64];
 #pragma unroll
     for (int d = 0; d < D / 64; d++) o[d] = 0.0f;
-    for (int k = 0; k < chunks; k++) {
-        const float f = exp2f(a.part_ml[2 * (at + k)] - base);
-        l = fmaf(f, a.part_ml[2 * (at + k) + 1], l);
+    for (int g = g0; g <= g1; g += 64) {
+        const int parts = min(64, g1 + 1 - g);
+        float f = 0.0f;
+        if (lane < parts) {
+            f = exp2f(a.part_ml[2 * slot(g + lane)] - base);
+            l = fmaf(f, a.part_ml[2 * slot(g + lane) + 1], l);
+        }
+#pragma unroll 4
+        for (int k = 0; k < parts; k++) {
+            const float *p = a.part_o + slot(g + k) * D + lane;
+            const float fk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), k));
 #pragma unroll
-        for (int d = 0; d < D / 64; d++) o[d] = fmaf(f, a.part_o[(at + k) * D + 64 * d + lane], o[d]);
+            for (int d = 0; d < D / 64; d++) o[d] = fmaf(fk, p[64 * d], o[d]);
+        }
     }
+    l = fm_group_sum<64>(l);
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int d = 0; d < D / 64; d++) fm_st1<BF16>(a.out, (row * a.q_heads + qh) * D + 64 * d + lane, o[d] * inv);
+    for (int d = 0; d < D / 64; d++)
+        fm_st1<BF16>(a.out, (row * a.q_heads + h * a.group + cc % a.group) * D + 64 * d + lane, o[d] * inv);
 }
 
 // ---- the cache's rows --------------------------------------------------------------------------
@@ -404,9 +573,10 @@ __global__ __launch_bounds__(256) void fm_kv_read(FmKv c, FmKvRows x, int D, FmS
 
 template <int D, bool BF16>
 void launch_cols(const FmKv &c, const FmAttn &a, const FmSeqs &b, hipStream_t st) {
-    hipLaunchKernelGGL((fm_attn_cols<D, BF16>), dim3(a.n_chunks * a.n_tiles, c.kv_heads, b.n_seq), dim3(256), 0, st, c, a, b);
-    if (a.n_chunks > 1)
-        hipLaunchKernelGGL((fm_attn_join<D, BF16>), dim3(a.q_heads, fm_most_rows(b), b.n_seq), dim3(64), 0, st, c, a, b);
+    if (a.n_tiles == 1) hipLaunchKernelGGL((fm_attn_cols<D, BF16, true>), dim3(a.groups), dim3(256), 0, st, c, a, b);
+    else hipLaunchKernelGGL((fm_attn_cols<D, BF16, false>), dim3(a.groups), dim3(256), 0, st, c, a, b);
+    if (a.groups > 1)
+        hipLaunchKernelGGL((fm_attn_join<D, BF16>), dim3(4 * a.n_tiles, c.kv_heads, b.n_seq), dim3(256), 0, st, c, a, b);
 }
 
 }  // namespace
@@ -414,7 +584,8 @@ void launch_cols(const FmKv &c, const FmAttn &a, const FmSeqs &b, hipStream_t st
 extern "C" int fm_launch_attn(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int bf16, void *ws, hipStream_t st) {
     if (a->n_tiles < 1) return FM_OK;
     a->part_o = (float *)ws;
-    a->part_ml = a->part_o ? a->part_o + (size_t)fm_all_rows(*b) * a->q_heads * a->n_chunks * D : nullptr;
+    a->part_ml = a->part_o + (size_t)2 * a->groups * COLS * D;
+    a->first = (int *)(a->part_ml + (size_t)2 * a->groups * COLS * 2);
     switch (D) {
         case 64: bf16 ? launch_cols<64, true>(*c, *a, *b, st) : launch_cols<64, false>(*c, *a, *b, st); break;
         case 128: bf16 ? launch_cols<128, true>(*c, *a, *b, st) : launch_cols<128, false>(*c, *a, *b, st); break;

@@ -131,11 +131,6 @@ __device__ __forceinline__ fm_v4f mfma16(fm_v4f x, fm_v4f y, fm_v4f c) {
     return c;
 }
 
-// Barrier behind this wave's LDS writes that leaves loads from memory in flight.
-__device__ __forceinline__ void lds_barrier() {
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-}
-
 __device__ __forceinline__ double lane_of(double v, int lane) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v);
     const uint32_t lo = __builtin_amdgcn_readlane((int)(uint32_t)b, lane), hi = __builtin_amdgcn_readlane((int)(b >> 32), lane);

@@ -11,6 +11,7 @@ typedef float fm_v4f __attribute__((ext_vector_type(4)));
 typedef short fm_v8s __attribute__((ext_vector_type(8)));
 typedef _Float16 fm_v8h __attribute__((ext_vector_type(8)));
 typedef _Float16 fm_v2h __attribute__((ext_vector_type(2)));
+typedef uint32_t fm_v4u __attribute__((ext_vector_type(4)));
 
 __device__ __forceinline__ float fm_bf16_f(uint16_t b) { return __uint_as_float((uint32_t)b << 16); }
 // round to nearest even; a NaN stays one
@@ -46,6 +47,11 @@ __device__ __forceinline__ void fm_st4(void *p, int64_t at, fm_v4f v) {
     } else {
         *(fm_v4f *)((float *)p + at) = v;
     }
+}
+
+// Barrier behind this wave's LDS writes that leaves loads from memory in flight.
+__device__ __forceinline__ void lds_barrier() {
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
 }
 
 #endif  // __HIPCC__

@@ -175,13 +175,45 @@ struct FmAttn {
     int q_heads, group;     // query heads per cache head
     float scale_log2;       // scale * log2(e)
     int max_len;            // keys from here on are not seen, at most max_pages * page_tokens
-    int chunk;              // keys of one workgroup (a multiple of 4 * FM_ATTN_KEYS)
-    int n_chunks;           // workgroups over the longest sequence
     int n_tiles;            // column tiles of the sequence with the most rows
+    int groups;             // workgroups that share the steps
     float *part_o, *part_ml;
+    int *first;             // steps before each sequence, for the join
 };
 #define FM_ATTN_KEYS 64     // keys of a wave's step
 #define FM_ATTN_COLS 16     // columns of a tile
+#define FM_ATTN_WAVES 4     // waves of a workgroup
+
+// ---- attention's steps and who takes them --------------------------------------------------
+// A sequence of n rows has, per cache head, tiles of 16 columns (row * group + query head of the group);
+// a tile's steps are those of 64 keys up to the last one its last column sees, at least one
+// (somebody has to write the zeros of a row that sees nothing).
+FM_HD int fm_attn_tiles(int n, int group) { return (n * group + FM_ATTN_COLS - 1) / FM_ATTN_COLS; }
+FM_HD int fm_attn_end(int n, int group, int len, int max_len, int tile) {
+    const int cols = n * group, col = tile * FM_ATTN_COLS + FM_ATTN_COLS - 1;
+    const int last = (col < cols - 1 ? col : cols - 1) / group, seen = len < max_len ? len : max_len;
+    const int end = len - n + last + 1;
+    return end < seen ? end : seen;
+}
+FM_HD int fm_attn_steps(int n, int group, int len, int max_len, int tile) {
+    const int end = fm_attn_end(n, group, len, max_len, tile);
+    return end <= FM_ATTN_KEYS ? 1 : (end + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS;
+}
+// all tiles of one cache head
+FM_HD int fm_attn_head_steps(int n, int group, int len, int max_len) {
+    int sum = 0;
+    for (int t = 0; t < fm_attn_tiles(n, group); t++) sum += fm_attn_steps(n, group, len, max_len, t);
+    return sum;
+}
+// Steps are numbered sequence by sequence, head by head, tile by tile; workgroup g takes those from
+// g * share on.  A share is at least one step per wave.
+FM_HD int fm_attn_share(int total, int groups) {
+    const int s = (total + groups - 1) / groups;
+    return s < FM_ATTN_WAVES ? FM_ATTN_WAVES : s;
+}
+// Where a workgroup leaves its part of a tile that it does not have whole: only its first tile can
+// have begun in an earlier workgroup, only its last can end in a later one.
+FM_HD int fm_attn_slot(int group, int first_step) { return 2 * group + (first_step > 0 ? 0 : 1); }
 
 // ---- the paged cache's addresses -----------------------------------------------------------
 // the page that holds position `pos` of sequence s, or -1 for one that is not there
@@ -372,22 +404,21 @@ inline int fm_most_rows(const FmSeqs &b) {
 }
 inline int fm_all_rows(const FmSeqs &b) { return b.one_row ? b.n_seq : b.start[b.n_seq]; }
 
-// Attention: chunks of keys so that about four workgroups per CU are there.  Returns the workspace.
+// Workgroups of a CU: heads of 256 take a wave more registers than half a SIMD has (and a spilled one
+// would wait for the codes in flight).
+FM_HDC int fm_attn_per_cu(int D) { return D == 256 ? 1 : 2; }
+// Attention: the workgroups that fit on the chip share the steps, fewer if there cannot be as many.  Returns the
+// workspace: two parts per workgroup and the steps before each sequence.
 inline size_t fm_attn_plan(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int n_cu) {
-    const int step = 4 * FM_ATTN_KEYS;
     const int64_t have = (int64_t)c->max_pages * c->page_tokens;
     if (a->max_len > have) a->max_len = (int)have;
-    a->n_tiles = (int)(((int64_t)fm_most_rows(*b) * a->group + FM_ATTN_COLS - 1) / FM_ATTN_COLS);
-    const int64_t groups = (int64_t)(a->n_tiles > 0 ? a->n_tiles : 1) * b->n_seq * c->kv_heads;
-    const int64_t want = (4 * (int64_t)n_cu + groups - 1) / groups;
-    int64_t chunk = ((int64_t)a->max_len + want - 1) / want;
-    chunk = (chunk + step - 1) / step * step;
-    if (chunk < step) chunk = step;
-    a->chunk = (int)chunk;
-    a->n_chunks = (int)(((int64_t)a->max_len + chunk - 1) / chunk);
-    if (a->n_chunks < 1) a->n_chunks = 1;
-    if (a->n_chunks == 1) return 0;
-    return (size_t)fm_all_rows(*b) * a->q_heads * a->n_chunks * (D + 2) * sizeof(float);
+    a->n_tiles = fm_attn_tiles(fm_most_rows(*b), a->group);
+    int64_t most = 0;
+    for (int s = 0; s < b->n_seq; s++)
+        most += (int64_t)c->kv_heads * fm_attn_tiles(fm_seq_rows(*b, s), a->group) * ((a->max_len + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS + 1);
+    const int64_t groups = (most + FM_ATTN_WAVES - 1) / FM_ATTN_WAVES;
+    a->groups = (int)(groups < 1 ? 1 : groups > fm_attn_per_cu(D) * n_cu ? fm_attn_per_cu(D) * n_cu : groups);
+    return (size_t)2 * a->groups * FM_ATTN_COLS * (D + 2) * sizeof(float) + (FM_MAX_SEQ + 1) * sizeof(int);
 }
 
 inline int fm_attn_check(FmWhy *w, const fm_attn_args *p, int n_cu, FmKv *k, FmAttn *a, FmSeqs *b, size_t *ws) {

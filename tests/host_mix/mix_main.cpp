@@ -184,6 +184,39 @@ static void refuse_logprobs() {
     CHECK(fm_logprob_args_check(&w, p, 3, 100, 100, p, 5, at((1 << 20) + 2), p, p, p) == FM_ERR_ARG);
 }
 
+// ---- attention's steps: shared out once each, the parts of a tile found again by the join
+static void share_out(const FmKv &c, const FmAttn &a, const FmSeqs &b, int D, size_t ws) {
+    std::vector<int> first(b.n_seq + 1, 0);
+    for (int s = 0; s < b.n_seq; s++)
+        first[s + 1] = first[s] + c.kv_heads * fm_attn_head_steps(fm_seq_rows(b, s), a.group, c.len[s], a.max_len);
+    const int total = first[b.n_seq], share = fm_attn_share(total, a.groups);
+    CHECK((int64_t)share * a.groups >= total);
+    CHECK(ws == (size_t)2 * a.groups * FM_ATTN_COLS * (D + 2) * 4 + (FM_MAX_SEQ + 1) * 4);
+    std::set<int> written;      // slots of parts
+    int seen = 0;
+    for (int s = 0; s < b.n_seq; s++) {
+        const int n = fm_seq_rows(b, s);
+        for (int h = 0; h < c.kv_heads; h++)
+            for (int t = 0; t < fm_attn_tiles(n, a.group); t++) {
+                const int steps = fm_attn_steps(n, a.group, c.len[s], a.max_len, t), at = seen;
+                const int end = fm_attn_end(n, a.group, c.len[s], a.max_len, t);
+                CHECK(steps >= 1 && end <= steps * FM_ATTN_KEYS && end <= a.max_len && (steps == 1 || end > (steps - 1) * FM_ATTN_KEYS));
+                seen += steps;
+                const int g0 = at / share, g1 = (at + steps - 1) / share;
+                CHECK(g1 < a.groups);
+                if (g0 == g1) continue;
+                for (int g = g0; g <= g1; g++) {
+                    // what the workgroup has of the tile, and where both kernels put it
+                    const int lo = g * share > at ? g * share - at : 0;
+                    const int slot = fm_attn_slot(g, lo);
+                    CHECK(slot == fm_attn_slot(g, g * share - at) && slot < 2 * a.groups);
+                    CHECK(written.insert(slot).second);
+                }
+            }
+    }
+    CHECK(seen == total);
+}
+
 // ---- the cache's addresses
 static void walk(int n_seq, int kv, int D, int P, int group) {
     const int n_pages = 1 + rnd(12), max_pages = 1 + rnd(6);
@@ -204,13 +237,12 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
     b.n_seq = n_seq;
     for (int s = 0; s <= n_seq; s++) b.start[s] = start[s];
     const size_t ws = fm_attn_plan(&c, &a, &b, D, 1 + rnd(64));
-    CHECK(a.max_len <= max_pages * P && a.chunk % (4 * FM_ATTN_KEYS) == 0 && a.n_chunks >= 1);
-    CHECK((int64_t)a.chunk * a.n_chunks >= a.max_len);
-    CHECK(a.n_chunks == 1 || ws == (size_t)start[n_seq] * a.q_heads * a.n_chunks * (D + 2) * 4);
+    CHECK(a.max_len <= max_pages * P && a.groups >= 1);
+    share_out(c, a, b, D, ws);
     for (int s = 0; s < n_seq; s++)
         for (int h = 0; h < kv; h++)
-            // (every step, also behind the length: a tile's last column may see more than its lane's own)
-            for (int pos0 = 0; pos0 < a.chunk * a.n_chunks; pos0 += FM_ATTN_KEYS)
+            // (every step of the table and some behind it)
+            for (int pos0 = 0; pos0 < (max_pages * P + 300) / 64 * 64; pos0 += FM_ATTN_KEYS)
                 for (int lane = 0; lane < 64; lane++) {
                     const int g = lane >> 4, r = lane & 15;
                     const int kp = fm_kv_page(c, s, pos0 + 16 * (r >> 2)), vp = fm_kv_page(c, s, pos0 + 16 * g);
