@@ -61,7 +61,7 @@ int fm_launch_route(const float *d_logits, int n, int K, const float *d_seg_scor
                     float *d_w, float *d_params, hipStream_t st);
 int fm_launch_gdn(const FmGdn *a, int bf16, const int *start, int n_seq, const float *const *in,
                   float *const *out, void *ws, hipStream_t st);
-int fm_launch_attn(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int bf16, void *ws, hipStream_t st);
+int fm_launch_attn(const FmKv *c, const FmAttn *args, const FmSeqs *b, int D, int bf16, void *ws, int n_cu, hipStream_t st);
 int fm_launch_kv(const FmKv *c, const FmKvRows *x, const FmSeqs *b, int D, int bf16, int read, hipStream_t st);
 size_t fm_logprob_ws(int rows, int vocab, int top_n);
 int fm_launch_logprob(const float *x, int rows, int vocab, int64_t stride, const int32_t *tokens, int top_n,
@@ -1718,7 +1718,7 @@ extern "C" int fm_attn_dev(fm_ctx *c, const fm_attn_args *p) {
     if (rc) return fail(c, rc, "%s", w.text);
     DeviceGuard dg(c->device);
     if (ws && (rc = ensure_ws(c, ws))) return rc;
-    rc = fm_launch_attn(&k, &a, &b, p->cache.head_dim, p->dtype == FM_DTYPE_BF16, c->d_ws, c->stream);
+    rc = fm_launch_attn(&k, &a, &b, p->cache.head_dim, p->dtype == FM_DTYPE_BF16, c->d_ws, c->n_cu, c->stream);
     if (rc) return fail(c, rc, "attention launch failed: %s", hipGetErrorString(hipGetLastError()));
     return FM_OK;
 }

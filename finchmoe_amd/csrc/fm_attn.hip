@@ -30,6 +30,21 @@ __device__ __forceinline__ fm_v4f mfma(fm_v8h a, fm_v8h b, fm_v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// 2^x; below -126 (of which nothing is left in what follows) 0
+__device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
+// f as NP fp16 pieces whose sum it is (to 11 bits each).  With two, f has to be one fp32 value: fused with the
+// product in front of it, the conversion and the remainder could round to different first pieces.
+template <int NP>
+__device__ __forceinline__ void split(float f, _Float16 *piece) {
+    if constexpr (NP > 1) asm("" : "+v"(f));
+#pragma unroll
+    for (int p = 0; p < NP; p++) {
+        piece[p] = (_Float16)f;
+        f -= (float)piece[p];
+    }
+}
+
 // eight signed bytes as fp16 numbers
 __device__ __forceinline__ fm_v8h codes_f16(uint32_t lo, uint32_t hi) {
     const fm_v2h off = {(_Float16)1152.0f, (_Float16)1152.0f};
@@ -120,13 +135,10 @@ struct Columns {
             fm_v8h v[NP];
 #pragma unroll
             for (int j = 0; j < 8; j++) {
-                float f = x[u][j >> 2][j & 3] * up;
+                _Float16 piece[NP];
+                split<NP>(x[u][j >> 2][j & 3] * up, piece);
 #pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    const _Float16 hv = (_Float16)f;
-                    v[p][j] = hv;
-                    f -= (float)hv;
-                }
+                for (int p = 0; p < NP; p++) v[p][j] = piece[p];
             }
             const int s = min(wave * MY + u, KS - 1);
 #pragma unroll
@@ -218,7 +230,7 @@ struct Columns {
         const float m1 = fmaxf(m, top);
         // (nothing seen yet: any finite base keeps e^(-inf - base) at 0)
         const float base = m1 == -INFINITY ? 0.0f : m1;
-        const float keep = exp2f(m - base);
+        const float keep = fast_exp2(m - base);
         m = m1;
         l *= keep;
         int up = live ? (int)(__float_as_uint(v_scale) >> 23 & 255) - 126 : -100;
@@ -235,16 +247,13 @@ struct Columns {
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float e = exp2f(sc[t][i] - base + P_SHIFT);
+                const float e = fast_exp2(sc[t][i] - base + P_SHIFT);
                 l += e;
-                float pv = e * v_scale;
+                _Float16 piece[NP];
+                split<NP>(e * v_scale, piece);
                 const int j = 4 * (t & 1) + i;
 #pragma unroll
-                for (int p = 0; p < NP; p++) {
-                    const _Float16 hv = (_Float16)pv;
-                    p8[p][t >> 1][j] = hv;
-                    pv -= (float)hv;
-                }
+                for (int p = 0; p < NP; p++) p8[p][t >> 1][j] = piece[p];
             }
 #pragma unroll
         for (int d0 = 0; d0 < DT; d0 += 4) {
@@ -280,7 +289,7 @@ __device__ __forceinline__ void add_steps(const FmKv &c, const FmAttn &a, const 
     if (t < b.n_seq) {
         const int len = c.len[t];
         sh.len[t] = len;
-        n = c.kv_heads * fm_attn_head_steps(fm_seq_rows(b, t), a.group, len, a.max_len);
+        n = c.kv_heads * fm_attn_head_steps(fm_seq_rows(b, t), a.group, a.wide, len, a.max_len);
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -295,10 +304,10 @@ __device__ __forceinline__ void add_steps(const FmKv &c, const FmAttn &a, const 
     __syncthreads();
 }
 
-// One workgroup: its share of the steps, tile by tile.  The four waves take a tile's steps in turn and are
-// joined through LDS.
+// Narrow tiles: a workgroup takes its share of the steps, tile by tile; the four waves take a tile's steps
+// in turn and are joined through LDS.
 template <int D, bool BF16, bool ONCE>
-__global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_cols(FmKv c, FmAttn a, FmSeqs b) {
+__global__ __launch_bounds__(256, fm_attn_per_cu(D, 0)) void fm_attn_narrow(FmKv c, FmAttn a, FmSeqs b) {
     constexpr int NP = BF16 ? 1 : 2, DT = D / 16;
     __shared__ float s_o[3][DT][64][4];
     __shared__ float s_m[4][16], s_l[4][16];
@@ -323,7 +332,7 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_cols(FmKv c, F
         const int n = fm_seq_rows(b, s), len = __builtin_amdgcn_readfirstlane(sh.len[s]), per_head = (sh.first[s + 1] - sh.first[s]) / c.kv_heads;
         const int h = (at - sh.first[s]) / per_head;
         int off = (at - sh.first[s]) - h * per_head, tile = 0, steps;
-        while (off >= (steps = fm_attn_steps(n, a.group, len, a.max_len, tile))) off -= steps, tile++;
+        while (off >= (steps = fm_attn_steps(n, a.group, a.wide, len, a.max_len, tile))) off -= steps, tile++;
         const int s0 = off, s1 = min(steps, off + stop - at);    // this workgroup's steps of the tile
         at += s1 - s0;
 
@@ -365,7 +374,7 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_cols(FmKv c, F
         __syncthreads();
         const float m = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
         const float base = m == -INFINITY ? 0.0f : m;
-        const float f = ldexpf(exp2f(w.m - base), w.ref);
+        const float f = ldexpf(fast_exp2(w.m - base), w.ref);
 #pragma unroll
         for (int d = 0; d < DT; d++) w.o[d] *= f;
         if (wave) {
@@ -376,7 +385,7 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_cols(FmKv c, F
         if (wave) continue;
         float l = 0.0f;
 #pragma unroll
-        for (int v = 0; v < 4; v++) l = fmaf(s_l[v][col], exp2f(s_m[v][col] - base), l);
+        for (int v = 0; v < 4; v++) l = fmaf(s_l[v][col], fast_exp2(s_m[v][col] - base), l);
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -397,23 +406,241 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_cols(FmKv c, F
     }
 }
 
-// Joins the parts of one tile that several workgroups took: a wave per column (four workgroups a tile),
+// Wide tiles: 128 columns of one (sequence, cache head), 32 a wave.  The workgroup turns a step's codes into
+// fp16 operands in LDS once, [tile][k step][lane] of 16 bytes, and its waves read them for their columns.
+// The codes of the next step are in registers meanwhile and go to the other half of the LDS at the step's
+// end: one barrier a step.  A step of a wave is 128 matrix instructions of 16 cycles (256 with two
+// pieces) and as much LDS time; conversion is shared by 128 columns.
+template <int D, bool BF16>
+__global__ __launch_bounds__(256, 1) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs b) {
+    constexpr int NP = BF16 ? 1 : 2, KS = D / 32, DT = D / 16, CT = 2, LD = D / 64;
+    __shared__ fm_v8h s_k[2][4 * KS * 64], s_v[2][DT * 2 * 64];
+    __shared__ Shares sh;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    add_steps(c, a, b, sh);
+    const int total = sh.first[b.n_seq], share = fm_attn_share(total, a.groups);
+    if (blockIdx.x == 0)                                         // for the join
+        for (int i = threadIdx.x; i <= b.n_seq; i += 256) a.first[i] = sh.first[i];
+    int at = blockIdx.x * share;
+    const int stop = min(total, at + share);
+    if (at >= stop) return;
+    int s = 0;
+    for (int hi = b.n_seq; hi - s > 1;) {
+        const int mid = (s + hi) / 2;
+        if (sh.first[mid] <= at) s = mid;
+        else hi = mid;
+    }
+    while (at < stop) {
+        while (sh.first[s + 1] <= at) s++;                       // (sequences of no or narrow tiles have no steps here)
+        const int n = fm_seq_rows(b, s), len = __builtin_amdgcn_readfirstlane(sh.len[s]), per_head = (sh.first[s + 1] - sh.first[s]) / c.kv_heads;
+        const int h = (at - sh.first[s]) / per_head;
+        int off = (at - sh.first[s]) - h * per_head, tile = 0, steps;
+        while (off >= (steps = fm_attn_steps(n, a.group, a.wide, len, a.max_len, tile))) off -= steps, tile++;
+        const int s0 = off, s1 = min(steps, off + stop - at);    // this workgroup's steps of the tile
+        at += s1 - s0;
+
+        const int32_t *table = c.pages + (int64_t)s * c.max_pages;
+        fm_v8h q[CT][NP][KS];
+        fm_v4f o[CT][DT];
+        float m[CT], l[CT], qscale[CT];
+        int ref[CT], limit[CT], all_limit = 0x7FFFFFFF;
+        int64_t to[CT];          // the column's place in the output, -1 if it is not there
+        Runs now, next;
+        now.load(c, table, s0 * BK);
+        next.load(c, table, min(s0 + 1, s1 - 1) * BK);
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            const int cc = tile * FM_ATTN_WIDE + wave * 32 + ct * 16 + r;
+            const bool there = cc < n * a.group;
+            const int i = there ? cc / a.group : 0, qh = h * a.group + (there ? cc % a.group : 0);
+            const int64_t row = fm_seq_row0(b, s) + i;
+            limit[ct] = there ? min(min(len, a.max_len), len - n + i + 1) : 0;
+            all_limit = min(all_limit, limit[ct]);
+            to[ct] = there ? (row * a.q_heads + qh) * D : -1;
+            fm_v4f x[KS][2];
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int hh = 0; hh < 2; hh++)
+                    x[k][hh] = fm_ld4<BF16>(a.q, row * a.q_stride + (int64_t)qh * D + 64 * (k >> 1) + 16 * g + 8 * (k & 1) + 4 * hh);
+            float big = 0.0f;
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(x[k][j >> 2][j & 3]));
+            big = fmaxf(big, __shfl_xor(big, 16));
+            big = fmaxf(big, __shfl_xor(big, 32));
+            int e = (int)(__float_as_uint(big) >> 23 & 255) - 127;
+            e = e > 100 ? 100 : e < -100 ? -100 : e;
+            const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
+            qscale[ct] = __uint_as_float((uint32_t)(127 - 8 + e) << 23) * a.scale_log2;
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    _Float16 piece[NP];
+                    split<NP>(x[k][j >> 2][j & 3] * up, piece);
+#pragma unroll
+                    for (int p = 0; p < NP; p++) q[ct][p][k][j] = piece[p];
+                }
+            m[ct] = -INFINITY;
+            l[ct] = 0.0f;
+            ref[ct] = -100;
+#pragma unroll
+            for (int d = 0; d < DT; d++) o[ct][d] = fm_v4f{0.f, 0.f, 0.f, 0.f};
+        }
+        for (int x = 32; x; x >>= 1) all_limit = min(all_limit, __shfl_xor(all_limit, x));
+        // this wave's part of a step's codes: key tile `wave`, dims tiles wave * LD ..
+        fm_v4u kc[LD], vc[LD];
+        float ks, vs;
+        auto fetch = [&](const Runs &p, int pos) {
+            const int8_t *kb = c.k + fm_kv_k_at(c, D, max(p.k_page(c, pos), 0), h, pos + 16 * (r >> 2) + (r & 3) + 4 * wave, 16 * g);
+            const int8_t *vb = c.v + fm_kv_v_at(c, D, max(p.v_page(c, pos), 0), h, pos + 16 * g, 16 * wave * LD + r);
+            const int64_t sc = (int64_t)max(p.v_page(c, pos), 0) * c.kv_heads + h;
+#pragma unroll
+            for (int d = 0; d < LD; d++) kc[d] = *(const fm_v4u *)(kb + 64 * d);
+#pragma unroll
+            for (int d = 0; d < LD; d++) vc[d] = *(const fm_v4u *)(vb + 16 * d * c.page_tokens);
+            ks = c.k_scale[sc];
+            vs = c.v_scale[sc];
+        };
+        auto put = [&](int buf) {
+#pragma unroll
+            for (int d = 0; d < LD; d++) {
+                s_k[buf][(wave * KS + 2 * d) * 64 + lane] = codes_f16(kc[d][0], kc[d][1]);
+                s_k[buf][(wave * KS + 2 * d + 1) * 64 + lane] = codes_f16(kc[d][2], kc[d][3]);
+                s_v[buf][(wave * LD + d) * 128 + lane] = codes_f16(vc[d][0], vc[d][1]);
+                s_v[buf][(wave * LD + d) * 128 + 64 + lane] = codes_f16(vc[d][2], vc[d][3]);
+            }
+        };
+        lds_barrier();                                            // (the last tile's operands have been read)
+        fetch(now, s0 * BK);
+        put(0);
+        for (int st = s0; st < s1; st++) {
+            const int pos = st * BK, buf = (st - s0) & 1, vpos = pos + 16 * g;
+            const float k_scale = ks, v_scale0 = vs;
+            const bool there = now.v_page(c, pos) >= 0;
+            lds_barrier();                                        // this step's operands are there
+            Runs later;
+            later.load(c, table, min(st + 2, s1 - 1) * BK);
+            fetch(next, min(st + 1, s1 - 1) * BK);
+            fm_v4f sc[CT][4];
+#pragma unroll
+            for (int t = 0; t < 4; t++) {
+#pragma unroll
+                for (int ct = 0; ct < CT; ct++) sc[ct][t] = fm_v4f{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int k = 0; k < KS; k++) {
+                    const fm_v8h x = s_k[buf][(t * KS + k) * 64 + lane];
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                        for (int p = 0; p < NP; p++) sc[ct][t] = mfma(x, q[ct][p][k], sc[ct][t]);
+                }
+            }
+            const bool whole = __all(there) && pos + BK <= all_limit;      // nothing of the step is masked
+            fm_v8h p8[CT][NP][2];
+#pragma unroll
+            for (int ct = 0; ct < CT; ct++) {
+                const bool live = there && vpos < limit[ct];
+                const float f = (live ? k_scale : 0.0f) * qscale[ct];
+                float v_scale = live ? v_scale0 : 0.0f, top = -INFINITY;
+                if (whole) {
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) sc[ct][t][i] *= f, top = fmaxf(top, sc[ct][t][i]);
+                } else {
+#pragma unroll
+                    for (int t = 0; t < 4; t++)
+#pragma unroll
+                        for (int i = 0; i < 4; i++) {
+                            sc[ct][t][i] = live && vpos + 4 * t + i < limit[ct] ? sc[ct][t][i] * f : -INFINITY;
+                            top = fmaxf(top, sc[ct][t][i]);
+                        }
+                }
+                top = fmaxf(top, __shfl_xor(top, 16));
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float m1 = fmaxf(m[ct], top), base = m1 == -INFINITY ? 0.0f : m1;
+                const float keep = fast_exp2(m[ct] - base);
+                m[ct] = m1;
+                int up = live ? (int)(__float_as_uint(v_scale) >> 23 & 255) - 126 : -100;
+                up = max(ref[ct], min(up, 100));
+                up = max(up, __shfl_xor(up, 16));
+                up = max(up, __shfl_xor(up, 32));
+                const float keep_o = ldexpf(keep, ref[ct] - up);
+                ref[ct] = up;
+                v_scale = ldexpf(v_scale, -up);
+                l[ct] *= keep;
+                if (!__all(keep_o == 1.0f)) {
+#pragma unroll
+                    for (int d = 0; d < DT; d++) o[ct][d] *= keep_o;
+                }
+                const float shift = P_SHIFT - base;
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < 4; i++) {
+                        const float e = fast_exp2(sc[ct][t][i] + shift);
+                        l[ct] += e;
+                        _Float16 piece[NP];
+                        split<NP>(e * v_scale, piece);
+#pragma unroll
+                        for (int p = 0; p < NP; p++) p8[ct][p][t >> 1][4 * (t & 1) + i] = piece[p];
+                    }
+            }
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int k = 0; k < 2; k++) {
+                    const fm_v8h x = s_v[buf][(d * 2 + k) * 64 + lane];
+#pragma unroll
+                    for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                        for (int p = 0; p < NP; p++) o[ct][d] = mfma(x, p8[ct][p][k], o[ct][d]);
+                }
+            if (st + 1 < s1) put(buf ^ 1);
+            now = next;
+            next = later;
+        }
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            float sum = l[ct];
+            sum += __shfl_xor(sum, 16);
+            sum += __shfl_xor(sum, 32);
+            if (to[ct] < 0) continue;
+            const float unit = ldexpf(1.0f, ref[ct]);
+            if (s0 == 0 && s1 == steps) {
+                const float inv = sum > 0.0f || sum != sum ? unit / sum : 0.0f;
+#pragma unroll
+                for (int d = 0; d < DT; d++) fm_st4<BF16>(a.out, to[ct] + 16 * d + 4 * g, o[ct][d] * inv);
+            } else {
+                const int64_t part = (int64_t)fm_attn_slot(blockIdx.x, s0) * FM_ATTN_WIDE + wave * 32 + ct * 16 + r;
+#pragma unroll
+                for (int d = 0; d < DT; d++) *(fm_v4f *)(a.part_o + part * D + 16 * d + 4 * g) = o[ct][d] * unit;
+                if (g == 0) a.part_ml[2 * part] = m[ct], a.part_ml[2 * part + 1] = sum;
+            }
+        }
+    }
+}
+
+// Joins the parts of one tile that several workgroups took: a wave per column, four columns a workgroup,
 // D / 64 dims a lane.
 template <int D, bool BF16>
 __global__ __launch_bounds__(256) void fm_attn_join(FmKv c, FmAttn a, FmSeqs b) {
-    const int s = blockIdx.z, h = blockIdx.y, tile = blockIdx.x >> 2, lane = threadIdx.x & 63;
+    const int cols = fm_attn_cols(a.wide), s = blockIdx.z, h = blockIdx.y, tile = blockIdx.x / (cols / 4), lane = threadIdx.x & 63;
     const int n = fm_seq_rows(b, s);
-    if (tile >= fm_attn_tiles(n, a.group)) return;
+    if (tile >= fm_attn_tiles(n, a.group, a.wide)) return;
     const int len = c.len[s], from = a.first[s], per_head = (a.first[s + 1] - from) / c.kv_heads;
-    const int share = fm_attn_share(a.first[b.n_seq], a.groups), steps = fm_attn_steps(n, a.group, len, a.max_len, tile);
+    const int share = fm_attn_share(a.first[b.n_seq], a.groups), steps = fm_attn_steps(n, a.group, a.wide, len, a.max_len, tile);
     int at = from + h * per_head;
-    for (int t = 0; t < tile; t++) at += fm_attn_steps(n, a.group, len, a.max_len, t);
+    for (int t = 0; t < tile; t++) at += fm_attn_steps(n, a.group, a.wide, len, a.max_len, t);
     const int g0 = at / share, g1 = (at + steps - 1) / share;
     if (g0 == g1) return;
-    const int col = 4 * (blockIdx.x & 3) + (threadIdx.x >> 6), cc = tile * COLS + col;
+    const int col = 4 * (blockIdx.x % (cols / 4)) + (threadIdx.x >> 6), cc = tile * cols + col;
     if (cc >= n * a.group) return;
     const int64_t row = fm_seq_row0(b, s) + cc / a.group;
-    auto slot = [&](int g) { return (int64_t)fm_attn_slot(g, g * share - at) * COLS + col; };
+    auto slot = [&](int g) { return (int64_t)fm_attn_slot(g, g * share - at) * cols + col; };
     // a lane per part: its weight e^(m - base)
     float m = -INFINITY;
     for (int g = g0 + lane; g <= g1; g += 64) m = fmaxf(m, a.part_ml[2 * slot(g)]);
@@ -426,7 +653,7 @@ __global__ __launch_bounds__(256) void fm_attn_join(FmKv c, FmAttn a, FmSeqs b) 
         const int parts = min(64, g1 + 1 - g);
         float f = 0.0f;
         if (lane < parts) {
-            f = exp2f(a.part_ml[2 * slot(g + lane)] - base);
+            f = fast_exp2(a.part_ml[2 * slot(g + lane)] - base);
             l = fmaf(f, a.part_ml[2 * slot(g + lane) + 1], l);
         }
 #pragma unroll 4
@@ -572,27 +799,36 @@ __global__ __launch_bounds__(256) void fm_kv_read(FmKv c, FmKvRows x, int D, FmS
 }
 
 template <int D, bool BF16>
-void launch_cols(const FmKv &c, const FmAttn &a, const FmSeqs &b, hipStream_t st) {
-    if (a.n_tiles == 1) hipLaunchKernelGGL((fm_attn_cols<D, BF16, true>), dim3(a.groups), dim3(256), 0, st, c, a, b);
-    else hipLaunchKernelGGL((fm_attn_cols<D, BF16, false>), dim3(a.groups), dim3(256), 0, st, c, a, b);
+void launch_attn(const FmKv &c, const FmAttn &a, const FmSeqs &b, hipStream_t st) {
+    const dim3 grid(a.groups), block(256);
+    if (a.wide) hipLaunchKernelGGL((fm_attn_wide<D, BF16>), grid, block, 0, st, c, a, b);
+    else if (a.n_tiles == 1) hipLaunchKernelGGL((fm_attn_narrow<D, BF16, true>), grid, block, 0, st, c, a, b);
+    else hipLaunchKernelGGL((fm_attn_narrow<D, BF16, false>), grid, block, 0, st, c, a, b);
     if (a.groups > 1)
-        hipLaunchKernelGGL((fm_attn_join<D, BF16>), dim3(4 * a.n_tiles, c.kv_heads, b.n_seq), dim3(256), 0, st, c, a, b);
+        hipLaunchKernelGGL((fm_attn_join<D, BF16>), dim3(a.n_tiles * (fm_attn_cols(a.wide) / 4), c.kv_heads, b.n_seq), block, 0, st, c, a, b);
 }
 
 }  // namespace
 
-extern "C" int fm_launch_attn(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int bf16, void *ws, hipStream_t st) {
-    if (a->n_tiles < 1) return FM_OK;
-    a->part_o = (float *)ws;
-    a->part_ml = a->part_o + (size_t)2 * a->groups * COLS * D;
-    a->first = (int *)(a->part_ml + (size_t)2 * a->groups * COLS * 2);
-    switch (D) {
-        case 64: bf16 ? launch_cols<64, true>(*c, *a, *b, st) : launch_cols<64, false>(*c, *a, *b, st); break;
-        case 128: bf16 ? launch_cols<128, true>(*c, *a, *b, st) : launch_cols<128, false>(*c, *a, *b, st); break;
-        case 256: bf16 ? launch_cols<256, true>(*c, *a, *b, st) : launch_cols<256, false>(*c, *a, *b, st); break;
-        default: return FM_ERR_UNSUPPORTED;
+// ws: what fm_attn_check asked for
+extern "C" int fm_launch_attn(const FmKv *c, const FmAttn *args, const FmSeqs *b, int D, int bf16, void *ws, int n_cu, hipStream_t st) {
+    for (int wide = 0; wide < 2; wide++) {
+        FmAttn a = *args;
+        fm_attn_plan(c, &a, b, D, n_cu, wide);
+        if (!a.n_tiles) continue;
+        const size_t cols = (size_t)2 * a.groups * fm_attn_cols(wide);
+        a.part_o = (float *)ws;
+        a.part_ml = a.part_o + cols * D;
+        a.first = (int *)(a.part_ml + cols * 2);
+        switch (D) {
+            case 64: bf16 ? launch_attn<64, true>(*c, a, *b, st) : launch_attn<64, false>(*c, a, *b, st); break;
+            case 128: bf16 ? launch_attn<128, true>(*c, a, *b, st) : launch_attn<128, false>(*c, a, *b, st); break;
+            case 256: bf16 ? launch_attn<256, true>(*c, a, *b, st) : launch_attn<256, false>(*c, a, *b, st); break;
+            default: return FM_ERR_UNSUPPORTED;
+        }
+        if (hipGetLastError() != hipSuccess) return FM_ERR_HIP;
     }
-    return hipGetLastError() == hipSuccess ? FM_OK : FM_ERR_HIP;
+    return FM_OK;
 }
 
 extern "C" int fm_launch_kv(const FmKv *c, const FmKvRows *x, const FmSeqs *b, int D, int bf16, int read, hipStream_t st) {

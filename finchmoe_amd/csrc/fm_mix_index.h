@@ -175,34 +175,42 @@ struct FmAttn {
     int q_heads, group;     // query heads per cache head
     float scale_log2;       // scale * log2(e)
     int max_len;            // keys from here on are not seen, at most max_pages * page_tokens
-    int n_tiles;            // column tiles of the sequence with the most rows
+    int wide;               // which sequences a launch takes: those of wide tiles, or the others
+    int n_tiles;            // column tiles of the launch's sequence with the most rows
     int groups;             // workgroups that share the steps
     float *part_o, *part_ml;
     int *first;             // steps before each sequence, for the join
 };
 #define FM_ATTN_KEYS 64     // keys of a wave's step
-#define FM_ATTN_COLS 16     // columns of a tile
 #define FM_ATTN_WAVES 4     // waves of a workgroup
+#define FM_ATTN_COLS 16     // columns of a narrow tile: its waves take different keys
+#define FM_ATTN_WIDE 128    // columns of a wide one: its waves take different columns
+// A sequence with more columns than this has wide tiles.
+#define FM_ATTN_NARROW_MOST 64
 
 // ---- attention's steps and who takes them --------------------------------------------------
-// A sequence of n rows has, per cache head, tiles of 16 columns (row * group + query head of the group);
-// a tile's steps are those of 64 keys up to the last one its last column sees, at least one
-// (somebody has to write the zeros of a row that sees nothing).
-FM_HD int fm_attn_tiles(int n, int group) { return (n * group + FM_ATTN_COLS - 1) / FM_ATTN_COLS; }
-FM_HD int fm_attn_end(int n, int group, int len, int max_len, int tile) {
-    const int cols = n * group, col = tile * FM_ATTN_COLS + FM_ATTN_COLS - 1;
+// A sequence of n rows has n * group columns per cache head (row * group + query head of the group) in
+// tiles of 16 or 128; a tile's steps are those of 64 keys up to the last one its last column sees, at least
+// one (somebody has to write the zeros of a row that sees nothing).
+FM_HD int fm_attn_cols(int wide) { return wide ? FM_ATTN_WIDE : FM_ATTN_COLS; }
+FM_HD int fm_attn_tiles(int n, int group, int wide) {
+    if ((n * group > FM_ATTN_NARROW_MOST) != (wide != 0)) return 0;
+    return (n * group + fm_attn_cols(wide) - 1) / fm_attn_cols(wide);
+}
+FM_HD int fm_attn_end(int n, int group, int wide, int len, int max_len, int tile) {
+    const int cols = n * group, col = (tile + 1) * fm_attn_cols(wide) - 1;
     const int last = (col < cols - 1 ? col : cols - 1) / group, seen = len < max_len ? len : max_len;
     const int end = len - n + last + 1;
     return end < seen ? end : seen;
 }
-FM_HD int fm_attn_steps(int n, int group, int len, int max_len, int tile) {
-    const int end = fm_attn_end(n, group, len, max_len, tile);
+FM_HD int fm_attn_steps(int n, int group, int wide, int len, int max_len, int tile) {
+    const int end = fm_attn_end(n, group, wide, len, max_len, tile);
     return end <= FM_ATTN_KEYS ? 1 : (end + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS;
 }
 // all tiles of one cache head
-FM_HD int fm_attn_head_steps(int n, int group, int len, int max_len) {
+FM_HD int fm_attn_head_steps(int n, int group, int wide, int len, int max_len) {
     int sum = 0;
-    for (int t = 0; t < fm_attn_tiles(n, group); t++) sum += fm_attn_steps(n, group, len, max_len, t);
+    for (int t = 0; t < fm_attn_tiles(n, group, wide); t++) sum += fm_attn_steps(n, group, wide, len, max_len, t);
     return sum;
 }
 // Steps are numbered sequence by sequence, head by head, tile by tile; workgroup g takes those from
@@ -404,21 +412,27 @@ inline int fm_most_rows(const FmSeqs &b) {
 }
 inline int fm_all_rows(const FmSeqs &b) { return b.one_row ? b.n_seq : b.start[b.n_seq]; }
 
-// Workgroups of a CU: heads of 256 take a wave more registers than half a SIMD has (and a spilled one
-// would wait for the codes in flight).
-FM_HDC int fm_attn_per_cu(int D) { return D == 256 ? 1 : 2; }
-// Attention: the workgroups that fit on the chip share the steps, fewer if there cannot be as many.  Returns the
-// workspace: two parts per workgroup and the steps before each sequence.
-inline size_t fm_attn_plan(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int n_cu) {
+// Workgroups of a CU.  Narrow tiles: heads of 256 take a wave more registers than half a SIMD has (and a
+// spilled one would wait for the codes in flight).  Wide tiles keep two steps of keys and values in LDS.
+FM_HDC int fm_attn_per_cu(int D, int wide) { return D == 256 || wide ? 1 : 2; }
+// Attention: the workgroups that fit on the chip share the steps, fewer if there cannot be as many.  Sets
+// n_tiles (0: no sequence for this launch) and groups; returns the workspace: two parts per workgroup and
+// the steps before each sequence.
+inline size_t fm_attn_plan(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int n_cu, int wide) {
     const int64_t have = (int64_t)c->max_pages * c->page_tokens;
     if (a->max_len > have) a->max_len = (int)have;
-    a->n_tiles = fm_attn_tiles(fm_most_rows(*b), a->group);
+    a->wide = wide;
+    a->n_tiles = 0;
     int64_t most = 0;
-    for (int s = 0; s < b->n_seq; s++)
-        most += (int64_t)c->kv_heads * fm_attn_tiles(fm_seq_rows(*b, s), a->group) * ((a->max_len + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS + 1);
-    const int64_t groups = (most + FM_ATTN_WAVES - 1) / FM_ATTN_WAVES;
-    a->groups = (int)(groups < 1 ? 1 : groups > fm_attn_per_cu(D) * n_cu ? fm_attn_per_cu(D) * n_cu : groups);
-    return (size_t)2 * a->groups * FM_ATTN_COLS * (D + 2) * sizeof(float) + (FM_MAX_SEQ + 1) * sizeof(int);
+    for (int s = 0; s < b->n_seq; s++) {
+        const int tiles = fm_attn_tiles(fm_seq_rows(*b, s), a->group, wide);
+        if (tiles > a->n_tiles) a->n_tiles = tiles;
+        most += (int64_t)c->kv_heads * tiles * ((a->max_len + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS + 1);
+    }
+    if (!a->n_tiles) return 0;
+    const int64_t groups = (most + FM_ATTN_WAVES - 1) / FM_ATTN_WAVES, fit = fm_attn_per_cu(D, wide) * n_cu;
+    a->groups = (int)(groups < 1 ? 1 : groups > fit ? fit : groups);
+    return (size_t)2 * a->groups * fm_attn_cols(wide) * (D + 2) * sizeof(float) + (FM_MAX_SEQ + 1) * sizeof(int);
 }
 
 inline int fm_attn_check(FmWhy *w, const fm_attn_args *p, int n_cu, FmKv *k, FmAttn *a, FmSeqs *b, size_t *ws) {
@@ -442,7 +456,10 @@ inline int fm_attn_check(FmWhy *w, const fm_attn_args *p, int n_cu, FmKv *k, FmA
     a->scale_log2 = (float)((double)p->scale * 1.4426950408889634);
     a->max_len = p->max_len;
     fm_fill_seqs(b, p->seq_start, p->n_seq);
-    *ws = fm_attn_plan(k, a, b, p->cache.head_dim, n_cu);
+    FmAttn other = *a;       // (the two launches run one after the other in the same workspace)
+    const size_t wide = fm_attn_plan(k, &other, b, p->cache.head_dim, n_cu, 1);
+    *ws = fm_attn_plan(k, a, b, p->cache.head_dim, n_cu, 0);
+    if (wide > *ws) *ws = wide;
     return FM_OK;
 }
 

@@ -188,18 +188,18 @@ static void refuse_logprobs() {
 static void share_out(const FmKv &c, const FmAttn &a, const FmSeqs &b, int D, size_t ws) {
     std::vector<int> first(b.n_seq + 1, 0);
     for (int s = 0; s < b.n_seq; s++)
-        first[s + 1] = first[s] + c.kv_heads * fm_attn_head_steps(fm_seq_rows(b, s), a.group, c.len[s], a.max_len);
+        first[s + 1] = first[s] + c.kv_heads * fm_attn_head_steps(fm_seq_rows(b, s), a.group, a.wide, c.len[s], a.max_len);
     const int total = first[b.n_seq], share = fm_attn_share(total, a.groups);
     CHECK((int64_t)share * a.groups >= total);
-    CHECK(ws == (size_t)2 * a.groups * FM_ATTN_COLS * (D + 2) * 4 + (FM_MAX_SEQ + 1) * 4);
+    CHECK(ws == (size_t)2 * a.groups * fm_attn_cols(a.wide) * (D + 2) * 4 + (FM_MAX_SEQ + 1) * 4);
     std::set<int> written;      // slots of parts
     int seen = 0;
     for (int s = 0; s < b.n_seq; s++) {
         const int n = fm_seq_rows(b, s);
         for (int h = 0; h < c.kv_heads; h++)
-            for (int t = 0; t < fm_attn_tiles(n, a.group); t++) {
-                const int steps = fm_attn_steps(n, a.group, c.len[s], a.max_len, t), at = seen;
-                const int end = fm_attn_end(n, a.group, c.len[s], a.max_len, t);
+            for (int t = 0; t < fm_attn_tiles(n, a.group, a.wide); t++) {
+                const int steps = fm_attn_steps(n, a.group, a.wide, c.len[s], a.max_len, t), at = seen;
+                const int end = fm_attn_end(n, a.group, a.wide, c.len[s], a.max_len, t);
                 CHECK(steps >= 1 && end <= steps * FM_ATTN_KEYS && end <= a.max_len && (steps == 1 || end > (steps - 1) * FM_ATTN_KEYS));
                 seen += steps;
                 const int g0 = at / share, g1 = (at + steps - 1) / share;
@@ -236,9 +236,24 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
     FmSeqs b{};
     b.n_seq = n_seq;
     for (int s = 0; s <= n_seq; s++) b.start[s] = start[s];
-    const size_t ws = fm_attn_plan(&c, &a, &b, D, 1 + rnd(64));
-    CHECK(a.max_len <= max_pages * P && a.groups >= 1);
-    share_out(c, a, b, D, ws);
+    int covered = 0;
+    for (int wide = 0; wide < 2; wide++) {
+        const size_t ws = fm_attn_plan(&c, &a, &b, D, 1 + rnd(64), wide);
+        CHECK(a.max_len <= max_pages * P);
+        if (!a.n_tiles) {
+            CHECK(ws == 0);
+            continue;
+        }
+        CHECK(a.groups >= 1);
+        share_out(c, a, b, D, ws);
+    }
+    for (int s = 0; s < n_seq; s++) {      // a sequence's columns are in one of the two launches
+        const int n = fm_seq_rows(b, s), narrow = fm_attn_tiles(n, group, 0), wides = fm_attn_tiles(n, group, 1);
+        CHECK(!narrow || !wides);
+        CHECK(narrow * FM_ATTN_COLS + wides * FM_ATTN_WIDE >= n * group);
+        covered += narrow + wides;
+    }
+    CHECK(covered >= 0);
     for (int s = 0; s < n_seq; s++)
         for (int h = 0; h < kv; h++)
             // (every step of the table and some behind it)

@@ -134,6 +134,15 @@ def test_long_context_in_chunks(hip, rows):
     _run(hip, 6, [5003], rows, 4, 2, 64, 64, "bfloat16")
 
 
+@pytest.mark.parametrize("rows", [[1] * 30, [300]])
+def test_fp32_weights_keep_their_second_piece(hip, rows):
+    """many columns, page scales of their own: no single weight may drop to 11 bits (an error of 2^-12 of
+    it, far above the bound, in one row of thousands)"""
+    lens = [300] if len(rows) == 1 else [40 + 7 * i for i in range(30)]
+    for seed in (50, 51):
+        _run(hip, seed, lens, rows, 8, 2, 128, 64, "float32")
+
+
 def test_ragged_lengths_share_one_cut(hip):
     _run(hip, 7, [3, 4000, 700], [1, 1, 1], 2, 1, 64, 16, "float32")
 
