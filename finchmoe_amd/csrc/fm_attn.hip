@@ -412,32 +412,18 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D, 0)) void fm_attn_narrow(FmKv
 // end: one barrier a step.  A step of a wave is 128 matrix instructions of 16 cycles (256 with two
 // pieces) and as much LDS time; conversion is shared by 128 columns.
 template <int D, bool BF16>
-__global__ __launch_bounds__(256, 1) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs b) {
+__global__ __launch_bounds__(256, 1) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs b, FmWide w) {
     constexpr int NP = BF16 ? 1 : 2, KS = D / 32, DT = D / 16, CT = 2, LD = D / 64;
     __shared__ fm_v8h s_k[2][4 * KS * 64], s_v[2][DT * 2 * 64];
-    __shared__ Shares sh;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
-    add_steps(c, a, b, sh);
-    const int total = sh.first[b.n_seq], share = fm_attn_share(total, a.groups);
-    if (blockIdx.x == 0)                                         // for the join
-        for (int i = threadIdx.x; i <= b.n_seq; i += 256) a.first[i] = sh.first[i];
-    int at = blockIdx.x * share;
-    const int stop = min(total, at + share);
-    if (at >= stop) return;
-    int s = 0;
-    for (int hi = b.n_seq; hi - s > 1;) {
-        const int mid = (s + hi) / 2;
-        if (sh.first[mid] <= at) s = mid;
-        else hi = mid;
-    }
-    while (at < stop) {
-        while (sh.first[s + 1] <= at) s++;                       // (sequences of no or narrow tiles have no steps here)
-        const int n = fm_seq_rows(b, s), len = __builtin_amdgcn_readfirstlane(sh.len[s]), per_head = (sh.first[s + 1] - sh.first[s]) / c.kv_heads;
-        const int h = (at - sh.first[s]) / per_head;
-        int off = (at - sh.first[s]) - h * per_head, tile = 0, steps;
-        while (off >= (steps = fm_attn_steps(n, a.group, a.wide, len, a.max_len, tile))) off -= steps, tile++;
-        const int s0 = off, s1 = min(steps, off + stop - at);    // this workgroup's steps of the tile
-        at += s1 - s0;
+    const int units = w.first[b.n_seq] * c.kv_heads * a.splits;
+    for (int round = 0; round * a.groups < units; round++) {
+        const int unit = fm_attn_wide_pick(round, blockIdx.x, a.groups);
+        if (unit >= units) continue;
+        const FmWideUnit at = fm_attn_wide_unit(w, b.n_seq, c.kv_heads, a.splits, unit);
+        const int s = at.s, h = at.h, tile = at.tile, n = fm_seq_rows(b, s), len = __builtin_amdgcn_readfirstlane(c.len[s]);
+        const int steps = fm_attn_steps(n, a.group, 1, len, a.max_len, tile);
+        const int s0 = (int)((int64_t)steps * at.part / a.splits), s1 = (int)((int64_t)steps * (at.part + 1) / a.splits);
 
         const int32_t *table = c.pages + (int64_t)s * c.max_pages;
         fm_v8h q[CT][NP][KS];
@@ -447,7 +433,7 @@ __global__ __launch_bounds__(256, 1) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
         int64_t to[CT];          // the column's place in the output, -1 if it is not there
         Runs now, next;
         now.load(c, table, s0 * BK);
-        next.load(c, table, min(s0 + 1, s1 - 1) * BK);
+        next.load(c, table, max(min(s0 + 1, s1 - 1), 0) * BK);
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             const int cc = tile * FM_ATTN_WIDE + wave * 32 + ct * 16 + r;
@@ -609,56 +595,43 @@ __global__ __launch_bounds__(256, 1) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
             sum += __shfl_xor(sum, 16);
             sum += __shfl_xor(sum, 32);
             if (to[ct] < 0) continue;
-            const float unit = ldexpf(1.0f, ref[ct]);
-            if (s0 == 0 && s1 == steps) {
-                const float inv = sum > 0.0f || sum != sum ? unit / sum : 0.0f;
+            const float unit2 = ldexpf(1.0f, ref[ct]);
+            if (a.splits == 1) {
+                const float inv = sum > 0.0f || sum != sum ? unit2 / sum : 0.0f;
 #pragma unroll
                 for (int d = 0; d < DT; d++) fm_st4<BF16>(a.out, to[ct] + 16 * d + 4 * g, o[ct][d] * inv);
             } else {
-                const int64_t part = (int64_t)fm_attn_slot(blockIdx.x, s0) * FM_ATTN_WIDE + wave * 32 + ct * 16 + r;
+                const int64_t part = (int64_t)unit * FM_ATTN_WIDE + wave * 32 + ct * 16 + r;
 #pragma unroll
-                for (int d = 0; d < DT; d++) *(fm_v4f *)(a.part_o + part * D + 16 * d + 4 * g) = o[ct][d] * unit;
+                for (int d = 0; d < DT; d++) *(fm_v4f *)(a.part_o + part * D + 16 * d + 4 * g) = o[ct][d] * unit2;
                 if (g == 0) a.part_ml[2 * part] = m[ct], a.part_ml[2 * part + 1] = sum;
             }
         }
     }
 }
 
-// Joins the parts of one tile that several workgroups took: a wave per column, four columns a workgroup,
-// D / 64 dims a lane.
-template <int D, bool BF16>
-__global__ __launch_bounds__(256) void fm_attn_join(FmKv c, FmAttn a, FmSeqs b) {
-    const int cols = fm_attn_cols(a.wide), s = blockIdx.z, h = blockIdx.y, tile = blockIdx.x / (cols / 4), lane = threadIdx.x & 63;
-    const int n = fm_seq_rows(b, s);
-    if (tile >= fm_attn_tiles(n, a.group, a.wide)) return;
-    const int len = c.len[s], from = a.first[s], per_head = (a.first[s + 1] - from) / c.kv_heads;
-    const int share = fm_attn_share(a.first[b.n_seq], a.groups), steps = fm_attn_steps(n, a.group, a.wide, len, a.max_len, tile);
-    int at = from + h * per_head;
-    for (int t = 0; t < tile; t++) at += fm_attn_steps(n, a.group, a.wide, len, a.max_len, t);
-    const int g0 = at / share, g1 = (at + steps - 1) / share;
-    if (g0 == g1) return;
-    const int col = 4 * (blockIdx.x % (cols / 4)) + (threadIdx.x >> 6), cc = tile * cols + col;
-    if (cc >= n * a.group) return;
-    const int64_t row = fm_seq_row0(b, s) + cc / a.group;
-    auto slot = [&](int g) { return (int64_t)fm_attn_slot(g, g * share - at) * cols + col; };
-    // a lane per part: its weight e^(m - base)
+// One column out of `parts` parts, by a wave: D / 64 dims a lane, a lane per part for its weight
+// e^(m - base).  slot(k): where part k's column lies.
+template <int D, bool BF16, class Slot>
+__device__ __forceinline__ void join_column(const FmAttn &a, int parts, Slot slot, int64_t to) {
+    const int lane = threadIdx.x & 63;
     float m = -INFINITY;
-    for (int g = g0 + lane; g <= g1; g += 64) m = fmaxf(m, a.part_ml[2 * slot(g)]);
+    for (int k = lane; k < parts; k += 64) m = fmaxf(m, a.part_ml[2 * slot(k)]);
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
     const float base = m == -INFINITY ? 0.0f : m;
     float l = 0.0f, o[D / 64];
 #pragma unroll
     for (int d = 0; d < D / 64; d++) o[d] = 0.0f;
-    for (int g = g0; g <= g1; g += 64) {
-        const int parts = min(64, g1 + 1 - g);
+    for (int k0 = 0; k0 < parts; k0 += 64) {
+        const int some = min(64, parts - k0);
         float f = 0.0f;
-        if (lane < parts) {
-            f = fast_exp2(a.part_ml[2 * slot(g + lane)] - base);
-            l = fmaf(f, a.part_ml[2 * slot(g + lane) + 1], l);
+        if (lane < some) {
+            f = fast_exp2(a.part_ml[2 * slot(k0 + lane)] - base);
+            l = fmaf(f, a.part_ml[2 * slot(k0 + lane) + 1], l);
         }
 #pragma unroll 4
-        for (int k = 0; k < parts; k++) {
-            const float *p = a.part_o + slot(g + k) * D + lane;
+        for (int k = 0; k < some; k++) {
+            const float *p = a.part_o + slot(k0 + k) * D + lane;
             const float fk = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, f), k));
 #pragma unroll
             for (int d = 0; d < D / 64; d++) o[d] = fmaf(fk, p[64 * d], o[d]);
@@ -667,8 +640,36 @@ __global__ __launch_bounds__(256) void fm_attn_join(FmKv c, FmAttn a, FmSeqs b) 
     l = fm_group_sum<64>(l);
     const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int d = 0; d < D / 64; d++)
-        fm_st1<BF16>(a.out, (row * a.q_heads + h * a.group + cc % a.group) * D + 64 * d + lane, o[d] * inv);
+    for (int d = 0; d < D / 64; d++) fm_st1<BF16>(a.out, to + 64 * d + lane, o[d] * inv);
+}
+
+// Narrow tiles that several workgroups took: four columns a workgroup.
+template <int D, bool BF16>
+__global__ __launch_bounds__(256) void fm_attn_join(FmKv c, FmAttn a, FmSeqs b) {
+    const int s = blockIdx.z, h = blockIdx.y, tile = blockIdx.x >> 2;
+    const int n = fm_seq_rows(b, s);
+    if (tile >= fm_attn_tiles(n, a.group, 0)) return;
+    const int len = c.len[s], from = a.first[s], per_head = (a.first[s + 1] - from) / c.kv_heads;
+    const int share = fm_attn_share(a.first[b.n_seq], a.groups), steps = fm_attn_steps(n, a.group, 0, len, a.max_len, tile);
+    int at = from + h * per_head;
+    for (int t = 0; t < tile; t++) at += fm_attn_steps(n, a.group, 0, len, a.max_len, t);
+    const int g0 = at / share, g1 = (at + steps - 1) / share;
+    if (g0 == g1) return;
+    const int col = 4 * (blockIdx.x & 3) + (threadIdx.x >> 6), cc = tile * COLS + col;
+    if (cc >= n * a.group) return;
+    join_column<D, BF16>(a, g1 - g0 + 1, [&](int k) { return (int64_t)fm_attn_slot(g0 + k, (g0 + k) * share - at) * COLS + col; },
+                         ((int64_t)(fm_seq_row0(b, s) + cc / a.group) * a.q_heads + h * a.group + cc % a.group) * D);
+}
+
+// Wide tiles in parts: four columns a workgroup.
+template <int D, bool BF16>
+__global__ __launch_bounds__(256) void fm_attn_wide_join(FmKv c, FmAttn a, FmSeqs b, FmWide w) {
+    const int tile = blockIdx.x / (FM_ATTN_WIDE / 4), col = 4 * (blockIdx.x % (FM_ATTN_WIDE / 4)) + (threadIdx.x >> 6);
+    const FmWideUnit at = fm_attn_wide_unit(w, b.n_seq, c.kv_heads, a.splits, tile * a.splits);
+    const int cc = at.tile * FM_ATTN_WIDE + col;
+    if (cc >= fm_seq_rows(b, at.s) * a.group) return;
+    join_column<D, BF16>(a, a.splits, [&](int k) { return ((int64_t)tile * a.splits + k) * FM_ATTN_WIDE + col; },
+                         ((int64_t)(fm_seq_row0(b, at.s) + cc / a.group) * a.q_heads + at.h * a.group + cc % a.group) * D);
 }
 
 // ---- the cache's rows --------------------------------------------------------------------------
@@ -801,11 +802,17 @@ __global__ __launch_bounds__(256) void fm_kv_read(FmKv c, FmKvRows x, int D, FmS
 template <int D, bool BF16>
 void launch_attn(const FmKv &c, const FmAttn &a, const FmSeqs &b, hipStream_t st) {
     const dim3 grid(a.groups), block(256);
-    if (a.wide) hipLaunchKernelGGL((fm_attn_wide<D, BF16>), grid, block, 0, st, c, a, b);
-    else if (a.n_tiles == 1) hipLaunchKernelGGL((fm_attn_narrow<D, BF16, true>), grid, block, 0, st, c, a, b);
+    if (a.wide) {
+        FmWide w;
+        fm_attn_wide_tiles(b, a.group, &w);
+        hipLaunchKernelGGL((fm_attn_wide<D, BF16>), grid, block, 0, st, c, a, b, w);
+        if (a.splits > 1)
+            hipLaunchKernelGGL((fm_attn_wide_join<D, BF16>), dim3(w.first[b.n_seq] * c.kv_heads * (FM_ATTN_WIDE / 4)), block, 0, st, c, a, b, w);
+        return;
+    }
+    if (a.n_tiles == 1) hipLaunchKernelGGL((fm_attn_narrow<D, BF16, true>), grid, block, 0, st, c, a, b);
     else hipLaunchKernelGGL((fm_attn_narrow<D, BF16, false>), grid, block, 0, st, c, a, b);
-    if (a.groups > 1)
-        hipLaunchKernelGGL((fm_attn_join<D, BF16>), dim3(a.n_tiles * (fm_attn_cols(a.wide) / 4), c.kv_heads, b.n_seq), block, 0, st, c, a, b);
+    if (a.groups > 1) hipLaunchKernelGGL((fm_attn_join<D, BF16>), dim3(4 * a.n_tiles, c.kv_heads, b.n_seq), block, 0, st, c, a, b);
 }
 
 }  // namespace
@@ -816,8 +823,10 @@ extern "C" int fm_launch_attn(const FmKv *c, const FmAttn *args, const FmSeqs *b
         FmAttn a = *args;
         fm_attn_plan(c, &a, b, D, n_cu, wide);
         if (!a.n_tiles) continue;
-        const size_t cols = (size_t)2 * a.groups * fm_attn_cols(wide);
-        a.part_o = (float *)ws;
+        FmWide w;
+        fm_attn_wide_tiles(*b, a.group, &w);
+        const size_t cols = wide ? (size_t)w.first[b->n_seq] * c->kv_heads * a.splits * FM_ATTN_WIDE : (size_t)2 * a.groups * COLS;
+        a.part_o = (float *)ws;      // (parts | maximum and sum of each | steps before each sequence)
         a.part_ml = a.part_o + cols * D;
         a.first = (int *)(a.part_ml + cols * 2);
         switch (D) {

@@ -179,7 +179,8 @@ struct FmAttn {
     int n_tiles;            // column tiles of the launch's sequence with the most rows
     int groups;             // workgroups that share the steps
     float *part_o, *part_ml;
-    int *first;             // steps before each sequence, for the join
+    int *first;             // narrow tiles: steps before each sequence, for the join
+    int splits;             // wide tiles: parts that a tile's steps are cut into
 };
 #define FM_ATTN_KEYS 64     // keys of a wave's step
 #define FM_ATTN_WAVES 4     // waves of a workgroup
@@ -412,17 +413,65 @@ inline int fm_most_rows(const FmSeqs &b) {
 }
 inline int fm_all_rows(const FmSeqs &b) { return b.one_row ? b.n_seq : b.start[b.n_seq]; }
 
+// Wide tiles: a workgroup takes whole tiles, or one of `splits` equal parts of a tile's steps where there are fewer
+// tiles than workgroups.  Unit u of the launch is part u % splits of tile u / splits; tiles are numbered with the
+// cache head running fastest (workgroups of one XCD then share a head's codes) and the sequences' last,
+// longest tiles first.
+struct FmWide {
+    int first[FM_MAX_SEQ + 1];      // tiles of one head in the sequences before
+};
+inline void fm_attn_wide_tiles(const FmSeqs &b, int group, FmWide *w) {
+    w->first[0] = 0;
+    for (int s = 0; s < b.n_seq; s++) w->first[s + 1] = w->first[s] + fm_attn_tiles(fm_seq_rows(b, s), group, 1);
+}
+struct FmWideUnit {
+    int s, h, tile, part;
+};
+FM_HD FmWideUnit fm_attn_wide_unit(const FmWide &w, int n_seq, int kv_heads, int splits, int u) {
+    FmWideUnit r;
+    r.part = u % splits;
+    u /= splits;
+    r.h = u % kv_heads;
+    const int t = w.first[n_seq] - 1 - u / kv_heads;
+    int lo = 0, hi = n_seq;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (w.first[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    r.s = lo;
+    r.tile = t - w.first[lo];
+    return r;
+}
+// Rounds of workgroups go through the units to and fro, so that whoever got the longest of a round gets
+// the shortest of the next.
+FM_HD int fm_attn_wide_pick(int round, int group, int groups) {
+    return round * groups + (round & 1 ? groups - 1 - group : group);
+}
+// Parts of a tile: the number up to 16 whose rounds take least, a part costing a sixteenth of a tile's
+// longest on top for being written and joined.
+inline int fm_attn_splits(int64_t tiles, int groups, int most_steps) {
+    int best = 1;
+    double least = 1e30;
+    for (int s = 1; s <= 16 && (s == 1 || s * FM_ATTN_WAVES <= most_steps); s++) {
+        const double t = (double)((tiles * s + groups - 1) / groups) * (1.0 / s + (s > 1 ? 1.0 / 16 : 0.0));
+        if (t < least * 0.999) least = t, best = s;
+    }
+    return best;
+}
+
 // Workgroups of a CU.  Narrow tiles: heads of 256 take a wave more registers than half a SIMD has (and a
 // spilled one would wait for the codes in flight).  Wide tiles keep two steps of keys and values in LDS.
 FM_HDC int fm_attn_per_cu(int D, int wide) { return D == 256 || wide ? 1 : 2; }
 // Attention: the workgroups that fit on the chip share the steps, fewer if there cannot be as many.  Sets
-// n_tiles (0: no sequence for this launch) and groups; returns the workspace: two parts per workgroup and
-// the steps before each sequence.
+// n_tiles (0: no sequence for this launch), groups and splits; returns the workspace: of narrow tiles two parts
+// per workgroup and the steps before each sequence, of wide ones the parts of split tiles.
 inline size_t fm_attn_plan(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int n_cu, int wide) {
     const int64_t have = (int64_t)c->max_pages * c->page_tokens;
     if (a->max_len > have) a->max_len = (int)have;
     a->wide = wide;
     a->n_tiles = 0;
+    a->splits = 1;
     int64_t most = 0;
     for (int s = 0; s < b->n_seq; s++) {
         const int tiles = fm_attn_tiles(fm_seq_rows(*b, s), a->group, wide);
@@ -430,6 +479,14 @@ inline size_t fm_attn_plan(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int
         most += (int64_t)c->kv_heads * tiles * ((a->max_len + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS + 1);
     }
     if (!a->n_tiles) return 0;
+    if (wide) {
+        FmWide w;
+        fm_attn_wide_tiles(*b, a->group, &w);
+        const int64_t tiles = (int64_t)w.first[b->n_seq] * c->kv_heads;
+        a->splits = fm_attn_splits(tiles, n_cu, (a->max_len + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS);
+        a->groups = (int)(tiles * a->splits < n_cu ? tiles * a->splits : n_cu);
+        return a->splits == 1 ? 0 : (size_t)tiles * a->splits * FM_ATTN_WIDE * (D + 2) * sizeof(float);
+    }
     const int64_t groups = (most + FM_ATTN_WAVES - 1) / FM_ATTN_WAVES, fit = fm_attn_per_cu(D, wide) * n_cu;
     a->groups = (int)(groups < 1 ? 1 : groups > fit ? fit : groups);
     return (size_t)2 * a->groups * fm_attn_cols(wide) * (D + 2) * sizeof(float) + (FM_MAX_SEQ + 1) * sizeof(int);

@@ -225,7 +225,7 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
     std::vector<int> start(n_seq + 1, 0);
     for (int s = 0; s < n_seq; s++) {
         len[s] = rnd(8) ? rnd(max_pages * P + 40) : (rnd(2) ? -3 : 0);
-        start[s + 1] = start[s] + rnd(70);
+        start[s + 1] = start[s] + rnd(rnd(3) ? 70 : 400);
     }
     FmKv c{};
     c.n_pages = n_pages, c.page_tokens = P, c.page_shift = __builtin_ctz((unsigned)P), c.kv_heads = kv;
@@ -245,7 +245,28 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
             continue;
         }
         CHECK(a.groups >= 1);
-        share_out(c, a, b, D, ws);
+        if (!wide) share_out(c, a, b, D, ws);
+        else {
+            FmWide w;
+            fm_attn_wide_tiles(b, group, &w);
+            const int tiles = w.first[n_seq] * kv, units = tiles * a.splits;
+            CHECK(a.groups <= units && ws == (a.splits == 1 ? 0 : (size_t)units * FM_ATTN_WIDE * (D + 2) * 4));
+            std::set<int> picked;
+            for (int round = 0; round * a.groups < units; round++)
+                for (int g = 0; g < a.groups; g++) {
+                    const int u = fm_attn_wide_pick(round, g, a.groups);
+                    if (u < units) CHECK(picked.insert(u).second);
+                }
+            CHECK((int)picked.size() == units);
+            std::set<std::vector<int>> seen;
+            for (int u = 0; u < units; u++) {
+                const FmWideUnit at = fm_attn_wide_unit(w, n_seq, kv, a.splits, u);
+                CHECK(at.s < n_seq && at.h < kv && at.part < a.splits && at.tile >= 0 && at.tile < fm_attn_tiles(fm_seq_rows(b, at.s), group, 1));
+                CHECK(seen.insert({at.s, at.h, at.tile, at.part}).second);
+                const FmWideUnit one = fm_attn_wide_unit(w, n_seq, kv, a.splits, u / a.splits * a.splits);
+                CHECK(one.s == at.s && one.h == at.h && one.tile == at.tile && one.part == 0);
+            }
+        }
     }
     for (int s = 0; s < n_seq; s++) {      // a sequence's columns are in one of the two launches
         const int n = fm_seq_rows(b, s), narrow = fm_attn_tiles(n, group, 0), wides = fm_attn_tiles(n, group, 1);
@@ -328,7 +349,7 @@ static void plan_gdn() {
     CHECK(fm_gdn_ws_bytes(&a, nullptr, 200) == 0);
     const FmGdnWs w = fm_gdn_ws(a);
     CHECK(w.tm % 4 == 0 && w.p % 4 == 0 && w.sc % 4 == 0 && w.floats % 4 == 0 && w.end + a.v_heads <= w.floats);
-    CHECK(sizeof(FmGdnSeqs) + sizeof(FmGdn) + 8 <= 4096 && sizeof(FmSeqs) + sizeof(FmKv) + sizeof(FmAttn) <= 4096);
+    CHECK(sizeof(FmGdnSeqs) + sizeof(FmGdn) + 8 <= 4096 && sizeof(FmSeqs) + sizeof(FmKv) + sizeof(FmAttn) + sizeof(FmWide) <= 4096);
 }
 
 int main() {
