@@ -307,7 +307,7 @@ __device__ __forceinline__ void add_steps(const FmKv &c, const FmAttn &a, const 
 // Narrow tiles: a workgroup takes its share of the steps, tile by tile; the four waves take a tile's steps
 // in turn and are joined through LDS.
 template <int D, bool BF16, bool ONCE>
-__global__ __launch_bounds__(256, fm_attn_per_cu(D, 0)) void fm_attn_narrow(FmKv c, FmAttn a, FmSeqs b) {
+__global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c, FmAttn a, FmSeqs b) {
     constexpr int NP = BF16 ? 1 : 2, DT = D / 16;
     __shared__ float s_o[3][DT][64][4];
     __shared__ float s_m[4][16], s_l[4][16];
@@ -406,37 +406,47 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D, 0)) void fm_attn_narrow(FmKv
     }
 }
 
-// Wide tiles: 128 columns of one (sequence, cache head), 32 a wave.  The workgroup turns a step's codes into
-// fp16 operands in LDS once, [tile][k step][lane] of 16 bytes, and its waves read them for their columns.
-// The codes of the next step are in registers meanwhile and go to the other half of the LDS at the step's
-// end: one barrier a step.  A step of a wave is 128 matrix instructions of 16 cycles (256 with two
-// pieces) and as much LDS time; conversion is shared by 128 columns.
+// Wide tiles: 128 columns of one (sequence, cache head), 64 with two pieces.  The workgroup turns a step's codes
+// into fp16 operands in LDS once, [tile][k step][lane] of 16 bytes; the queries lie there too.  Eight waves:
+// wave w has the columns of group w & 3 (16 CT of them) and one half of a step's keys, w >> 2, with a
+// running maximum, sum and output of its own; the halves are joined at the tile's end.  Two waves per
+// SIMD, so that one's softmax runs beside the other's products, in 256 registers each.
+// The codes of the next step are on their way in registers meanwhile; keys are replaced behind the first
+// product's barrier, values behind the second's, so a step has two barriers and one copy of each.
+// Bound by the matrix cores and the LDS alike: of a step of 128 columns x 64 keys x 256 dims, 2048 cycles of
+// products per SIMD, 3072 cycles of operand reads per CU.
 template <int D, bool BF16>
-__global__ __launch_bounds__(256, 1) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs b, FmWide w) {
-    constexpr int NP = BF16 ? 1 : 2, KS = D / 32, DT = D / 16, CT = 2, LD = D / 64;
-    __shared__ fm_v8h s_k[2][4 * KS * 64], s_v[2][DT * 2 * 64];
+__global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs b, FmWide w) {
+    constexpr int NP = BF16 ? 1 : 2, CT = BF16 ? 2 : 1, KS = D / 32, DT = D / 16, LD = D / 64, WIDE = 64 * CT;
+    constexpr int UNITS = 4 * LD, MY = (UNITS + 7) / 8;          // loads of a wave and step, for K and for V
+    // K [4][KS][64] | V [DT][2][64] | q [4][CT][NP][KS][64], then o of four waves [4][CT][DT][64]
+    constexpr int K_AT = 0, V_AT = 4 * KS * 64, Q_AT = V_AT + DT * 2 * 64, ALL = Q_AT + 4 * CT * NP * KS * 64;
+    constexpr int O_ALL = 4 * CT * DT * 64;
+    __shared__ fm_v8h lds[ALL > O_ALL ? ALL : O_ALL];
+    __shared__ float s_m[4][CT][16], s_l[4][CT][16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
+    const int cg = wave & 3, half = wave >> 2;
+    const fm_v8h *s_k = lds + K_AT + lane, *s_v = lds + V_AT + lane;
+    fm_v8h *s_q = lds + Q_AT + cg * CT * NP * KS * 64 + lane;
     const int units = w.first[b.n_seq] * c.kv_heads * a.splits;
     for (int round = 0; round * a.groups < units; round++) {
         const int unit = fm_attn_wide_pick(round, blockIdx.x, a.groups);
         if (unit >= units) continue;
         const FmWideUnit at = fm_attn_wide_unit(w, b.n_seq, c.kv_heads, a.splits, unit);
         const int s = at.s, h = at.h, tile = at.tile, n = fm_seq_rows(b, s), len = __builtin_amdgcn_readfirstlane(c.len[s]);
-        const int steps = fm_attn_steps(n, a.group, 1, len, a.max_len, tile);
+        const int steps = fm_attn_steps(n, a.group, WIDE, len, a.max_len, tile);
         const int s0 = (int)((int64_t)steps * at.part / a.splits), s1 = (int)((int64_t)steps * (at.part + 1) / a.splits);
-
         const int32_t *table = c.pages + (int64_t)s * c.max_pages;
-        fm_v8h q[CT][NP][KS];
+        Runs now, next;
+        now.load(c, table, s0 * BK);
+        next.load(c, table, max(min(s0 + 1, s1 - 1), 0) * BK);
         fm_v4f o[CT][DT];
         float m[CT], l[CT], qscale[CT];
         int ref[CT], limit[CT], all_limit = 0x7FFFFFFF;
         int64_t to[CT];          // the column's place in the output, -1 if it is not there
-        Runs now, next;
-        now.load(c, table, s0 * BK);
-        next.load(c, table, max(min(s0 + 1, s1 - 1), 0) * BK);
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            const int cc = tile * FM_ATTN_WIDE + wave * 32 + ct * 16 + r;
+            const int cc = tile * WIDE + (cg * CT + ct) * 16 + r;
             const bool there = cc < n * a.group;
             const int i = there ? cc / a.group : 0, qh = h * a.group + (there ? cc % a.group : 0);
             const int64_t row = fm_seq_row0(b, s) + i;
@@ -460,15 +470,22 @@ __global__ __launch_bounds__(256, 1) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
             e = e > 100 ? 100 : e < -100 ? -100 : e;
             const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
             qscale[ct] = __uint_as_float((uint32_t)(127 - 8 + e) << 23) * a.scale_log2;
+            // (both halves' waves have the columns: each writes half of the k steps)
+            if (!ct) lds_barrier();                               // (the last tile's operands have been read)
 #pragma unroll
-            for (int k = 0; k < KS; k++)
+            for (int k = 0; k < KS; k++) {
+                if ((k & 1) != half) continue;
+                fm_v8h v[NP];
 #pragma unroll
                 for (int j = 0; j < 8; j++) {
                     _Float16 piece[NP];
                     split<NP>(x[k][j >> 2][j & 3] * up, piece);
 #pragma unroll
-                    for (int p = 0; p < NP; p++) q[ct][p][k][j] = piece[p];
+                    for (int p = 0; p < NP; p++) v[p][j] = piece[p];
                 }
+#pragma unroll
+                for (int p = 0; p < NP; p++) s_q[((ct * NP + p) * KS + k) * 64] = v[p];
+            }
             m[ct] = -INFINITY;
             l[ct] = 0.0f;
             ref[ct] = -100;
@@ -476,56 +493,70 @@ __global__ __launch_bounds__(256, 1) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
             for (int d = 0; d < DT; d++) o[ct][d] = fm_v4f{0.f, 0.f, 0.f, 0.f};
         }
         for (int x = 32; x; x >>= 1) all_limit = min(all_limit, __shfl_xor(all_limit, x));
-        // this wave's part of a step's codes: key tile `wave`, dims tiles wave * LD ..
-        fm_v4u kc[LD], vc[LD];
+        // this wave's loads: unit u of K is tile u & 3, dims 64 (u >> 2) ..; of V dims 16 u ..
+        fm_v4u kc[MY], vc[MY];
         float ks, vs;
         auto fetch = [&](const Runs &p, int pos) {
-            const int8_t *kb = c.k + fm_kv_k_at(c, D, max(p.k_page(c, pos), 0), h, pos + 16 * (r >> 2) + (r & 3) + 4 * wave, 16 * g);
-            const int8_t *vb = c.v + fm_kv_v_at(c, D, max(p.v_page(c, pos), 0), h, pos + 16 * g, 16 * wave * LD + r);
             const int64_t sc = (int64_t)max(p.v_page(c, pos), 0) * c.kv_heads + h;
+            const int8_t *kb = c.k + fm_kv_k_at(c, D, max(p.k_page(c, pos), 0), h, pos + 16 * (r >> 2) + (r & 3) + 4 * (wave & 3), 16 * g);
+            const int8_t *vb = c.v + fm_kv_v_at(c, D, max(p.v_page(c, pos), 0), h, pos + 16 * g, r);
 #pragma unroll
-            for (int d = 0; d < LD; d++) kc[d] = *(const fm_v4u *)(kb + 64 * d);
+            for (int j = 0; j < MY; j++) kc[j] = *(const fm_v4u *)(kb + 64 * (min(wave + 8 * j, UNITS - 1) >> 2));
 #pragma unroll
-            for (int d = 0; d < LD; d++) vc[d] = *(const fm_v4u *)(vb + 16 * d * c.page_tokens);
+            for (int j = 0; j < MY; j++) vc[j] = *(const fm_v4u *)(vb + 16 * min(wave + 8 * j, UNITS - 1) * c.page_tokens);
             ks = c.k_scale[sc];
             vs = c.v_scale[sc];
         };
-        auto put = [&](int buf) {
+        auto put_k = [&]() {
 #pragma unroll
-            for (int d = 0; d < LD; d++) {
-                s_k[buf][(wave * KS + 2 * d) * 64 + lane] = codes_f16(kc[d][0], kc[d][1]);
-                s_k[buf][(wave * KS + 2 * d + 1) * 64 + lane] = codes_f16(kc[d][2], kc[d][3]);
-                s_v[buf][(wave * LD + d) * 128 + lane] = codes_f16(vc[d][0], vc[d][1]);
-                s_v[buf][(wave * LD + d) * 128 + 64 + lane] = codes_f16(vc[d][2], vc[d][3]);
+            for (int j = 0; j < MY; j++) {
+                const int u = wave + 8 * j;
+                if (u >= UNITS) continue;
+                fm_v8h *z = lds + K_AT + ((u & 3) * KS + 2 * (u >> 2)) * 64 + lane;
+                z[0] = codes_f16(kc[j][0], kc[j][1]);
+                z[64] = codes_f16(kc[j][2], kc[j][3]);
             }
         };
-        lds_barrier();                                            // (the last tile's operands have been read)
+        auto put_v = [&]() {
+#pragma unroll
+            for (int j = 0; j < MY; j++) {
+                const int u = wave + 8 * j;
+                if (u >= UNITS) continue;
+                fm_v8h *z = lds + V_AT + u * 128 + lane;
+                z[0] = codes_f16(vc[j][0], vc[j][1]);
+                z[64] = codes_f16(vc[j][2], vc[j][3]);
+            }
+        };
         fetch(now, s0 * BK);
-        put(0);
+        put_k();
         for (int st = s0; st < s1; st++) {
-            const int pos = st * BK, buf = (st - s0) & 1, vpos = pos + 16 * g;
+            const int pos = st * BK, vpos = pos + 16 * g + 8 * half;      // first of this lane's eight keys
             const float k_scale = ks, v_scale0 = vs;
             const bool there = now.v_page(c, pos) >= 0;
-            lds_barrier();                                        // this step's operands are there
+            lds_barrier();                                        // the step's keys are there, the last one's values read
+            put_v();
             Runs later;
             later.load(c, table, min(st + 2, s1 - 1) * BK);
             fetch(next, min(st + 1, s1 - 1) * BK);
-            fm_v4f sc[CT][4];
+            fm_v4f sc[CT][2];
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
+            for (int ct = 0; ct < CT; ct++) sc[ct][0] = sc[ct][1] = fm_v4f{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++) sc[ct][t] = fm_v4f{0.f, 0.f, 0.f, 0.f};
+            for (int k = 0; k < KS; k++) {
+                const fm_v8h x0 = s_k[(2 * half * KS + k) * 64], x1 = s_k[((2 * half + 1) * KS + k) * 64];
 #pragma unroll
-                for (int k = 0; k < KS; k++) {
-                    const fm_v8h x = s_k[buf][(t * KS + k) * 64 + lane];
+                for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                    for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                        for (int p = 0; p < NP; p++) sc[ct][t] = mfma(x, q[ct][p][k], sc[ct][t]);
-                }
+                    for (int p = 0; p < NP; p++) {
+                        const fm_v8h y = s_q[((ct * NP + p) * KS + k) * 64];
+                        sc[ct][0] = mfma(x0, y, sc[ct][0]);
+                        sc[ct][1] = mfma(x1, y, sc[ct][1]);
+                    }
             }
+            lds_barrier();                                        // the keys have been read, the values are there
+            if (st + 1 < s1) put_k();
             const bool whole = __all(there) && pos + BK <= all_limit;      // nothing of the step is masked
-            fm_v8h p8[CT][NP][2];
+            fm_v8h p8[CT][NP];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
                 const bool live = there && vpos < limit[ct];
@@ -533,12 +564,12 @@ __global__ __launch_bounds__(256, 1) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
                 float v_scale = live ? v_scale0 : 0.0f, top = -INFINITY;
                 if (whole) {
 #pragma unroll
-                    for (int t = 0; t < 4; t++)
+                    for (int t = 0; t < 2; t++)
 #pragma unroll
                         for (int i = 0; i < 4; i++) sc[ct][t][i] *= f, top = fmaxf(top, sc[ct][t][i]);
                 } else {
 #pragma unroll
-                    for (int t = 0; t < 4; t++)
+                    for (int t = 0; t < 2; t++)
 #pragma unroll
                         for (int i = 0; i < 4; i++) {
                             sc[ct][t][i] = live && vpos + 4 * t + i < limit[ct] ? sc[ct][t][i] * f : -INFINITY;
@@ -564,7 +595,7 @@ __global__ __launch_bounds__(256, 1) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
                 }
                 const float shift = P_SHIFT - base;
 #pragma unroll
-                for (int t = 0; t < 4; t++)
+                for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
                         const float e = fast_exp2(sc[ct][t][i] + shift);
@@ -572,40 +603,53 @@ __global__ __launch_bounds__(256, 1) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
                         _Float16 piece[NP];
                         split<NP>(e * v_scale, piece);
 #pragma unroll
-                        for (int p = 0; p < NP; p++) p8[ct][p][t >> 1][4 * (t & 1) + i] = piece[p];
+                        for (int p = 0; p < NP; p++) p8[ct][p][4 * t + i] = piece[p];
                     }
             }
 #pragma unroll
-            for (int d = 0; d < DT; d++)
+            for (int d = 0; d < DT; d++) {
+                const fm_v8h x = s_v[(d * 2 + half) * 64];
 #pragma unroll
-                for (int k = 0; k < 2; k++) {
-                    const fm_v8h x = s_v[buf][(d * 2 + k) * 64 + lane];
+                for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                    for (int ct = 0; ct < CT; ct++)
-#pragma unroll
-                        for (int p = 0; p < NP; p++) o[ct][d] = mfma(x, p8[ct][p][k], o[ct][d]);
-                }
-            if (st + 1 < s1) put(buf ^ 1);
+                    for (int p = 0; p < NP; p++) o[ct][d] = mfma(x, p8[ct][p], o[ct][d]);
+            }
             now = next;
             next = later;
         }
+        // the second halves' outputs to the first halves' waves, at the common maximum
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
-            float sum = l[ct];
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (to[ct] < 0) continue;
-            const float unit2 = ldexpf(1.0f, ref[ct]);
-            if (a.splits == 1) {
-                const float inv = sum > 0.0f || sum != sum ? unit2 / sum : 0.0f;
+            l[ct] += __shfl_xor(l[ct], 16);
+            l[ct] += __shfl_xor(l[ct], 32);
+        }
+        lds_barrier();                                            // operands have been read
+        if (half) {
 #pragma unroll
-                for (int d = 0; d < DT; d++) fm_st4<BF16>(a.out, to[ct] + 16 * d + 4 * g, o[ct][d] * inv);
-            } else {
-                const int64_t part = (int64_t)unit * FM_ATTN_WIDE + wave * 32 + ct * 16 + r;
+            for (int ct = 0; ct < CT; ct++) {
+                const float unit2 = ldexpf(1.0f, ref[ct]);
+                if (g == 0) s_m[cg][ct][r] = m[ct], s_l[cg][ct][r] = l[ct];
 #pragma unroll
-                for (int d = 0; d < DT; d++) *(fm_v4f *)(a.part_o + part * D + 16 * d + 4 * g) = o[ct][d] * unit2;
-                if (g == 0) a.part_ml[2 * part] = m[ct], a.part_ml[2 * part + 1] = sum;
+                for (int d = 0; d < DT; d++) *(fm_v4f *)(lds + ((cg * CT + ct) * DT + d) * 64 + lane) = o[ct][d] * unit2;
             }
+        }
+        lds_barrier();
+        if (half) continue;
+#pragma unroll
+        for (int ct = 0; ct < CT; ct++) {
+            if (to[ct] < 0) continue;
+            const float m2 = s_m[cg][ct][r], both = fmaxf(m[ct], m2), base = both == -INFINITY ? 0.0f : both;
+            const float e1 = fast_exp2(m[ct] - base), e2 = fast_exp2(m2 - base), f1 = ldexpf(e1, ref[ct]);
+            const float sum = e1 * l[ct] + e2 * s_l[cg][ct][r];
+            const float inv = a.splits > 1 ? 1.0f : sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+            const int64_t part = (int64_t)unit * WIDE + (cg * CT + ct) * 16 + r;
+#pragma unroll
+            for (int d = 0; d < DT; d++) {
+                const fm_v4f z = (o[ct][d] * f1 + *(const fm_v4f *)(lds + ((cg * CT + ct) * DT + d) * 64 + lane) * e2) * inv;
+                if (a.splits == 1) fm_st4<BF16>(a.out, to[ct] + 16 * d + 4 * g, z);
+                else *(fm_v4f *)(a.part_o + part * D + 16 * d + 4 * g) = z;
+            }
+            if (a.splits > 1 && g == 0) a.part_ml[2 * part] = both, a.part_ml[2 * part + 1] = sum;
         }
     }
 }
@@ -664,11 +708,11 @@ __global__ __launch_bounds__(256) void fm_attn_join(FmKv c, FmAttn a, FmSeqs b) 
 // Wide tiles in parts: four columns a workgroup.
 template <int D, bool BF16>
 __global__ __launch_bounds__(256) void fm_attn_wide_join(FmKv c, FmAttn a, FmSeqs b, FmWide w) {
-    const int tile = blockIdx.x / (FM_ATTN_WIDE / 4), col = 4 * (blockIdx.x % (FM_ATTN_WIDE / 4)) + (threadIdx.x >> 6);
+    const int tile = blockIdx.x / (a.wide / 4), col = 4 * (blockIdx.x % (a.wide / 4)) + (threadIdx.x >> 6);
     const FmWideUnit at = fm_attn_wide_unit(w, b.n_seq, c.kv_heads, a.splits, tile * a.splits);
-    const int cc = at.tile * FM_ATTN_WIDE + col;
+    const int cc = at.tile * a.wide + col;
     if (cc >= fm_seq_rows(b, at.s) * a.group) return;
-    join_column<D, BF16>(a, a.splits, [&](int k) { return ((int64_t)tile * a.splits + k) * FM_ATTN_WIDE + col; },
+    join_column<D, BF16>(a, a.splits, [&](int k) { return ((int64_t)tile * a.splits + k) * a.wide + col; },
                          ((int64_t)(fm_seq_row0(b, at.s) + cc / a.group) * a.q_heads + at.h * a.group + cc % a.group) * D);
 }
 
@@ -804,10 +848,10 @@ void launch_attn(const FmKv &c, const FmAttn &a, const FmSeqs &b, hipStream_t st
     const dim3 grid(a.groups), block(256);
     if (a.wide) {
         FmWide w;
-        fm_attn_wide_tiles(b, a.group, &w);
-        hipLaunchKernelGGL((fm_attn_wide<D, BF16>), grid, block, 0, st, c, a, b, w);
+        fm_attn_wide_tiles(b, a.group, a.wide, &w);
+        hipLaunchKernelGGL((fm_attn_wide<D, BF16>), grid, dim3(512), 0, st, c, a, b, w);
         if (a.splits > 1)
-            hipLaunchKernelGGL((fm_attn_wide_join<D, BF16>), dim3(w.first[b.n_seq] * c.kv_heads * (FM_ATTN_WIDE / 4)), block, 0, st, c, a, b, w);
+            hipLaunchKernelGGL((fm_attn_wide_join<D, BF16>), dim3(w.first[b.n_seq] * c.kv_heads * (a.wide / 4)), block, 0, st, c, a, b, w);
         return;
     }
     if (a.n_tiles == 1) hipLaunchKernelGGL((fm_attn_narrow<D, BF16, true>), grid, block, 0, st, c, a, b);
@@ -819,13 +863,14 @@ void launch_attn(const FmKv &c, const FmAttn &a, const FmSeqs &b, hipStream_t st
 
 // ws: what fm_attn_check asked for
 extern "C" int fm_launch_attn(const FmKv *c, const FmAttn *args, const FmSeqs *b, int D, int bf16, void *ws, int n_cu, hipStream_t st) {
-    for (int wide = 0; wide < 2; wide++) {
+    for (int pass = 0; pass < 2; pass++) {
+        const int wide = pass ? fm_attn_wide_cols(bf16) : 0;
         FmAttn a = *args;
         fm_attn_plan(c, &a, b, D, n_cu, wide);
         if (!a.n_tiles) continue;
         FmWide w;
-        fm_attn_wide_tiles(*b, a.group, &w);
-        const size_t cols = wide ? (size_t)w.first[b->n_seq] * c->kv_heads * a.splits * FM_ATTN_WIDE : (size_t)2 * a.groups * COLS;
+        fm_attn_wide_tiles(*b, a.group, wide, &w);
+        const size_t cols = wide ? (size_t)w.first[b->n_seq] * c->kv_heads * a.splits * wide : (size_t)2 * a.groups * COLS;
         a.part_o = (float *)ws;      // (parts | maximum and sum of each | steps before each sequence)
         a.part_ml = a.part_o + cols * D;
         a.first = (int *)(a.part_ml + cols * 2);

@@ -175,7 +175,7 @@ struct FmAttn {
     int q_heads, group;     // query heads per cache head
     float scale_log2;       // scale * log2(e)
     int max_len;            // keys from here on are not seen, at most max_pages * page_tokens
-    int wide;               // which sequences a launch takes: those of wide tiles, or the others
+    int wide;               // columns of a wide tile; 0: the launch of the sequences that have narrow ones
     int n_tiles;            // column tiles of the launch's sequence with the most rows
     int groups;             // workgroups that share the steps
     float *part_o, *part_ml;
@@ -183,17 +183,18 @@ struct FmAttn {
     int splits;             // wide tiles: parts that a tile's steps are cut into
 };
 #define FM_ATTN_KEYS 64     // keys of a wave's step
-#define FM_ATTN_WAVES 4     // waves of a workgroup
+#define FM_ATTN_WAVES 4     // waves of a narrow tile's workgroup
 #define FM_ATTN_COLS 16     // columns of a narrow tile: its waves take different keys
-#define FM_ATTN_WIDE 128    // columns of a wide one: its waves take different columns
+// columns of a wide one, whose queries lie in LDS: fp32 ones as two pieces
+FM_HDC int fm_attn_wide_cols(int bf16) { return bf16 ? 128 : 64; }
 // A sequence with more columns than this has wide tiles.
 #define FM_ATTN_NARROW_MOST 64
 
 // ---- attention's steps and who takes them --------------------------------------------------
 // A sequence of n rows has n * group columns per cache head (row * group + query head of the group) in
-// tiles of 16 or 128; a tile's steps are those of 64 keys up to the last one its last column sees, at least
+// tiles of 16 or (wide) 64 or 128; a tile's steps are those of 64 keys up to the last one its last column sees, at least
 // one (somebody has to write the zeros of a row that sees nothing).
-FM_HD int fm_attn_cols(int wide) { return wide ? FM_ATTN_WIDE : FM_ATTN_COLS; }
+FM_HD int fm_attn_cols(int wide) { return wide ? wide : FM_ATTN_COLS; }
 FM_HD int fm_attn_tiles(int n, int group, int wide) {
     if ((n * group > FM_ATTN_NARROW_MOST) != (wide != 0)) return 0;
     return (n * group + fm_attn_cols(wide) - 1) / fm_attn_cols(wide);
@@ -420,9 +421,9 @@ inline int fm_all_rows(const FmSeqs &b) { return b.one_row ? b.n_seq : b.start[b
 struct FmWide {
     int first[FM_MAX_SEQ + 1];      // tiles of one head in the sequences before
 };
-inline void fm_attn_wide_tiles(const FmSeqs &b, int group, FmWide *w) {
+inline void fm_attn_wide_tiles(const FmSeqs &b, int group, int wide, FmWide *w) {
     w->first[0] = 0;
-    for (int s = 0; s < b.n_seq; s++) w->first[s + 1] = w->first[s] + fm_attn_tiles(fm_seq_rows(b, s), group, 1);
+    for (int s = 0; s < b.n_seq; s++) w->first[s + 1] = w->first[s] + fm_attn_tiles(fm_seq_rows(b, s), group, wide);
 }
 struct FmWideUnit {
     int s, h, tile, part;
@@ -461,8 +462,8 @@ inline int fm_attn_splits(int64_t tiles, int groups, int most_steps) {
 }
 
 // Workgroups of a CU.  Narrow tiles: heads of 256 take a wave more registers than half a SIMD has (and a
-// spilled one would wait for the codes in flight).  Wide tiles keep two steps of keys and values in LDS.
-FM_HDC int fm_attn_per_cu(int D, int wide) { return D == 256 || wide ? 1 : 2; }
+// spilled one would wait for the codes in flight).
+FM_HDC int fm_attn_per_cu(int D) { return D == 256 ? 1 : 2; }
 // Attention: the workgroups that fit on the chip share the steps, fewer if there cannot be as many.  Sets
 // n_tiles (0: no sequence for this launch), groups and splits; returns the workspace: of narrow tiles two parts
 // per workgroup and the steps before each sequence, of wide ones the parts of split tiles.
@@ -481,13 +482,13 @@ inline size_t fm_attn_plan(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int
     if (!a->n_tiles) return 0;
     if (wide) {
         FmWide w;
-        fm_attn_wide_tiles(*b, a->group, &w);
+        fm_attn_wide_tiles(*b, a->group, wide, &w);
         const int64_t tiles = (int64_t)w.first[b->n_seq] * c->kv_heads;
         a->splits = fm_attn_splits(tiles, n_cu, (a->max_len + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS);
         a->groups = (int)(tiles * a->splits < n_cu ? tiles * a->splits : n_cu);
-        return a->splits == 1 ? 0 : (size_t)tiles * a->splits * FM_ATTN_WIDE * (D + 2) * sizeof(float);
+        return a->splits == 1 ? 0 : (size_t)tiles * a->splits * wide * (D + 2) * sizeof(float);
     }
-    const int64_t groups = (most + FM_ATTN_WAVES - 1) / FM_ATTN_WAVES, fit = fm_attn_per_cu(D, wide) * n_cu;
+    const int64_t groups = (most + FM_ATTN_WAVES - 1) / FM_ATTN_WAVES, fit = fm_attn_per_cu(D) * n_cu;
     a->groups = (int)(groups < 1 ? 1 : groups > fit ? fit : groups);
     return (size_t)2 * a->groups * fm_attn_cols(wide) * (D + 2) * sizeof(float) + (FM_MAX_SEQ + 1) * sizeof(int);
 }
@@ -514,7 +515,7 @@ inline int fm_attn_check(FmWhy *w, const fm_attn_args *p, int n_cu, FmKv *k, FmA
     a->max_len = p->max_len;
     fm_fill_seqs(b, p->seq_start, p->n_seq);
     FmAttn other = *a;       // (the two launches run one after the other in the same workspace)
-    const size_t wide = fm_attn_plan(k, &other, b, p->cache.head_dim, n_cu, 1);
+    const size_t wide = fm_attn_plan(k, &other, b, p->cache.head_dim, n_cu, fm_attn_wide_cols(p->dtype == FM_DTYPE_BF16));
     *ws = fm_attn_plan(k, a, b, p->cache.head_dim, n_cu, 0);
     if (wide > *ws) *ws = wide;
     return FM_OK;

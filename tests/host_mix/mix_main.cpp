@@ -237,7 +237,7 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
     b.n_seq = n_seq;
     for (int s = 0; s <= n_seq; s++) b.start[s] = start[s];
     int covered = 0;
-    for (int wide = 0; wide < 2; wide++) {
+    for (int wide : {0, rnd(2) ? 64 : 128}) {
         const size_t ws = fm_attn_plan(&c, &a, &b, D, 1 + rnd(64), wide);
         CHECK(a.max_len <= max_pages * P);
         if (!a.n_tiles) {
@@ -248,9 +248,9 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
         if (!wide) share_out(c, a, b, D, ws);
         else {
             FmWide w;
-            fm_attn_wide_tiles(b, group, &w);
+            fm_attn_wide_tiles(b, group, wide, &w);
             const int tiles = w.first[n_seq] * kv, units = tiles * a.splits;
-            CHECK(a.groups <= units && ws == (a.splits == 1 ? 0 : (size_t)units * FM_ATTN_WIDE * (D + 2) * 4));
+            CHECK(a.groups <= units && ws == (a.splits == 1 ? 0 : (size_t)units * wide * (D + 2) * 4));
             std::set<int> picked;
             for (int round = 0; round * a.groups < units; round++)
                 for (int g = 0; g < a.groups; g++) {
@@ -261,7 +261,7 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
             std::set<std::vector<int>> seen;
             for (int u = 0; u < units; u++) {
                 const FmWideUnit at = fm_attn_wide_unit(w, n_seq, kv, a.splits, u);
-                CHECK(at.s < n_seq && at.h < kv && at.part < a.splits && at.tile >= 0 && at.tile < fm_attn_tiles(fm_seq_rows(b, at.s), group, 1));
+                CHECK(at.s < n_seq && at.h < kv && at.part < a.splits && at.tile >= 0 && at.tile < fm_attn_tiles(fm_seq_rows(b, at.s), group, wide));
                 CHECK(seen.insert({at.s, at.h, at.tile, at.part}).second);
                 const FmWideUnit one = fm_attn_wide_unit(w, n_seq, kv, a.splits, u / a.splits * a.splits);
                 CHECK(one.s == at.s && one.h == at.h && one.tile == at.tile && one.part == 0);
@@ -269,9 +269,9 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
         }
     }
     for (int s = 0; s < n_seq; s++) {      // a sequence's columns are in one of the two launches
-        const int n = fm_seq_rows(b, s), narrow = fm_attn_tiles(n, group, 0), wides = fm_attn_tiles(n, group, 1);
+        const int n = fm_seq_rows(b, s), narrow = fm_attn_tiles(n, group, 0), wides = fm_attn_tiles(n, group, 64);
         CHECK(!narrow || !wides);
-        CHECK(narrow * FM_ATTN_COLS + wides * FM_ATTN_WIDE >= n * group);
+        CHECK(narrow * FM_ATTN_COLS + wides * 64 >= n * group);
         covered += narrow + wides;
     }
     CHECK(covered >= 0);
