@@ -541,19 +541,35 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
             fm_v4f sc[CT][2];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) sc[ct][0] = sc[ct][1] = fm_v4f{0.f, 0.f, 0.f, 0.f};
+            // operands are read a group of products ahead (the scheduler would put each read in front of its use)
+            fm_v8h xk[2][2], yq[2][CT * NP];
+            auto read_k = [&](int k) {
+                xk[k & 1][0] = s_k[(2 * half * KS + k) * 64];
+                xk[k & 1][1] = s_k[((2 * half + 1) * KS + k) * 64];
+#pragma unroll
+                for (int y = 0; y < CT * NP; y++) yq[k & 1][y] = s_q[(y * KS + k) * 64];
+            };
+            read_k(0);
 #pragma unroll
             for (int k = 0; k < KS; k++) {
-                const fm_v8h x0 = s_k[(2 * half * KS + k) * 64], x1 = s_k[((2 * half + 1) * KS + k) * 64];
+                if (k + 1 < KS) read_k(k + 1);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int ct = 0; ct < CT; ct++)
 #pragma unroll
                     for (int p = 0; p < NP; p++) {
-                        const fm_v8h y = s_q[((ct * NP + p) * KS + k) * 64];
-                        sc[ct][0] = mfma(x0, y, sc[ct][0]);
-                        sc[ct][1] = mfma(x1, y, sc[ct][1]);
+                        sc[ct][0] = mfma(xk[k & 1][0], yq[k & 1][ct * NP + p], sc[ct][0]);
+                        sc[ct][1] = mfma(xk[k & 1][1], yq[k & 1][ct * NP + p], sc[ct][1]);
                     }
+                __builtin_amdgcn_sched_barrier(0);
             }
             lds_barrier();                                        // the keys have been read, the values are there
+            fm_v8h xv[2][4];
+            auto read_v = [&](int d0) {
+#pragma unroll
+                for (int d = 0; d < 4; d++) xv[d0 >> 2 & 1][d] = s_v[((d0 + d) * 2 + half) * 64];
+            };
+            read_v(0);
             if (st + 1 < s1) put_k();
             const bool whole = __all(there) && pos + BK <= all_limit;      // nothing of the step is masked
             fm_v8h p8[CT][NP];
@@ -607,12 +623,16 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
                     }
             }
 #pragma unroll
-            for (int d = 0; d < DT; d++) {
-                const fm_v8h x = s_v[(d * 2 + half) * 64];
+            for (int d0 = 0; d0 < DT; d0 += 4) {
+                if (d0 + 4 < DT) read_v(d0 + 4);
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int ct = 0; ct < CT; ct++)
+                for (int d = 0; d < 4; d++)
 #pragma unroll
-                    for (int p = 0; p < NP; p++) o[ct][d] = mfma(x, p8[ct][p], o[ct][d]);
+                    for (int ct = 0; ct < CT; ct++)
+#pragma unroll
+                        for (int p = 0; p < NP; p++) o[ct][d0 + d] = mfma(xv[d0 >> 2 & 1][d], p8[ct][p], o[ct][d0 + d]);
+                __builtin_amdgcn_sched_barrier(0);
             }
             now = next;
             next = later;
