@@ -140,6 +140,9 @@ __device__ __forceinline__ float lane_of(float v, int lane) {
     return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane));
 }
 
+// 2^x by the instruction; results below 2^-126 are 0
+__device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
+
 // Per (chunk, key head): K K^T and Q K^T of the chunk's rows, then per value head of the key head the
 // decay factors, P, and T = (1 + A)^-1.  T in 16 x 16 blocks: the diagonal ones by forward substitution,
 // a column per lane; below them, block column by block column,
@@ -160,6 +163,10 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
     const int64_t row0 = b.row[s] + first;
     const FmGdnWs w = fm_gdn_ws(a);
     float *out = ws + (int64_t)c * w.floats;
+    const int rep = a.v_heads / a.k_heads;
+    const int64_t gate_at = (row0 + min(lane, n - 1)) * a.v_heads + hk * rep;
+    const float *gates = a.g + gate_at, *betas = a.beta + gate_at;
+    float next_gate = gates[0], next_beta = betas[0];      // a head ahead
     {
         constexpr int PER = DK / 16;         // float4 of K (and of Q) a thread
         fm_v4f x[2][PER];
@@ -233,15 +240,15 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
         for (int e = 0; e < 4; e++) z[e * LA] = prod[t][e];
     }
     const float rk = norm[0][lane], rq = norm[1][lane];
-    const int rep = a.v_heads / a.k_heads;
     for (int hh = 0; hh < rep; hh++) {
         const int h = hk * rep + hh;
-        const int64_t at = (row0 + min(lane, n - 1)) * a.v_heads + h;
-        float gate = a.g[at], beta = a.beta[at];
+        float gate = next_gate, beta = next_beta;
+        next_gate = gates[min(hh + 1, rep - 1)];
+        next_beta = betas[min(hh + 1, rep - 1)];
         if (lane >= n) gate = beta = 0.0f;
         // e^-104 is 0 in fp32: a stronger decay, -inf included, is the same factor with finite sums
         if (gate < -104.0f) gate = -104.0f;
-        double G = gate;
+        double G = (double)gate * 1.4426950408889634;     // (in powers of two from here on)
 #pragma unroll
         for (int o = 1; o < 64; o <<= 1) {
             const double up = __shfl_up(G, o);
@@ -250,21 +257,23 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
         if (wave == 0) {
             // factors of a token: of v, of (K S), of u in the state's update, of (Q S)
             float *sc = out + w.sc + (int64_t)h * 256;
-            const float eg = expf((float)G);
+            const float eg = exp2_of((float)G);
             sc[lane] = beta;
             sc[64 + lane] = beta * eg * rk;
-            sc[128 + lane] = lane < n ? expf((float)(lane_of(G, 63) - G)) * rk : 0.0f;
+            sc[128 + lane] = lane < n ? exp2_of((float)(lane_of(G, 63) - G)) * rk : 0.0f;
             sc[192 + lane] = rq * eg;
             if (lane == 63) out[w.end + h] = eg;
         }
         __syncthreads();                       // the products are there; the last head's T and P are out
         // rows 16 wave .. of A and P, a column per lane
+        // (computed for every column and dropped above the diagonal: branches would cost more)
+#pragma unroll 4
         for (int ii = 0; ii < 16; ii++) {
             const int i = 16 * wave + ii;
-            const float e = lane <= i ? expf((float)(lane_of(G, i) - G)) : 0.0f;
-            const float bi = lane_of(beta, i), ki = lane_of(rk, i), qi = lane_of(rq, i);
-            am[i * LA + lane] = lane < i ? bi * e * (kk[i * LA + lane] * (ki * rk)) : 0.0f;
-            pm[i * LA + lane] = lane <= i ? e * (qk[i * LA + lane] * (qi * rk)) : 0.0f;
+            const float x = kk[i * LA + lane], y = qk[i * LA + lane], e = exp2_of((float)(lane_of(G, i) - G));
+            const float ai = lane_of(beta, i) * e * (x * (lane_of(rk, i) * rk)), pi = e * (y * (lane_of(rq, i) * rk));
+            am[i * LA + lane] = lane < i ? ai : 0.0f;
+            pm[i * LA + lane] = lane <= i ? pi : 0.0f;
         }
         __syncthreads();
         if (wave == 3) {
@@ -273,10 +282,15 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
             float t[16];
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                float x = r == i ? 1.0f : 0.0f;
+                float x = r == i ? 1.0f : 0.0f, y = 0.0f;
 #pragma unroll
-                for (int m = 0; m < i; m++) x = fmaf(-d[i * LA + m], t[m], x);
-                t[i] = x;
+                for (int m = 0; m < i; m += 4) {
+                    const fm_v4f ai = *(const fm_v4f *)(d + i * LA + m);
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (m + e < i) (e & 1 ? y : x) = fmaf(-ai[e], t[m + e], e & 1 ? y : x);
+                }
+                t[i] = x + y;
             }
             __builtin_amdgcn_wave_barrier();   // (one wave: its LDS accesses run in order)
 #pragma unroll
