@@ -16,7 +16,7 @@
 //   u_i + beta_i sum_{j<i} E_ij (k_i.k_j) u_j = beta_i (v_i - e^G_i S k_i)    =:  (1 + A) u = R
 //   o_i = scale (e^G_i S q_i + sum_{j<=i} E_ij (q_i.k_j) u_j)
 //   S <- e^G_C S + sum_i e^(G_C - G_i) u_i k_i^T
-// Everything that does not need the state — the inverse T of 1 + A, P = scale tril(E . Q K^T), K^T and the
+// Everything that does not need the state — the inverse T of 1 + A, P = scale tril(E . Q K^T) and the
 // factors of a token — is computed for all chunks at once by fm_gdn_prep; fm_gdn_scan walks the chunks in
 // order, sixteen state rows (value dims) a workgroup, with five small products a chunk.  Both use
 // the fp32 matrix instruction v_mfma_f32_16x16x4_f32: the state is an fp32 result, which 16-bit
@@ -216,19 +216,14 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
         }
         prod[t] = (z[0] + z[1]) + (z[2] + z[3]);
     }
-    // K, Q and K^T in the order of the second kernel
+    // K and Q in the order of the second kernel
     {
-        float *k = out + w.k + (int64_t)hk * DK * 64, *q = out + w.q + (int64_t)hk * DK * 64, *kt = out + w.kt + (int64_t)hk * DK * 64;
+        float *k = out + w.k + (int64_t)hk * DK * 64, *q = out + w.q + (int64_t)hk * DK * 64;
 #pragma unroll
         for (int d = 0; d < DK / 16; d++) {
             const int at = (wave * (DK / 16) + d) * FM_GDN_TILE + 4 * lane;
             *(fm_v4f *)(k + at) = *(const fm_v4f *)(sk + (16 * wave + r) * LD + 16 * d + 4 * g);
             *(fm_v4f *)(q + at) = *(const fm_v4f *)(sq + (16 * wave + r) * LD + 16 * d + 4 * g);
-        }
-#pragma unroll
-        for (int u = 0; u < DK / 16; u++) {      // tile u * 4 + wave: k rows 16 u .., tokens 16 wave ..
-            const float *x = sk + (16 * wave + 4 * g) * LD + 16 * u + r;
-            *(fm_v4f *)(kt + (u * 4 + wave) * FM_GDN_TILE + 4 * lane) = fm_v4f{x[0], x[LD], x[2 * LD], x[3 * LD]};
         }
     }
     __syncthreads();
@@ -338,9 +333,10 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
 
 // The chunks of a sequence in order, 16 value dims of one head per workgroup: eight waves, two per
 // token tile of 16.  Of the state [k_dim][16] a wave keeps a tile of 16 k in registers (k_dim 64: the
-// second four keep none).  S, R and u pass through LDS as [column][k or token], so that both the
-// writers (four consecutive rows of a result) and the readers (four consecutive k of an operand) move
-// 16 bytes.  A chunk is three phases between barriers,
+// second four keep none).  S, R and u pass through LDS as [column][k or token], so that both the writers
+// (four consecutive rows of a result) and the readers (four consecutive k of an operand) move 16
+// bytes; K as [token][k], of which K^T u reads columns.  A chunk is three phases
+// between barriers,
 //   1  waves 0-3: R = beta V - f K S                waves 4-7: half of Q S
 //   2  waves 0-3: u = T R                                      the other half
 //   3  waves 0-3: S += K^T u, k 0-63                waves 4-7: S += K^T u, k 64-127; P u, the output
@@ -353,7 +349,7 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
 template <int DK, bool BF16>
 __global__ __launch_bounds__(512, 2) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, const float *ws) {
     constexpr int LS = DK + 4, LU = 68, ND = DK / 16;
-    __shared__ __attribute__((aligned(16))) float ss[16 * LS], sr[16 * LU], su[16 * LU], sw[16 * LU], none[4];
+    __shared__ __attribute__((aligned(16))) float ss[16 * LS], sr[16 * LU], su[16 * LU], sw[16 * LU], sk[64 * LS], none[4];
     const int wv = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), wave = wv & 3, lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const bool second = wv >= 4;
     const int h = blockIdx.x % a.v_heads, v0 = 16 * (blockIdx.x / a.v_heads), s = blockIdx.y;
@@ -383,12 +379,10 @@ __global__ __launch_bounds__(512, 2) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, cons
     const unsigned lane4 = 4 * lane;
     const int64_t row_at = (second ? w.q : w.k) + ((int64_t)hk * DK * 64 + wave * ND * FM_GDN_TILE);
     const int64_t low_at = (second ? w.p : w.tm) + (int64_t)h * 10 * FM_GDN_TILE + fm_gdn_lower(wave, 0);
-    const int64_t kt_at = w.kt + (int64_t)hk * DK * 64 + (keeps ? wv : 0) * 4 * FM_GDN_TILE;
     const unsigned sc_lane = 16 * wave + 4 * g;
     auto ld = [&](int64_t at) { return *(const fm_v4f *)(in + at + lane4); };
-    fm_v4f rows[ND], low[4], kt[4], beta = zero, f0 = zero, f1 = zero;   // K or Q, T or P, K^T, factors
+    fm_v4f rows[ND], low[4], beta = zero, f0 = zero, f1 = zero;      // K or Q, T or P, factors
     float v[4] = {0.f, 0.f, 0.f, 0.f}, decay;
-    auto load_kt = [&](int j) { kt[j] = ld(kt_at + j * FM_GDN_TILE); };
     auto load_low = [&](int j) { low[j] = ld(low_at + min(j, wave) * FM_GDN_TILE); };
     auto load_rows = [&](int d) { rows[d] = ld(row_at + d * FM_GDN_TILE); };
     auto load_v = [&]() {
@@ -429,9 +423,9 @@ __global__ __launch_bounds__(512, 2) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, cons
 #pragma unroll
         for (int j = 0; j < 4; j++) {
             const fm_v4f y = *(const fm_v4f *)(sw + r * LU + 16 * j + 4 * g);
+            const float *x = sk + (16 * j + 4 * g) * LS + 16 * wv + r;
 #pragma unroll
-            for (int e = 0; e < 4; e++) z[e] = mfma4(kt[j][e], y[e], z[e]);
-            load_kt(j);
+            for (int e = 0; e < 4; e++) z[e] = mfma4(x[e * LS], y[e], z[e]);
         }
         st = (z[0] + z[1]) + (z[2] + z[3]);
         *(fm_v4f *)(ss + r * LS + k_at) = st;
@@ -442,7 +436,7 @@ __global__ __launch_bounds__(512, 2) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, cons
     load_f1();
     load_decay();
 #pragma unroll
-    for (int j = 0; j < 4; j++) load_low(j), load_kt(j);
+    for (int j = 0; j < 4; j++) load_low(j);
     if (!second) load_v();
     // (the first chunk's operands arrive before the loop: its waits then go by the loop's own order of loads)
     __builtin_amdgcn_s_waitcnt(0x0F70);                    // vmcnt(0)
@@ -451,7 +445,9 @@ __global__ __launch_bounds__(512, 2) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, cons
             const int n = n_in;
             at_chunk(min(c + 1, chunks - 1));
             fm_v4f x[4] = {zero, zero, zero, zero};
-            lds_barrier();                                 // S is there
+            lds_barrier();                                 // S is there, the last chunk's K has been read
+#pragma unroll
+            for (int d = 0; d < ND; d++) *(fm_v4f *)(sk + (16 * wave + r) * LS + 16 * d + 4 * g) = rows[d];
             times_s(0, ND, x);
             const fm_v4f ks = (x[0] + x[1]) + (x[2] + x[3]);
             fm_v4f rr;

@@ -60,12 +60,12 @@ FM_HD int fm_gdn_seq_of(const FmGdnSeqs &b, int c) {
 #define FM_GDN_CHUNK 64
 // Sequences of fewer rows run token by token.
 #define FM_GDN_MIN_CHUNKED 24
-// What the chunked form keeps per chunk between its two kernels, in floats: K, Q and K^T of a key head,
+// What the chunked form keeps per chunk between its two kernels, in floats: K and Q of a key head,
 // the lower tiles of T and P of a value head, each in the order the second kernel's lanes take them — tiles of 16
 // x 16 in 64 groups of four floats, lane 16 g + r has columns 4 g .. 4 g + 3 of row r — then four
 // factors per token (sc) and one per chunk (end) of a value head.
 struct FmGdnWs {
-    int64_t k, q, kt, tm, p, sc, end, floats;
+    int64_t k, q, tm, p, sc, end, floats;
 };
 #define FM_GDN_TILE 256     // floats
 // tile (i, j <= i) of the lower tiles of a 64 x 64 matrix
@@ -75,8 +75,7 @@ FM_HD FmGdnWs fm_gdn_ws(const FmGdn &a) {
     const int64_t rows = (int64_t)a.k_heads * a.k_dim * 64, low = (int64_t)a.v_heads * 10 * FM_GDN_TILE;
     w.k = 0;
     w.q = rows;
-    w.kt = 2 * rows;
-    w.tm = 3 * rows;
+    w.tm = 2 * rows;
     w.p = w.tm + low;
     w.sc = w.p + low;
     w.end = w.sc + (int64_t)a.v_heads * 256;
@@ -116,10 +115,15 @@ struct FmGdnPlan {
         *chunked = 1;
         for (;;) {
             // a group: up to FM_GDN_SEQS long sequences, run window by window
-            int n_long = 0, end = group0;
-            for (; end < n_seq && n_long < FM_GDN_SEQS; end++) n_long += rows(end) >= FM_GDN_MIN_CHUNKED;
+            int n_long = 0, most = 0, end = group0;
+            for (; end < n_seq && n_long < FM_GDN_SEQS; end++) {
+                n_long += rows(end) >= FM_GDN_MIN_CHUNKED;
+                most = rows(end) > most ? rows(end) : most;
+            }
             if (!n_long) return false;
-            const int win = fm_gdn_window(*a, n_long) * FM_GDN_CHUNK;
+            // windows of one size rather than a short last one
+            const int chunks = (most + FM_GDN_CHUNK - 1) / FM_GDN_CHUNK, full = fm_gdn_window(*a, n_long);
+            const int passes = (chunks + full - 1) / full, win = (chunks + passes - 1) / passes * FM_GDN_CHUNK;
             b->n = 0;
             for (int i = group0; i < end; i++) {
                 const int left = rows(i) - done;
