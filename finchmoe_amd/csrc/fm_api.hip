@@ -60,7 +60,7 @@ int fm_launch_layer_tail(const FmTailArgs *a, int bits, int scale_fp16, hipStrea
 int fm_launch_route(const float *d_logits, int n, int K, const float *d_seg_score, int32_t *d_idx,
                     float *d_w, float *d_params, hipStream_t st);
 int fm_launch_gdn(const FmGdn *a, int bf16, const int *start, int n_seq, const float *const *in,
-                  float *const *out, void *ws, hipStream_t st);
+                  float *const *out, void *ws, int n_cu, hipStream_t st);
 int fm_launch_attn(const FmKv *c, const FmAttn *args, const FmSeqs *b, int D, int bf16, void *ws, int n_cu, hipStream_t st);
 int fm_launch_kv(const FmKv *c, const FmKvRows *x, const FmSeqs *b, int D, int bf16, int read, hipStream_t st);
 size_t fm_logprob_ws(int rows, int vocab, int top_n);
@@ -1677,7 +1677,7 @@ extern "C" int fm_gated_delta_dev(fm_ctx *c, const fm_gated_delta_args *p) {
     const size_t ws = fm_gdn_ws_bytes(&a, p->seq_start, p->n_seq);
     if (ws && (rc = ensure_ws(c, ws))) return rc;
     rc = fm_launch_gdn(&a, p->dtype == FM_DTYPE_BF16, p->seq_start, p->n_seq, p->d_state_in, p->d_state_out, c->d_ws,
-                       c->stream);
+                       c->n_cu, c->stream);
     if (rc) return fail(c, rc, "gated delta launch failed: %s", hipGetErrorString(hipGetLastError()));
     return FM_OK;
 }

@@ -32,7 +32,7 @@ struct RowPart {   // a lane's part of a k_dim vector: elements 4 li .. and, of 
     fm_v4f p[N];
     __device__ __forceinline__ void load(const float *row, int li) {
 #pragma unroll
-        for (int n = 0; n < N; n++) p[n] = *(const fm_v4f *)(row + 64 * n + 4 * li);
+        for (int n = 0; n < N; n++) p[n] = __builtin_nontemporal_load((const fm_v4f *)(row + 64 * n + 4 * li));
     }
     template <bool BF16>
     __device__ __forceinline__ void load_any(const void *base, int64_t at, int li) {
@@ -118,7 +118,7 @@ __global__ __launch_bounds__(256) void fm_gdn_steps(FmGdn a, FmGdnSeqs b) {
         if (v0 + 4 * r < a.v_dim)
 #pragma unroll
             for (int n = 0; n < RowPart<DK>::N; n++)
-                *(fm_v4f *)(out + head + (int64_t)(v0 + 4 * r) * DK + 64 * n + 4 * li) = st[r].p[n];
+                __builtin_nontemporal_store(st[r].p[n], (fm_v4f *)(out + head + (int64_t)(v0 + 4 * r) * DK + 64 * n + 4 * li));
 }
 
 __device__ __forceinline__ fm_v4f mfma4(float x, float y, fm_v4f c) {
@@ -143,6 +143,8 @@ __device__ __forceinline__ float lane_of(float v, int lane) {
 // 2^x by the instruction; results below 2^-126 are 0
 __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// (Where the chunks and key heads are fewer than the CUs hold, gridDim.z workgroups share a key head's value
+// heads, each with the products of its own: 77 tokens 17 us with one, 12 with two.)
 // Per (chunk, key head): K K^T and Q K^T of the chunk's rows, then per value head of the key head the
 // decay factors, P, and T = (1 + A)^-1.  T in 16 x 16 blocks: the diagonal ones by forward substitution,
 // a column per lane; below them, block column by block column,
@@ -163,10 +165,10 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
     const int64_t row0 = b.row[s] + first;
     const FmGdnWs w = fm_gdn_ws(a);
     float *out = ws + (int64_t)c * w.floats;
-    const int rep = a.v_heads / a.k_heads;
+    const int rep = a.v_heads / a.k_heads, step = gridDim.z;
     const int64_t gate_at = (row0 + min(lane, n - 1)) * a.v_heads + hk * rep;
     const float *gates = a.g + gate_at, *betas = a.beta + gate_at;
-    float next_gate = gates[0], next_beta = betas[0];      // a head ahead
+    float next_gate = gates[blockIdx.z], next_beta = betas[blockIdx.z];      // a head ahead
     {
         constexpr int PER = DK / 16;         // float4 of K (and of Q) a thread
         fm_v4f x[2][PER];
@@ -217,7 +219,7 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
         prod[t] = (z[0] + z[1]) + (z[2] + z[3]);
     }
     // K and Q in the order of the second kernel
-    {
+    if (blockIdx.z == 0) {
         float *k = out + w.k + (int64_t)hk * DK * 64, *q = out + w.q + (int64_t)hk * DK * 64;
 #pragma unroll
         for (int d = 0; d < DK / 16; d++) {
@@ -235,11 +237,11 @@ __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *
         for (int e = 0; e < 4; e++) z[e * LA] = prod[t][e];
     }
     const float rk = norm[0][lane], rq = norm[1][lane];
-    for (int hh = 0; hh < rep; hh++) {
+    for (int hh = blockIdx.z; hh < rep; hh += step) {
         const int h = hk * rep + hh;
         float gate = next_gate, beta = next_beta;
-        next_gate = gates[min(hh + 1, rep - 1)];
-        next_beta = betas[min(hh + 1, rep - 1)];
+        next_gate = gates[min(hh + step, rep - 1)];
+        next_beta = betas[min(hh + step, rep - 1)];
         if (lane >= n) gate = beta = 0.0f;
         // e^-104 is 0 in fp32: a stronger decay, -inf included, is the same factor with finite sums
         if (gate < -104.0f) gate = -104.0f;
@@ -486,11 +488,13 @@ __global__ __launch_bounds__(512, 2) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, cons
 }
 
 template <int DK, bool BF16>
-int launch_seqs(const FmGdn &a, const FmGdnSeqs &b, int chunked, float *ws, hipStream_t st) {
+int launch_seqs(const FmGdn &a, const FmGdnSeqs &b, int chunked, float *ws, int n_cu, hipStream_t st) {
     if (!chunked) {
         hipLaunchKernelGGL((fm_gdn_steps<DK, BF16, 1>), dim3(a.v_dim / 16, a.v_heads, b.n), dim3(256), 0, st, a, b);
     } else {
-        hipLaunchKernelGGL((fm_gdn_prep<DK, BF16>), dim3(b.chunk0[b.n], a.k_heads), dim3(256), 0, st, a, b, ws);
+        const int rep = a.v_heads / a.k_heads, share = 2 * n_cu / (b.chunk0[b.n] * a.k_heads);
+        const int z = share < 1 ? 1 : share < rep ? share : rep;
+        hipLaunchKernelGGL((fm_gdn_prep<DK, BF16>), dim3(b.chunk0[b.n], a.k_heads, z), dim3(256), 0, st, a, b, ws);
         hipLaunchKernelGGL((fm_gdn_scan<DK, BF16>), dim3(a.v_heads * (a.v_dim / 16), b.n), dim3(512), 0, st, a, b, ws);
     }
     return hipGetLastError() == hipSuccess ? FM_OK : FM_ERR_HIP;
@@ -500,14 +504,14 @@ int launch_seqs(const FmGdn &a, const FmGdnSeqs &b, int chunked, float *ws, hipS
 
 // start: n_seq + 1 row numbers (null: one row per sequence); in, out: n_seq state pointers
 extern "C" int fm_launch_gdn(const FmGdn *a, int bf16, const int *start, int n_seq, const float *const *in,
-                             float *const *out, void *ws, hipStream_t st) {
+                             float *const *out, void *ws, int n_cu, hipStream_t st) {
     FmGdnPlan plan{a, start, n_seq, in, out};
     FmGdnSeqs b;
     int chunked;
     while (plan.next(&b, &chunked)) {
         int rc;
-        if (a->k_dim == 128) rc = bf16 ? launch_seqs<128, true>(*a, b, chunked, (float *)ws, st) : launch_seqs<128, false>(*a, b, chunked, (float *)ws, st);
-        else rc = bf16 ? launch_seqs<64, true>(*a, b, chunked, (float *)ws, st) : launch_seqs<64, false>(*a, b, chunked, (float *)ws, st);
+        if (a->k_dim == 128) rc = bf16 ? launch_seqs<128, true>(*a, b, chunked, (float *)ws, n_cu, st) : launch_seqs<128, false>(*a, b, chunked, (float *)ws, n_cu, st);
+        else rc = bf16 ? launch_seqs<64, true>(*a, b, chunked, (float *)ws, n_cu, st) : launch_seqs<64, false>(*a, b, chunked, (float *)ws, n_cu, st);
         if (rc) return rc;
     }
     return FM_OK;
