@@ -30,9 +30,24 @@ template <int DK>
 struct RowPart {   // a lane's part of a k_dim vector: elements 4 li .. and, of 128, 64 + 4 li ..
     static constexpr int N = DK / 64;
     fm_v4f p[N];
+    // (the state is read once and written once: it is not kept in the caches)
     __device__ __forceinline__ void load(const float *row, int li) {
 #pragma unroll
         for (int n = 0; n < N; n++) p[n] = __builtin_nontemporal_load((const fm_v4f *)(row + 64 * n + 4 * li));
+    }
+    __device__ __forceinline__ void store(float *row, int li) const {
+#pragma unroll
+        for (int n = 0; n < N; n++) __builtin_nontemporal_store(p[n], (fm_v4f *)(row + 64 * n + 4 * li));
+    }
+    __device__ __forceinline__ void clear() {
+#pragma unroll
+        for (int n = 0; n < N; n++) p[n] = fm_v4f{0.f, 0.f, 0.f, 0.f};
+    }
+    __device__ __forceinline__ void update(float decay, float u, const RowPart &k) {
+#pragma unroll
+        for (int n = 0; n < N; n++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) p[n][i] = fmaf(u, k.p[n][i], decay * p[n][i]);
     }
     template <bool BF16>
     __device__ __forceinline__ void load_any(const void *base, int64_t at, int li) {
@@ -49,76 +64,42 @@ struct RowPart {   // a lane's part of a k_dim vector: elements 4 li .. and, of 
     }
 };
 
-template <int DK, bool BF16, int R>
+template <int DK, bool BF16>
 __global__ __launch_bounds__(256) void fm_gdn_steps(FmGdn a, FmGdnSeqs b) {
     const int wave = threadIdx.x >> 6, lane = threadIdx.x & 63, li = lane & 15;
     const int s = blockIdx.z, h = blockIdx.y, hk = h / (a.v_heads / a.k_heads);
-    const int v0 = (blockIdx.x * 4 + wave) * 4 * R + (lane >> 4);   // rows v0, v0 + 4, ...
+    const int v0 = 16 * blockIdx.x + 4 * wave + (lane >> 4);         // the lane group's row of the state
     const int t0 = b.row[s], T = b.rows[s];
-    const int64_t head = (int64_t)h * a.v_dim * DK;
-    const float *in = b.in[s];
-    RowPart<DK> st[R];
-#pragma unroll
-    for (int r = 0; r < R; r++) {
-        if (in && v0 + 4 * r < a.v_dim) st[r].load(in + head + (int64_t)(v0 + 4 * r) * DK, li);
-        else
-#pragma unroll
-            for (int n = 0; n < RowPart<DK>::N; n++) st[r].p[n] = fm_v4f{0.f, 0.f, 0.f, 0.f};
-    }
+    const int64_t state_at = ((int64_t)h * a.v_dim + v0) * DK;
+    RowPart<DK> st;
+    if (b.in[s]) st.load(b.in[s] + state_at, li);
+    else st.clear();
     RowPart<DK> k, q, nk, nq;
-    float vv[R], nv[R], g = 0.f, beta = 0.f, ng = 0.f, nbeta = 0.f;
-    auto fetch = [&](int t, RowPart<DK> &kk, RowPart<DK> &qq, float *v, float &gg, float &bb) {
+    float v = 0.f, nv = 0.f, g = 0.f, beta = 0.f, ng = 0.f, nbeta = 0.f;
+    auto fetch = [&](int t, RowPart<DK> &kk, RowPart<DK> &qq, float &vv, float &gg, float &bb) {
         const int64_t row = t0 + t;
         kk.template load_any<BF16>(a.k, row * a.k_stride + (int64_t)hk * DK, li);
         qq.template load_any<BF16>(a.q, row * a.q_stride + (int64_t)hk * DK, li);
-#pragma unroll
-        for (int r = 0; r < R; r++)
-            v[r] = v0 + 4 * r < a.v_dim ? fm_ld1<BF16>(a.v, row * a.v_stride + (int64_t)h * a.v_dim + v0 + 4 * r) : 0.0f;
+        vv = fm_ld1<BF16>(a.v, row * a.v_stride + (int64_t)h * a.v_dim + v0);
         gg = a.g[row * a.v_heads + h];
         bb = a.beta[row * a.v_heads + h];
     };
-    if (T > 0) fetch(0, k, q, vv, g, beta);
+    if (T > 0) fetch(0, k, q, v, g, beta);
     for (int t = 0; t < T; t++) {
         if (t + 1 < T) fetch(t + 1, nk, nq, nv, ng, nbeta);
-        float kq = k.dot(q), kk = 1.0f, qq = 1.0f;
-        float sk[R], sq[R];
-#pragma unroll
-        for (int r = 0; r < R; r++) sk[r] = st[r].dot(k), sq[r] = st[r].dot(q);
-        kq = fm_group_sum<16>(kq);
+        float kq = fm_group_sum<16>(k.dot(q)), sk = fm_group_sum<16>(st.dot(k)), sq = fm_group_sum<16>(st.dot(q));
         float kn = 1.0f, qn = a.scale;
         if (a.l2norm) {
-            kk = fm_group_sum<16>(k.dot(k));
-            qq = fm_group_sum<16>(q.dot(q));
-            kn = 1.0f / sqrtf(kk + 1e-6f);
-            qn = a.scale / sqrtf(qq + 1e-6f);
+            kn = 1.0f / sqrtf(fm_group_sum<16>(k.dot(k)) + 1e-6f);
+            qn = a.scale / sqrtf(fm_group_sum<16>(q.dot(q)) + 1e-6f);
         }
-        const float decay = expf(g);
-        kq *= kn * qn;
-#pragma unroll
-        for (int r = 0; r < R; r++) {
-            sk[r] = fm_group_sum<16>(sk[r]) * kn;
-            sq[r] = fm_group_sum<16>(sq[r]) * qn;
-            const float u = beta * (vv[r] - decay * sk[r]);
-            const float o = fmaf(u, kq, decay * sq[r]);
-            const float uk = u * kn;
-#pragma unroll
-            for (int n = 0; n < RowPart<DK>::N; n++)
-#pragma unroll
-                for (int i = 0; i < 4; i++) st[r].p[n][i] = fmaf(uk, k.p[n][i], decay * st[r].p[n][i]);
-            if (li == 0 && v0 + 4 * r < a.v_dim)
-                fm_st1<BF16>(a.out, ((int64_t)(t0 + t) * a.v_heads + h) * a.v_dim + v0 + 4 * r, o);
-        }
-        k = nk, q = nq, g = ng, beta = nbeta;
-#pragma unroll
-        for (int r = 0; r < R; r++) vv[r] = nv[r];
+        const float decay = expf(g), u = beta * (v - decay * (sk * kn));
+        const float o = fmaf(u, kq * (kn * qn), decay * (sq * qn));
+        st.update(decay, u * kn, k);
+        if (li == 0) fm_st1<BF16>(a.out, ((int64_t)(t0 + t) * a.v_heads + h) * a.v_dim + v0, o);
+        k = nk, q = nq, v = nv, g = ng, beta = nbeta;
     }
-    float *out = b.out[s];
-#pragma unroll
-    for (int r = 0; r < R; r++)
-        if (v0 + 4 * r < a.v_dim)
-#pragma unroll
-            for (int n = 0; n < RowPart<DK>::N; n++)
-                __builtin_nontemporal_store(st[r].p[n], (fm_v4f *)(out + head + (int64_t)(v0 + 4 * r) * DK + 64 * n + 4 * li));
+    st.store(b.out[s] + state_at, li);
 }
 
 __device__ __forceinline__ fm_v4f mfma4(float x, float y, fm_v4f c) {
@@ -490,7 +471,7 @@ __global__ __launch_bounds__(512, 2) void fm_gdn_scan(FmGdn a, FmGdnSeqs b, cons
 template <int DK, bool BF16>
 int launch_seqs(const FmGdn &a, const FmGdnSeqs &b, int chunked, float *ws, int n_cu, hipStream_t st) {
     if (!chunked) {
-        hipLaunchKernelGGL((fm_gdn_steps<DK, BF16, 1>), dim3(a.v_dim / 16, a.v_heads, b.n), dim3(256), 0, st, a, b);
+        hipLaunchKernelGGL((fm_gdn_steps<DK, BF16>), dim3(a.v_dim / 16, a.v_heads, b.n), dim3(256), 0, st, a, b);
     } else {
         const int rep = a.v_heads / a.k_heads, share = 2 * n_cu / (b.chunk0[b.n] * a.k_heads);
         const int z = share < 1 ? 1 : share < rep ? share : rep;
