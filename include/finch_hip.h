@@ -390,15 +390,16 @@ enum { FM_DTYPE_F32 = 0, FM_DTYPE_BF16 = 1 };
  *   S = exp(g) * S;  u = beta * (v - S k);  S = S + u k^T;  out = scale * S q
  * FM_GDN_L2NORM: q and k are divided by sqrt(sum of squares + 1e-6) first.
  *   d_q, d_k [rows][k_heads][k_dim], d_v [rows][v_heads][v_dim], d_out [rows][v_heads][v_dim]
- *   contiguous, d_g (logarithm of the decay, -inf wipes the state) and d_beta
+ *   contiguous, d_g (logarithm of the decay, 0 or less; -inf wipes the state) and d_beta
  *   [rows][v_heads] fp32 contiguous.
  *   d_state_in, d_state_out: HOST arrays of n_seq device pointers, each a state
  *   [v_heads][v_dim][k_dim] fp32, 16-byte aligned.  d_state_in or an entry of it NULL: zeros.  An output may be
  *   its own sequence's input (update in place); any other overlap, also of two outputs, is
  *   FM_ERR_ARG.  An empty sequence's state is copied.
  * k_dim 64 or 128, v_dim a multiple of 16 up to 256, v_heads a multiple of k_heads (up to 256).
- * Short sequences run token by token, long ones in chunks of 64 tokens on the matrix cores; the
- * two agree to fp32 rounding. */
+ * Sequences of fewer than 24 rows run token by token, longer ones in chunks of 64 tokens on the matrix
+ * cores; the two agree to fp32 rounding.  A NaN reaches the rest of its head's sequence, in chunks
+ * also the earlier tokens of its chunk, and no other head or sequence. */
 enum { FM_GDN_L2NORM = 1 };
 typedef struct {
     int32_t n_seq, k_heads, v_heads, k_dim, v_dim, dtype, flags;

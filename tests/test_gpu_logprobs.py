@@ -147,3 +147,23 @@ def test_refusals(hip):
         with pytest.raises(fb.FinchError) as e:
             hip.logprobs_dev(*args)
         assert e.value.status == fb.ERR_ARG
+
+
+@pytest.mark.parametrize("stride", [5000, 5001])
+def test_enough_rows_for_large_segments(hip, stride):
+    """the form with more elements a thread, aligned rows and not, among them rows whose equal values are more
+    than a segment collects"""
+    import torch
+    g = torch.Generator().manual_seed(stride)
+    x = 2 * torch.randn(600, stride, generator=g)
+    x[3] = 1.5
+    x[4, :2500] = 7.0
+    x[5] = -float("inf")
+    x[6, 4999] = 60.0
+    x[7] = torch.randint(0, 2, (stride,), generator=g).float()
+    _check(hip, x, torch.arange(600) % 5000, 32, vocab=5000)
+    bad = x[:600].clone()
+    bad[9, 4000] = float("nan")
+    lp, en, ids, top = _call(hip, bad, torch.zeros(600, dtype=torch.int64), 2, vocab=5000)
+    assert math.isnan(lp[9]) and math.isnan(en[9]) and ids[9].tolist() == [-1, -1]
+    assert bool(torch.isfinite(en[10:]).all())
