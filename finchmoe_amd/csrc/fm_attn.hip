@@ -289,7 +289,7 @@ __device__ __forceinline__ void add_steps(const FmKv &c, const FmAttn &a, const 
     if (t < b.n_seq) {
         const int len = c.len[t];
         sh.len[t] = len;
-        n = c.kv_heads * fm_attn_head_steps(fm_seq_rows(b, t), a.group, a.wide, len, a.max_len);
+        n = c.kv_heads * fm_attn_head_steps(fm_seq_rows(b, t), a.group, a.wide, a.narrow_most, len, a.max_len);
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -712,7 +712,7 @@ template <int D, bool BF16>
 __global__ __launch_bounds__(256) void fm_attn_join(FmKv c, FmAttn a, FmSeqs b) {
     const int s = blockIdx.z, h = blockIdx.y, tile = blockIdx.x >> 2;
     const int n = fm_seq_rows(b, s);
-    if (tile >= fm_attn_tiles(n, a.group, 0)) return;
+    if (tile >= fm_attn_tiles(n, a.group, 0, a.narrow_most)) return;
     const int len = c.len[s], from = a.first[s], per_head = (a.first[s + 1] - from) / c.kv_heads;
     const int share = fm_attn_share(a.first[b.n_seq], a.groups), steps = fm_attn_steps(n, a.group, 0, len, a.max_len, tile);
     int at = from + h * per_head;
@@ -868,7 +868,7 @@ void launch_attn(const FmKv &c, const FmAttn &a, const FmSeqs &b, hipStream_t st
     const dim3 grid(a.groups), block(256);
     if (a.wide) {
         FmWide w;
-        fm_attn_wide_tiles(b, a.group, a.wide, &w);
+        fm_attn_wide_tiles(b, a.group, a.wide, a.narrow_most, &w);
         hipLaunchKernelGGL((fm_attn_wide<D, BF16>), grid, dim3(512), 0, st, c, a, b, w);
         if (a.splits > 1)
             hipLaunchKernelGGL((fm_attn_wide_join<D, BF16>), dim3(w.first[b.n_seq] * c.kv_heads * (a.wide / 4)), block, 0, st, c, a, b, w);
@@ -889,7 +889,7 @@ extern "C" int fm_launch_attn(const FmKv *c, const FmAttn *args, const FmSeqs *b
         fm_attn_plan(c, &a, b, D, n_cu, wide);
         if (!a.n_tiles) continue;
         FmWide w;
-        fm_attn_wide_tiles(*b, a.group, wide, &w);
+        fm_attn_wide_tiles(*b, a.group, wide, a.narrow_most, &w);
         const size_t cols = wide ? (size_t)w.first[b->n_seq] * c->kv_heads * a.splits * wide : (size_t)2 * a.groups * COLS;
         a.part_o = (float *)ws;      // (parts | maximum and sum of each | steps before each sequence)
         a.part_ml = a.part_o + cols * D;

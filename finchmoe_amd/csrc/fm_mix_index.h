@@ -180,6 +180,7 @@ struct FmAttn {
     float scale_log2;       // scale * log2(e)
     int max_len;            // keys from here on are not seen, at most max_pages * page_tokens
     int wide;               // columns of a wide tile; 0: the launch of the sequences that have narrow ones
+    int narrow_most;        // columns of a sequence up to which its tiles are narrow
     int n_tiles;            // column tiles of the launch's sequence with the most rows
     int groups;             // workgroups that share the steps
     float *part_o, *part_ml;
@@ -191,16 +192,21 @@ struct FmAttn {
 #define FM_ATTN_COLS 16     // columns of a narrow tile: its waves take different keys
 // columns of a wide one, whose queries lie in LDS: fp32 ones as two pieces
 FM_HDC int fm_attn_wide_cols(int bf16) { return bf16 ? 128 : 64; }
-// A sequence with more columns than this has wide tiles.
-#define FM_ATTN_NARROW_MOST 64
+// Which sequences have wide tiles: those of more than 48 columns, in a batch of 1024 columns over all its
+// sequences and cache heads.  Narrow tiles read the keys once per 16 columns but spread over the whole
+// chip; measured (narrow / wide, us; 2 cache heads of 256): one sequence over 4000 keys 256 columns
+// 33 / 33 (fp32) and 31 / 37 (bf16), 512 columns 43 / 33 and 41 / 38, 1024 columns 67 / 39 and 64 / 39;
+// 16 sequences over 3000 keys 32 columns 36 / 32 and 34 / 38, 64 columns 49 / 35 and 46 / 39.
+#define FM_ATTN_NARROW_MOST 48
+#define FM_ATTN_WIDE_LEAST 1024
 
 // ---- attention's steps and who takes them --------------------------------------------------
 // A sequence of n rows has n * group columns per cache head (row * group + query head of the group) in
 // tiles of 16 or (wide) 64 or 128; a tile's steps are those of 64 keys up to the last one its last column sees, at least
 // one (somebody has to write the zeros of a row that sees nothing).
 FM_HD int fm_attn_cols(int wide) { return wide ? wide : FM_ATTN_COLS; }
-FM_HD int fm_attn_tiles(int n, int group, int wide) {
-    if ((n * group > FM_ATTN_NARROW_MOST) != (wide != 0)) return 0;
+FM_HD int fm_attn_tiles(int n, int group, int wide, int narrow_most) {
+    if ((n * group > narrow_most) != (wide != 0)) return 0;
     return (n * group + fm_attn_cols(wide) - 1) / fm_attn_cols(wide);
 }
 FM_HD int fm_attn_end(int n, int group, int wide, int len, int max_len, int tile) {
@@ -214,9 +220,9 @@ FM_HD int fm_attn_steps(int n, int group, int wide, int len, int max_len, int ti
     return end <= FM_ATTN_KEYS ? 1 : (end + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS;
 }
 // all tiles of one cache head
-FM_HD int fm_attn_head_steps(int n, int group, int wide, int len, int max_len) {
+FM_HD int fm_attn_head_steps(int n, int group, int wide, int narrow_most, int len, int max_len) {
     int sum = 0;
-    for (int t = 0; t < fm_attn_tiles(n, group, wide); t++) sum += fm_attn_steps(n, group, wide, len, max_len, t);
+    for (int t = 0; t < fm_attn_tiles(n, group, wide, narrow_most); t++) sum += fm_attn_steps(n, group, wide, len, max_len, t);
     return sum;
 }
 // Steps are numbered sequence by sequence, head by head, tile by tile; workgroup g takes those from
@@ -425,9 +431,9 @@ inline int fm_all_rows(const FmSeqs &b) { return b.one_row ? b.n_seq : b.start[b
 struct FmWide {
     int first[FM_MAX_SEQ + 1];      // tiles of one head in the sequences before
 };
-inline void fm_attn_wide_tiles(const FmSeqs &b, int group, int wide, FmWide *w) {
+inline void fm_attn_wide_tiles(const FmSeqs &b, int group, int wide, int narrow_most, FmWide *w) {
     w->first[0] = 0;
-    for (int s = 0; s < b.n_seq; s++) w->first[s + 1] = w->first[s] + fm_attn_tiles(fm_seq_rows(b, s), group, wide);
+    for (int s = 0; s < b.n_seq; s++) w->first[s + 1] = w->first[s] + fm_attn_tiles(fm_seq_rows(b, s), group, wide, narrow_most);
 }
 struct FmWideUnit {
     int s, h, tile, part;
@@ -475,18 +481,19 @@ inline size_t fm_attn_plan(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int
     const int64_t have = (int64_t)c->max_pages * c->page_tokens;
     if (a->max_len > have) a->max_len = (int)have;
     a->wide = wide;
+    a->narrow_most = (int64_t)fm_all_rows(*b) * a->group * c->kv_heads >= FM_ATTN_WIDE_LEAST ? FM_ATTN_NARROW_MOST : 0x7FFFFFFF;
     a->n_tiles = 0;
     a->splits = 1;
     int64_t most = 0;
     for (int s = 0; s < b->n_seq; s++) {
-        const int tiles = fm_attn_tiles(fm_seq_rows(*b, s), a->group, wide);
+        const int tiles = fm_attn_tiles(fm_seq_rows(*b, s), a->group, wide, a->narrow_most);
         if (tiles > a->n_tiles) a->n_tiles = tiles;
         most += (int64_t)c->kv_heads * tiles * ((a->max_len + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS + 1);
     }
     if (!a->n_tiles) return 0;
     if (wide) {
         FmWide w;
-        fm_attn_wide_tiles(*b, a->group, wide, &w);
+        fm_attn_wide_tiles(*b, a->group, wide, a->narrow_most, &w);
         const int64_t tiles = (int64_t)w.first[b->n_seq] * c->kv_heads;
         a->splits = fm_attn_splits(tiles, n_cu, (a->max_len + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS);
         a->groups = (int)(tiles * a->splits < n_cu ? tiles * a->splits : n_cu);

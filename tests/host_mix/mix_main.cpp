@@ -188,7 +188,7 @@ static void refuse_logprobs() {
 static void share_out(const FmKv &c, const FmAttn &a, const FmSeqs &b, int D, size_t ws) {
     std::vector<int> first(b.n_seq + 1, 0);
     for (int s = 0; s < b.n_seq; s++)
-        first[s + 1] = first[s] + c.kv_heads * fm_attn_head_steps(fm_seq_rows(b, s), a.group, a.wide, c.len[s], a.max_len);
+        first[s + 1] = first[s] + c.kv_heads * fm_attn_head_steps(fm_seq_rows(b, s), a.group, a.wide, a.narrow_most, c.len[s], a.max_len);
     const int total = first[b.n_seq], share = fm_attn_share(total, a.groups);
     CHECK((int64_t)share * a.groups >= total);
     CHECK(ws == (size_t)2 * a.groups * fm_attn_cols(a.wide) * (D + 2) * 4 + (FM_MAX_SEQ + 1) * 4);
@@ -197,7 +197,7 @@ static void share_out(const FmKv &c, const FmAttn &a, const FmSeqs &b, int D, si
     for (int s = 0; s < b.n_seq; s++) {
         const int n = fm_seq_rows(b, s);
         for (int h = 0; h < c.kv_heads; h++)
-            for (int t = 0; t < fm_attn_tiles(n, a.group, a.wide); t++) {
+            for (int t = 0; t < fm_attn_tiles(n, a.group, a.wide, a.narrow_most); t++) {
                 const int steps = fm_attn_steps(n, a.group, a.wide, c.len[s], a.max_len, t), at = seen;
                 const int end = fm_attn_end(n, a.group, a.wide, c.len[s], a.max_len, t);
                 CHECK(steps >= 1 && end <= steps * FM_ATTN_KEYS && end <= a.max_len && (steps == 1 || end > (steps - 1) * FM_ATTN_KEYS));
@@ -248,7 +248,7 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
         if (!wide) share_out(c, a, b, D, ws);
         else {
             FmWide w;
-            fm_attn_wide_tiles(b, group, wide, &w);
+            fm_attn_wide_tiles(b, group, wide, a.narrow_most, &w);
             const int tiles = w.first[n_seq] * kv, units = tiles * a.splits;
             CHECK(a.groups <= units && ws == (a.splits == 1 ? 0 : (size_t)units * wide * (D + 2) * 4));
             std::set<int> picked;
@@ -261,7 +261,7 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
             std::set<std::vector<int>> seen;
             for (int u = 0; u < units; u++) {
                 const FmWideUnit at = fm_attn_wide_unit(w, n_seq, kv, a.splits, u);
-                CHECK(at.s < n_seq && at.h < kv && at.part < a.splits && at.tile >= 0 && at.tile < fm_attn_tiles(fm_seq_rows(b, at.s), group, wide));
+                CHECK(at.s < n_seq && at.h < kv && at.part < a.splits && at.tile >= 0 && at.tile < fm_attn_tiles(fm_seq_rows(b, at.s), group, wide, a.narrow_most));
                 CHECK(seen.insert({at.s, at.h, at.tile, at.part}).second);
                 const FmWideUnit one = fm_attn_wide_unit(w, n_seq, kv, a.splits, u / a.splits * a.splits);
                 CHECK(one.s == at.s && one.h == at.h && one.tile == at.tile && one.part == 0);
@@ -269,7 +269,7 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
         }
     }
     for (int s = 0; s < n_seq; s++) {      // a sequence's columns are in one of the two launches
-        const int n = fm_seq_rows(b, s), narrow = fm_attn_tiles(n, group, 0), wides = fm_attn_tiles(n, group, 64);
+        const int n = fm_seq_rows(b, s), narrow = fm_attn_tiles(n, group, 0, a.narrow_most), wides = fm_attn_tiles(n, group, 64, a.narrow_most);
         CHECK(!narrow || !wides);
         CHECK(narrow * FM_ATTN_COLS + wides * 64 >= n * group);
         covered += narrow + wides;

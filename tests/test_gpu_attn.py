@@ -143,6 +143,14 @@ def test_fp32_weights_keep_their_second_piece(hip, rows):
         _run(hip, seed, lens, rows, 8, 2, 128, 64, "float32")
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 128), (256, 32)])
+@pytest.mark.parametrize("lens,rows", [([140, 1, 300, 0, 33], [140, 1, 70, 0, 5]), ([700], [200]), ([260] * 5, [9, 40, 3, 60, 41])])
+def test_both_tile_widths_in_one_batch(hip, lens, rows, d, page, dtype):
+    """enough columns for wide tiles beside sequences that keep narrow ones; wide tiles split in parts"""
+    _run(hip, sum(rows) + d, lens, rows, 8, 2, d, page, dtype)
+
+
 def test_ragged_lengths_share_one_cut(hip):
     _run(hip, 7, [3, 4000, 700], [1, 1, 1], 2, 1, 64, 16, "float32")
 
@@ -156,7 +164,7 @@ def test_rows_that_see_nothing(hip):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("rows", [[1, 1], [40, 90]])
+@pytest.mark.parametrize("rows", [[1, 1], [40, 90], [300, 90]])
 def test_pages_that_are_not_there(hip, rows, dtype):
     """entries outside the pool are not seen; a sequence with none left gives zeros"""
     def spoil(cache, table):
@@ -167,7 +175,7 @@ def test_pages_that_are_not_there(hip, rows, dtype):
     assert float(got[:rows[0]].abs().max()) == 0.0
 
 
-@pytest.mark.parametrize("rows", [[1], [30]])
+@pytest.mark.parametrize("rows", [[1], [30], [530]])
 def test_shorter_max_len_and_table(hip, rows):
     _run(hip, 10, [200], rows, 2, 1, 64, 32, "float32", max_len=190)
     # more tokens than the table has pages for
@@ -182,7 +190,7 @@ def test_shorter_max_len_and_table(hip, rows):
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-@pytest.mark.parametrize("rows", [[1], [20]])
+@pytest.mark.parametrize("rows", [[1], [20], [530]])
 def test_what_is_masked_may_be_anything(hip, rows, dtype):
     """scales of pages behind the length are NaN and inf, so are later pages of the pool"""
     def spoil(cache, table):
@@ -197,7 +205,7 @@ def test_what_is_masked_may_be_anything(hip, rows, dtype):
     _run(hip, 12, [70], rows, 2, 1, 64, 32, dtype, more=4, spoil=spoil, max_len=200)
 
 
-@pytest.mark.parametrize("rows", [[1], [40]])
+@pytest.mark.parametrize("rows", [[1], [40], [530]])
 def test_value_scales_of_very_different_size(hip, rows):
     """pages whose values are 10^4 apart, in either order, and large ones"""
     def spoil(cache, table):
@@ -208,7 +216,7 @@ def test_value_scales_of_very_different_size(hip, rows):
 
 
 @pytest.mark.parametrize("size", [1e-30, 1e-3, 1e3])
-@pytest.mark.parametrize("rows", [[1], [40]])
+@pytest.mark.parametrize("rows", [[1], [40], [530]])
 def test_queries_of_any_size(hip, rows, size):
     import torch
     lens, page, d = [100], 16, 64
@@ -220,7 +228,7 @@ def test_queries_of_any_size(hip, rows, size):
     R.close(got, ref, _tol(most, vmax, d, 100, False), 0.0, "size %g" % size)
 
 
-@pytest.mark.parametrize("rows", [[1], [40]])
+@pytest.mark.parametrize("rows", [[1], [40], [530]])
 def test_large_scores_and_nan_rows(hip, rows):
     """scores in the thousands (one key takes all), and a query of NaN poisons its own row and head alone"""
     import torch
@@ -228,27 +236,29 @@ def test_large_scores_and_nan_rows(hip, rows):
     cache, table = _cache(16, 8, 1, page, d), _table(17, lens, page, 8)
     q = torch.randn(sum(rows), 2, d) * 300
     ref, _, vmax = R.attention(q, cache, table, lens, rows, 1.0, 100)
-    q[0, 1, 3] = float("nan")
+    q[-1, 1, 3] = float("nan")          # (the last row sees every key)
     got = Dev(hip, cache, table, lens).attn(q, rows, 1.0, 100)
-    assert bool(torch.isnan(got[0, 1]).all())
+    assert bool(torch.isnan(got[-1, 1]).all())
     fine = torch.ones(q.shape[:2], dtype=torch.bool)
-    fine[0, 1] = False
+    fine[-1, 1] = False
     assert bool(torch.isfinite(got[fine]).all())
     # (two nearly equal scores of a thousand may share the weight differently: none here)
-    near = (got[fine].double() - ref[fine]).abs().amax(-1)
+    near = (got[fine].double() - ref[fine]).abs().amax(-1)      # (rows that see nothing: zeros in both)
     assert float(near.median()) <= vmax * 1e-3
 
 
 @pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
-def test_strided_queries(hip, dtype):
+@pytest.mark.parametrize("rows", [[40, 1], [300, 1]])
+def test_strided_queries(hip, rows, dtype):
     import torch
-    lens, rows, page, d, hq = [90, 33], [40, 1], 32, 64, 4
+    lens, page, d, hq = [90, 33], 32, 64, 4
+    n = sum(rows)
     cache, table = _cache(18, 8, 2, page, d), _table(19, lens, page, 8)
-    wide = torch.randn(41, hq * d + 24).to(getattr(torch, dtype)).cuda()
+    wide = torch.randn(n, hq * d + 24).to(getattr(torch, dtype)).cuda()
     q = wide[:, 8:8 + hq * d]
-    ref, most, vmax = R.attention(q.cpu().reshape(41, hq, d), cache, table, lens, rows, 0.125, 90)
+    ref, most, vmax = R.attention(q.cpu().reshape(n, hq, d), cache, table, lens, rows, 0.125, 90)
     dev = Dev(hip, cache, table, lens)
-    out = torch.empty(41, hq, d, dtype=wide.dtype, device="cuda")
+    out = torch.empty(n, hq, d, dtype=wide.dtype, device="cuda")
     torch.cuda.synchronize()
     hip.attn_dev(dev.attn_args(q, rows, 0.125, 90, out, q_stride=wide.shape[1]))
     hip.sync()
@@ -256,7 +266,7 @@ def test_strided_queries(hip, dtype):
     R.close(out, ref, _tol(most, vmax, d, 90, bf), R.U_BF16 if bf else 0.0, "strided")
 
 
-@pytest.mark.parametrize("rows", [[1, 1, 1], [3, 90, 20]])
+@pytest.mark.parametrize("rows", [[1, 1, 1], [3, 90, 20], [3, 180, 20]])
 def test_attention_repeats_bit_for_bit(hip, rows):
     import torch
     lens, page, d = [3000, 100, 700], 32, 128
@@ -408,7 +418,7 @@ def test_offsets_past_32_bits(hip):
                     torch.tensor([[0, 1, 2]]), lens, lens, x, y)
     for got, ref in zip(small, want):
         assert torch.equal(got, ref)
-    for rows in ([1], [50]):
+    for rows in ([1], [50], [270]):
         q = torch.randn(sum(rows), kv, d, generator=g)
         ref, most, vmax = R.attention(q, small, torch.tensor([[0, 1, 2]]), lens, rows, 0.1, 300)
         R.close(dev.attn(q, rows, 0.1, 300), ref, _tol(most, vmax, d, 300, False), 0.0, "far pages")
