@@ -310,7 +310,7 @@ template <int D, bool BF16, bool ONCE>
 __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c, FmAttn a, FmSeqs b) {
     constexpr int NP = BF16 ? 1 : 2, DT = D / 16;
     __shared__ float s_o[3][DT][64][4];
-    __shared__ float s_m[4][16], s_l[4][16];
+    __shared__ float s_big[4][16], s_m[4][16], s_l[4][16];   // (wave 0 may still read s_m when the others take the next tile)
     __shared__ fm_v8h s_q[NP * (D / 32) * 64];
     __shared__ Shares sh;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
@@ -352,7 +352,7 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c,
         // (the queries first: who looks at a load's result waits for all that were issued before it)
         w.template fetch_q<BF16>(a.q, row * a.q_stride + (int64_t)qh * D);
         w.first(c, now, h, any ? pos : 0, any);
-        w.put_q(a.scale_log2, wave, s_q, s_m);
+        w.put_q(a.scale_log2, wave, s_q, s_big);
         lds_barrier();
         const fm_v8h *q = s_q + lane;
         if (any) {
@@ -414,7 +414,7 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c,
 // The codes of the next step are on their way in registers meanwhile; keys are replaced behind the first
 // product's barrier, values behind the second's, so a step has two barriers and one copy of each.
 // Bound by the matrix cores and the LDS alike: of a step of 128 columns x 64 keys x 256 dims, 2048 cycles of
-// products per SIMD, 3072 cycles of operand reads per CU.
+// products per SIMD and one and a half times that of operand reads per CU.
 template <int D, bool BF16>
 __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs b, FmWide w) {
     constexpr int NP = BF16 ? 1 : 2, CT = BF16 ? 2 : 1, KS = D / 32, DT = D / 16, LD = D / 64, WIDE = 64 * CT;
