@@ -803,7 +803,7 @@ __global__ __launch_bounds__(KV_T) void fm_kv_append(FmKv c, FmKvRows x, int D, 
     __syncthreads();                                             // (everybody has read the old scale, too)
 #pragma unroll
     for (int i = 0; i < KV_T / 64; i++) big = fmaxf(big, red[i]);
-    const float scale = fmaxf(old, __fdiv_rn(big, 127.0f));
+    const float scale = fmaxf(old, big * (1.0f / 127.0f));
     if (tid == 0) *scale_at = scale;
     int8_t *codes = value ? c.v + fm_kv_v_at(c, D, page, h, 0, 0) : c.k + fm_kv_k_at(c, D, page, h, 0, 0);
     if (t0 > 0 && scale != old) {                               // the old codes go to the new scale

@@ -432,7 +432,7 @@ typedef struct {
 
 /* fm_kv_append_dev: rows k, v [rows][kv_heads][head_dim] become the last tokens of their
  * sequences (positions d_len - rows of the sequence .. d_len - 1).  A page's scale is the largest finite
- * magnitude in it / 127; a page that already holds tokens keeps its scale unless a new token
+ * magnitude in it times the fp32 number 1/127; a page that already holds tokens keeps its scale unless a new token
  * exceeds it, then the old codes are rounded to the new scale.  code = round to nearest even of value / scale,
  * decided exactly; a NaN becomes 0, an infinity +-127.  The same rows appended again change nothing.
  * A page that two sequences of the call append to is not defined.

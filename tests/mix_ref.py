@@ -96,7 +96,7 @@ def append(cache, table, lens, rows, k, v):
                     x = x[row:row + take].double()                       # [take][heads][dim]
                     fin = torch.where(torch.isfinite(x), x.abs(), 0.0)
                     amax = fin.amax((0, 2)).float().numpy()
-                    new = torch.from_numpy((amax / np.float32(127)).astype(np.float32))
+                    new = torch.from_numpy((amax * (np.float32(1) / np.float32(127))).astype(np.float32))
                     old = sc[p].clone() if keep else torch.zeros_like(new)
                     new = torch.maximum(old, new)
                     div = new.double()[:, None, None]
