@@ -12,19 +12,20 @@
 // ones, the lower index.  The top_n keys of a segment: the top_n-th largest of a wave's 64 lane
 // maxima (to 16 bits, found bit by bit with ballots) bounds the segment's top_n-th value from below, so
 // does the largest of the waves' bounds; the elements that reach it, few more than top_n, are
-// collected and ranked by counting.  (Equal values, or many of the largest in one lane, may be more than
-// there is room for: then the maximum is taken top_n times instead.)  A second kernel joins a row's
+// collected, a list a wave, and ranked by counting.  (Equal values, or many of the largest in one lane, may be
+// more than there is room for: then the maximum is taken top_n times instead.)  A second kernel joins a row's
 // segments the same way.
 //
-// 257 rows of 248320: bound by the loads and, close behind, by the vector ALU (ten instruction slots an
-// element, four of them the exponential's).
+// 257 rows of 248320, top 5: 53 us, 4.8 TB/s, the rate of a large copy: bound by the loads and, close behind, by
+// the vector ALU (ten instruction slots an element, four of them the exponential's).  One row, top 20: 13.7 us,
+// the latency of two kernels, 8.8 of it without alternatives.
 #include "fm_common.h"
 
 namespace {
 
 constexpr int LP_T = 256;            // threads
 constexpr int LP_TOP = 32;
-constexpr int LP_CAND = 512;
+constexpr int LP_LIST = 128;         // candidates a wave has room for
 
 typedef unsigned long long LpKey;
 typedef float fm_v4 __attribute__((ext_vector_type(4)));
@@ -52,9 +53,9 @@ struct Part {             // what a segment leaves: statistics relative to its o
 };
 
 struct Shared {
-    LpKey cand[LP_CAND], bound[LP_T / 64];
+    LpKey cand[LP_T / 64][LP_LIST + 2], bound[LP_T / 64];   // (lists four banks apart)
     float red[2][LP_T / 64];
-    int n_cand;
+    int n_cand[LP_T / 64];
 };
 
 // The largest t with zero low half that at least n of the wave's lanes reach; 0 if fewer than n lanes have one.
@@ -73,34 +74,44 @@ __device__ __forceinline__ uint32_t nth_largest(uint32_t v, int n) {
 // big: the largest of those.
 template <int E, class Key, class Reaches>
 __device__ __forceinline__ void block_top(Key key, Reaches reaches, uint32_t big, int n, Shared &sh, LpKey *dst) {
-    const int t = threadIdx.x;
+    const int t = threadIdx.x, wave = t >> 6, lane = t & 63;
     const uint32_t of_wave = nth_largest(big, n);
-    if ((t & 63) == 0) sh.bound[t >> 6] = of_wave;
-    if (t == 0) sh.n_cand = 0;
+    if (lane == 0) sh.bound[wave] = of_wave;
     __syncthreads();
     uint32_t bound = 1;      // (order bits are never 0 for a number: 0 marks "none")
 #pragma unroll
     for (int w = 0; w < LP_T / 64; w++) bound = max(bound, (uint32_t)sh.bound[w]);
-    if (big >= bound) {
+    int c = 0;
+    if (__ballot(big >= bound)) {
 #pragma unroll
-        for (int e = 0; e < E; e++)
-            if (reaches(e, bound)) {
-                const LpKey k = key(e);
-                if (!k) continue;
-                const int at = atomicAdd(&sh.n_cand, 1);
-                if (at < LP_CAND) sh.cand[at] = k;
-            }
-    }
-    __syncthreads();
-    const int c = sh.n_cand;
-    if (c <= LP_CAND) {
-        for (int i = t; i < c; i += LP_T) {
-            const LpKey v = sh.cand[i];
-            int rank = 0;
-            for (int j = 0; j < c; j++) rank += sh.cand[j] > v;
-            if (rank < n) dst[rank] = v;
+        for (int e = 0; e < E; e++) {
+            const bool in = reaches(e, bound);
+            if (!__ballot(in)) continue;
+            const LpKey k = in ? key(e) : (LpKey)0;
+            const unsigned long long mask = __ballot(k != 0);
+            const int at = c + __popcll(mask & ((1ull << lane) - 1));
+            if (k && at < LP_LIST) sh.cand[wave][at] = k;
+            c += __popcll(mask);
         }
-        for (int i = c + t; i < n; i += LP_T) dst[i] = 0;
+    }
+    if (lane == 0) sh.n_cand[wave] = c;
+    __syncthreads();
+    static_assert(LP_T == 256, "four lists");
+    const int c0 = sh.n_cand[0], c1 = c0 + sh.n_cand[1], c2 = c1 + sh.n_cand[2], all = c2 + sh.n_cand[3];
+    if (max(max(c0, c1 - c0), max(c2 - c1, all - c2)) <= LP_LIST) {
+        // four lanes a candidate, each counts the larger ones of one list
+        const LpKey *list = sh.cand[t & 3];
+        const int many = sh.n_cand[t & 3];
+        for (int i = t >> 2; i < all; i += LP_T / 4) {
+            const LpKey v = i < c0 ? sh.cand[0][i] : i < c1 ? sh.cand[1][i - c0] : i < c2 ? sh.cand[2][i - c1] : sh.cand[3][i - c2];
+            int rank = 0;
+#pragma unroll 4
+            for (int j = 0; j < many; j++) rank += list[j] > v;
+            rank += __shfl_xor(rank, 1);
+            rank += __shfl_xor(rank, 2);
+            if (!(t & 3) && rank < n) dst[rank] = v;
+        }
+        for (int i = all + t; i < n; i += LP_T) dst[i] = 0;
         return;
     }
     LpKey below = ~0ull;
@@ -123,8 +134,9 @@ __device__ __forceinline__ void block_top(Key key, Reaches reaches, uint32_t big
 }
 
 // V4: rows are 16-byte aligned, a thread takes four elements side by side
+// (Five waves a SIMD: 257 rows 53 us; the 99 registers the compiler would take leave four, 57 us, and six spill, 55 us.)
 template <int E, bool V4>
-__global__ __launch_bounds__(LP_T) void fm_logprob_seg(const float *x, int vocab, int64_t stride, int n_seg, int top_n,
+__global__ __launch_bounds__(LP_T, 5) void fm_logprob_seg(const float *x, int vocab, int64_t stride, int n_seg, int top_n,
                                                        Part *parts, LpKey *tops) {
     __shared__ Shared sh;
     const int row = blockIdx.y, seg = blockIdx.x, t = threadIdx.x;
@@ -301,11 +313,13 @@ __global__ __launch_bounds__(LP_T) void fm_logprob_join(const float *x, int voca
     }
 }
 
-// Elements per thread: 32 when that still gives every CU two workgroups (the selection of the
-// largest runs once per segment), 16 otherwise.
+// Elements per thread: 32 when that still gives every CU three workgroups (the selection of the
+// largest runs once per segment), 16 otherwise.  Rows of 248320, top 20, with 32 / 16: 4 rows 15.0 / 13.8 us,
+// 16 rows 16.3 / 16.3, 24 rows 17.6 / 18.3, 32 rows 19.4 / 21.3, 128 rows 44.4 / 45.8; top 5: 24 rows
+// 13.8 / 13.6, 32 rows 14.9 / 15.4.
 int per_thread(int rows, int vocab, int n_cu) {
     const int64_t segs = ((int64_t)vocab + LP_T * 32 - 1) / (LP_T * 32);
-    return rows * segs >= 2 * n_cu ? 32 : 16;
+    return rows * segs >= 3 * n_cu ? 32 : 16;
 }
 
 }  // namespace
