@@ -1,7 +1,7 @@
 // fm_api.hip — the C ABI of libfinchhip.so (include/finch_hip.h): context,
 // HBM-resident weight stores, argument validation and kernel submission.
 // Host logic only; kernels live in fm_decode / fm_dense / fm_dequant / fm_gguf /
-// fm_prefill.
+// fm_prefill / fm_tail / fm_route / fm_gdn / fm_attn / fm_logprob.
 #include <stdarg.h>
 #include <stdio.h>
 #include <string.h>

@@ -58,7 +58,9 @@ FM_HD int fm_gdn_seq_of(const FmGdnSeqs &b, int c) {
 }
 
 #define FM_GDN_CHUNK 64
-// Sequences of fewer rows run token by token.
+// Sequences of fewer rows run token by token.  Measured (token by token / in chunks, us; 16 key and 32 value heads
+// of 128, bf16 alike): one sequence of 24 rows 18.6 / 19.0, of 32 22.7 / 18.9; eight sequences of 24 rows
+// 60.5 / 59.7.
 #define FM_GDN_MIN_CHUNKED 24
 // What the chunked form keeps per chunk between its two kernels, in floats: K and Q of a key head,
 // the lower tiles of T and P of a value head, each in the order the second kernel's lanes take them — tiles of 16
@@ -472,7 +474,8 @@ inline int fm_attn_splits(int64_t tiles, int groups, int most_steps) {
 }
 
 // Workgroups of a CU.  Narrow tiles: heads of 256 take a wave more registers than half a SIMD has (and a
-// spilled one would wait for the codes in flight).
+// spilled one would wait for the codes in flight); heads of 128 gain by a second one where few tiles are
+// long (one bf16 row over 30000 keys 38.7 us with two, 48.8 with one; 32 rows over 8000 keys 36.8 / 35.9).
 FM_HDC int fm_attn_per_cu(int D) { return D == 256 ? 1 : 2; }
 // Attention: the workgroups that fit on the chip share the steps, fewer if there cannot be as many.  Sets
 // n_tiles (0: no sequence for this launch), groups and splits; returns the workspace: of narrow tiles two parts
