@@ -890,7 +890,7 @@ void launch_attn(const FmKv &c, const FmAttn &a, const FmSeqs &b, hipStream_t st
 // ws: what fm_attn_check asked for
 extern "C" int fm_launch_attn(const FmKv *c, const FmAttn *args, const FmSeqs *b, int D, int bf16, void *ws, int n_cu, hipStream_t st) {
     for (int pass = 0; pass < 2; pass++) {
-        const int wide = pass ? fm_attn_wide_cols(bf16) : 0;
+        const int wide = pass ? args->wide_cols : 0;
         FmAttn a = *args;
         fm_attn_plan(c, &a, b, D, n_cu, wide);
         if (!a.n_tiles) continue;

@@ -183,6 +183,7 @@ struct FmAttn {
     int max_len;            // keys from here on are not seen, at most max_pages * page_tokens
     int wide;               // columns of a wide tile; 0: the launch of the sequences that have narrow ones
     int narrow_most;        // columns of a sequence up to which its tiles are narrow
+    int wide_cols;          // columns of the type's wide tiles
     int n_tiles;            // column tiles of the launch's sequence with the most rows
     int groups;             // workgroups that share the steps
     float *part_o, *part_ml;
@@ -199,8 +200,12 @@ FM_HDC int fm_attn_wide_cols(int bf16) { return bf16 ? 128 : 64; }
 // chip; measured (narrow / wide, us; 2 cache heads of 256): one sequence over 4000 keys 256 columns
 // 33 / 33 (fp32) and 31 / 37 (bf16), 512 columns 43 / 33 and 41 / 38, 1024 columns 67 / 39 and 64 / 39;
 // 16 sequences over 3000 keys 32 columns 36 / 32 and 34 / 38, 64 columns 49 / 35 and 46 / 39.
+// Beside wide ones the narrow tiles' two launches cost more than wide tiles for all where those are short: one
+// sequence of 300 rows and single rows, 2 cache heads of 256 (wide for all / separate, us; by the steps a workgroup then has):
+// bf16 4 steps 29 / 44, 8 42 / 48, 11 50 / 55 and 53 / 64, 21 78 / 74, 32 102 / 70; fp32 16 45 / 46, 21 65 / 52.
 #define FM_ATTN_NARROW_MOST 48
 #define FM_ATTN_WIDE_LEAST 1024
+#define FM_ATTN_MIXED_STEPS 12
 
 // ---- attention's steps and who takes them --------------------------------------------------
 // A sequence of n rows has n * group columns per cache head (row * group + query head of the group) in
@@ -477,6 +482,21 @@ inline int fm_attn_splits(int64_t tiles, int groups, int most_steps) {
 // spilled one would wait for the codes in flight); heads of 128 gain by a second one where few tiles are
 // long (one bf16 row over 30000 keys 38.7 us with two, 48.8 with one; 32 rows over 8000 keys 36.8 / 35.9).
 FM_HDC int fm_attn_per_cu(int D) { return D == 256 ? 1 : 2; }
+// Columns of a sequence up to which it has narrow tiles: none where with wide tiles for all a workgroup would have
+// FM_ATTN_MIXED_STEPS steps at most.
+inline int fm_attn_narrow_most(const FmKv *c, const FmAttn *a, const FmSeqs *b, int n_cu) {
+    if ((int64_t)fm_all_rows(*b) * a->group * c->kv_heads < FM_ATTN_WIDE_LEAST) return 0x7FFFFFFF;
+    bool some = false;
+    for (int s = 0; s < b->n_seq; s++) some |= fm_seq_rows(*b, s) * a->group > FM_ATTN_NARROW_MOST;
+    if (!some || !a->wide_cols) return FM_ATTN_NARROW_MOST;
+    FmWide w;
+    fm_attn_wide_tiles(*b, a->group, a->wide_cols, 0, &w);
+    const int64_t tiles = (int64_t)w.first[b->n_seq] * c->kv_heads;
+    const int steps = (a->max_len + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS, splits = fm_attn_splits(tiles, n_cu, steps);
+    const int64_t of_one = (tiles * splits + n_cu - 1) / n_cu * ((steps + splits - 1) / splits);
+    return of_one <= FM_ATTN_MIXED_STEPS ? 0 : FM_ATTN_NARROW_MOST;
+}
+
 // Attention: the workgroups that fit on the chip share the steps, fewer if there cannot be as many.  Sets
 // n_tiles (0: no sequence for this launch), groups and splits; returns the workspace: of narrow tiles two parts
 // per workgroup and the steps before each sequence, of wide ones the parts of split tiles.
@@ -484,7 +504,7 @@ inline size_t fm_attn_plan(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int
     const int64_t have = (int64_t)c->max_pages * c->page_tokens;
     if (a->max_len > have) a->max_len = (int)have;
     a->wide = wide;
-    a->narrow_most = (int64_t)fm_all_rows(*b) * a->group * c->kv_heads >= FM_ATTN_WIDE_LEAST ? FM_ATTN_NARROW_MOST : 0x7FFFFFFF;
+    a->narrow_most = fm_attn_narrow_most(c, a, b, n_cu);
     a->n_tiles = 0;
     a->splits = 1;
     int64_t most = 0;
@@ -527,9 +547,10 @@ inline int fm_attn_check(FmWhy *w, const fm_attn_args *p, int n_cu, FmKv *k, FmA
     a->group = p->q_heads / p->cache.kv_heads;
     a->scale_log2 = (float)((double)p->scale * 1.4426950408889634);
     a->max_len = p->max_len;
+    a->wide_cols = fm_attn_wide_cols(p->dtype == FM_DTYPE_BF16);
     fm_fill_seqs(b, p->seq_start, p->n_seq);
     FmAttn other = *a;       // (the two launches run one after the other in the same workspace)
-    const size_t wide = fm_attn_plan(k, &other, b, p->cache.head_dim, n_cu, fm_attn_wide_cols(p->dtype == FM_DTYPE_BF16));
+    const size_t wide = fm_attn_plan(k, &other, b, p->cache.head_dim, n_cu, a->wide_cols);
     *ws = fm_attn_plan(k, a, b, p->cache.head_dim, n_cu, 0);
     if (wide > *ws) *ws = wide;
     return FM_OK;

@@ -237,8 +237,10 @@ static void walk(int n_seq, int kv, int D, int P, int group) {
     b.n_seq = n_seq;
     for (int s = 0; s <= n_seq; s++) b.start[s] = start[s];
     int covered = 0;
-    for (int wide : {0, rnd(2) ? 64 : 128}) {
-        const size_t ws = fm_attn_plan(&c, &a, &b, D, 1 + rnd(64), wide);
+    const int wide_cols = rnd(2) ? 64 : 128, n_cu = 1 + rnd(64);
+    if (rnd(2)) a.wide_cols = wide_cols;      // (short sequences may go with the wide ones)
+    for (int wide : {0, wide_cols}) {
+        const size_t ws = fm_attn_plan(&c, &a, &b, D, n_cu, wide);
         CHECK(a.max_len <= max_pages * P);
         if (!a.n_tiles) {
             CHECK(ws == 0);

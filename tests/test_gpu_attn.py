@@ -151,6 +151,14 @@ def test_both_tile_widths_in_one_batch(hip, lens, rows, d, page, dtype):
     _run(hip, sum(rows) + d, lens, rows, 8, 2, d, page, dtype)
 
 
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("d,page", [(64, 16), (128, 128), (256, 32)])
+@pytest.mark.parametrize("lens,rows", [([140, 1, 300, 0, 33], [140, 1, 70, 0, 5]), ([900, 260, 5], [130, 1, 5])])
+def test_both_tile_widths_where_lengths_may_grow(hip, lens, rows, d, page, dtype):
+    """a bound of the lengths far above them: short sequences keep narrow tiles beside the wide ones"""
+    _run(hip, sum(rows) + d + 1, lens, rows, 8, 2, d, page, dtype, max_len=40000, more=40000 // page)
+
+
 def test_ragged_lengths_share_one_cut(hip):
     _run(hip, 7, [3, 4000, 700], [1, 1, 1], 2, 1, 64, 16, "float32")
 
