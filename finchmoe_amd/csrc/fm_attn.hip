@@ -416,9 +416,9 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c,
 // SIMD, so that one's softmax runs beside the other's products, in 256 registers each.
 // The codes of the next step are on their way in registers meanwhile; keys are replaced behind the first
 // product's barrier, values behind the second's, so a step has two barriers and one copy of each.
-// Bound by the matrix cores and the LDS alike: of a step of 128 columns x 64 keys x 256 dims, 2048 cycles of
-// products per SIMD and one and a half times that of operand reads per CU:
-// 2048 rows over 8192 keys, 16 heads of 256, bf16: 241 GFLOP in 335 us, 720 TFLOP/s.
+// 2048 rows over 8192 keys, 16 heads of 256, bf16: 241 GFLOP in 335 us, 720 TFLOP/s (a large library product 1050).  Bound
+// by no unit alone: of a step of 128 columns x 64 keys x 256 dims, 6200 cycles, products take 2048 per SIMD, operand
+// reads half of the LDS's time and the vector ALU is busy for 56 %, with two waves per SIMD and two barriers.
 template <int D, bool BF16>
 __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs b, FmWide w) {
     constexpr int NP = BF16 ? 1 : 2, CT = BF16 ? 2 : 1, KS = D / 32, DT = D / 16, LD = D / 64, WIDE = 64 * CT;
