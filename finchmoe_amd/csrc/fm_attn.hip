@@ -416,8 +416,8 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c,
 // SIMD, so that one's softmax runs beside the other's products, in 256 registers each.
 // The codes of the next step are on their way in registers meanwhile; keys are replaced behind the first
 // product's barrier, values behind the second's, so a step has two barriers and one copy of each.
-// 2048 rows over 8192 keys, 16 heads of 256, bf16: 241 GFLOP in 335 us, 720 TFLOP/s (a large library product 1050).  Bound
-// by no unit alone: of a step of 128 columns x 64 keys x 256 dims, 6200 cycles, products take 2048 per SIMD, operand
+// 2048 rows over 8192 keys, 16 heads of 256, bf16: 241 GFLOP in 328 us, 735 TFLOP/s (a large library product 1050).  Bound
+// by no unit alone: of a step of 128 columns x 64 keys x 256 dims, 6000 cycles, products take 2048 per SIMD, operand
 // reads half of the LDS's time and the vector ALU is busy for 56 %, with two waves per SIMD and two barriers.
 template <int D, bool BF16>
 __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs b, FmWide w) {

@@ -252,11 +252,13 @@ FM_HD int fm_kv_page(const FmKv &c, int s, int pos) {
     return p >= 0 && p < c.n_pages ? p : -1;
 }
 // byte offset of a code: keys [page][head][token][dim], values [page][head][dim][token]
+// (A shift for the values' page size: 2048 rows over 8192 keys 329 us, 335 with a 64-bit product.  With one for the
+// keys', too, narrow tiles come out slower, one row 17.2 us instead of 16.3.)
 FM_HD int64_t fm_kv_k_at(const FmKv &c, int D, int page, int head, int pos, int dim) {
     return (((int64_t)page * c.kv_heads + head) * c.page_tokens + (pos & (c.page_tokens - 1))) * D + dim;
 }
 FM_HD int64_t fm_kv_v_at(const FmKv &c, int D, int page, int head, int pos, int dim) {
-    return (((int64_t)page * c.kv_heads + head) * D + dim) * c.page_tokens + (pos & (c.page_tokens - 1));
+    return ((((int64_t)page * c.kv_heads + head) * D + dim) << c.page_shift) + (pos & (c.page_tokens - 1));
 }
 // Rows of one sequence that an append writes into its j-th page from the first one touched:
 // false if there are none.  start: the page's first position; tokens t0 .. t1 - 1 of it; row0: row
