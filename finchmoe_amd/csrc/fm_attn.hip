@@ -61,7 +61,7 @@ __device__ __forceinline__ fm_v8h codes_f16(uint32_t lo, uint32_t hi) {
 }
 
 // The pages of a lane's two runs of 16 keys: that of the tile rows it loads (run r / 4) and that of its
-// scores and of V (run g).  The table is read on every path and a step ahead, its entry judged when it
+// scores and of V (run g).  The table is read on every path and a step ahead, its entry checked when it
 // is used: whoever looks at a load's result waits for all that were issued before it.
 struct Runs {
     int k, v;        // table entries
@@ -71,11 +71,11 @@ struct Runs {
         v = table[min((pos0 + 16 * (lane >> 4)) >> c.page_shift, c.max_pages - 1)];
     }
     // page, or -1 for one that is not there
-    static __device__ __forceinline__ int judge(const FmKv &c, int entry, int pos) {
+    static __device__ __forceinline__ int checked(const FmKv &c, int entry, int pos) {
         return (pos >> c.page_shift) < c.max_pages && entry >= 0 && entry < c.n_pages ? entry : -1;
     }
-    __device__ __forceinline__ int k_page(const FmKv &c, int pos0) const { return judge(c, k, pos0 + 16 * ((threadIdx.x & 15) >> 2)); }
-    __device__ __forceinline__ int v_page(const FmKv &c, int pos0) const { return judge(c, v, pos0 + 16 * ((threadIdx.x & 63) >> 4)); }
+    __device__ __forceinline__ int k_page(const FmKv &c, int pos0) const { return checked(c, k, pos0 + 16 * ((threadIdx.x & 15) >> 2)); }
+    __device__ __forceinline__ int v_page(const FmKv &c, int pos0) const { return checked(c, v, pos0 + 16 * ((threadIdx.x & 63) >> 4)); }
 };
 
 // A wave's columns: running maximum (of scores in units of log2), sum and output, the codes of the step
