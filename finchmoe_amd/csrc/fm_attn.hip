@@ -17,14 +17,16 @@
 // straight into registers.
 // q and p are split in fp16 pieces behind a power of two that puts a column's largest element
 // near 2^8 (2^14 for p, whose keys' value scales ride along relative to the largest seen), far above
-// the subnormals: two pieces (22 bits) for fp32 vectors, one for bf16 ones (q is then exact, p
-// keeps 11 bits).
+// the subnormals: q in two pieces (22 bits) for fp32 vectors, in one for bf16 ones, which it holds exactly; p in
+// two pieces for either (one piece's 11 bits are an error of 2^-12 of a weight: where the values cancel, percents of
+// a bf16 result).
 #include "fm_mix.h"
 
 namespace {
 
 constexpr int BK = FM_ATTN_KEYS, COLS = FM_ATTN_COLS;
 constexpr float P_SHIFT = 14.0f;   // p is computed as 2^14 p
+constexpr int WP = 2;              // pieces of p
 
 __device__ __forceinline__ fm_v4f mfma(fm_v8h a, fm_v8h b, fm_v4f c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -242,18 +244,18 @@ struct Columns {
         v_scale = ldexpf(v_scale, -up);
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] *= keep_o;
-        fm_v8h p8[NP][2];
+        fm_v8h p8[WP][2];
 #pragma unroll
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
                 const float e = fast_exp2(sc[t][i] - base + P_SHIFT);
                 l += e;
-                _Float16 piece[NP];
-                split<NP>(e * v_scale, piece);
+                _Float16 piece[WP];
+                split<WP>(e * v_scale, piece);
                 const int j = 4 * (t & 1) + i;
 #pragma unroll
-                for (int p = 0; p < NP; p++) p8[p][t >> 1][j] = piece[p];
+                for (int p = 0; p < WP; p++) p8[p][t >> 1][j] = piece[p];
             }
 #pragma unroll
         for (int d0 = 0; d0 < DT; d0 += 4) {
@@ -261,7 +263,7 @@ struct Columns {
             for (int d = d0; d < d0 + 4; d++) {
                 const fm_v8h a0 = codes_f16(vc[d][0], vc[d][1]), a1 = codes_f16(vc[d][2], vc[d][3]);
 #pragma unroll
-                for (int p = 0; p < NP; p++) {
+                for (int p = 0; p < WP; p++) {
                     o[d] = mfma(a0, p8[p][0], o[d]);
                     o[d] = mfma(a1, p8[p][1], o[d]);
                 }
@@ -416,9 +418,9 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c,
 // SIMD, so that one's softmax runs beside the other's products, in 256 registers each.
 // The codes of the next step are on their way in registers meanwhile; keys are replaced behind the first
 // product's barrier, values behind the second's, so a step has two barriers and one copy of each.
-// 2048 rows over 8192 keys, 16 heads of 256, bf16: 241 GFLOP in 328 us, 735 TFLOP/s (a large library product 1050).  Bound
-// by no unit alone: of a step of 128 columns x 64 keys x 256 dims, 6000 cycles, products take 2048 per SIMD, operand
-// reads half of the LDS's time and the vector ALU is busy for 56 %, with two waves per SIMD and two barriers.
+// 2048 rows over 8192 keys, 16 heads of 256, bf16: 241 GFLOP in 390 us, 618 TFLOP/s (a large library product 1050);
+// with one piece of p 326 us.  A step of 128 columns x 64 keys x 256 dims has products for 3072 cycles a SIMD (1024 of
+// the scores, 2048 of the two pieces).
 template <int D, bool BF16>
 __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs b, FmWide w) {
     constexpr int NP = BF16 ? 1 : 2, CT = BF16 ? 2 : 1, KS = D / 32, DT = D / 16, LD = D / 64, WIDE = 64 * CT;
@@ -568,15 +570,15 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
                 __builtin_amdgcn_sched_barrier(0);
             }
             lds_barrier();                                        // the keys have been read, the values are there
-            fm_v8h xv[2][4];
+            fm_v8h xv[2][2];
             auto read_v = [&](int d0) {
 #pragma unroll
-                for (int d = 0; d < 4; d++) xv[d0 >> 2 & 1][d] = s_v[((d0 + d) * 2 + half) * 64];
+                for (int d = 0; d < 2; d++) xv[d0 >> 1 & 1][d] = s_v[((d0 + d) * 2 + half) * 64];
             };
             read_v(0);
             if (st + 1 < s1) put_k();
             const bool whole = __all(there) && pos + BK <= all_limit;      // nothing of the step is masked
-            fm_v8h p8[CT][NP];
+            fm_v8h p8[CT][WP];
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
                 const bool live = there && vpos < limit[ct];
@@ -620,22 +622,22 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
                     for (int i = 0; i < 4; i++) {
                         const float e = fast_exp2(sc[ct][t][i] + shift);
                         l[ct] += e;
-                        _Float16 piece[NP];
-                        split<NP>(e * v_scale, piece);
+                        _Float16 piece[WP];
+                        split<WP>(e * v_scale, piece);
 #pragma unroll
-                        for (int p = 0; p < NP; p++) p8[ct][p][4 * t + i] = piece[p];
+                        for (int p = 0; p < WP; p++) p8[ct][p][4 * t + i] = piece[p];
                     }
             }
 #pragma unroll
-            for (int d0 = 0; d0 < DT; d0 += 4) {
-                if (d0 + 4 < DT) read_v(d0 + 4);
+            for (int d0 = 0; d0 < DT; d0 += 2) {
+                if (d0 + 2 < DT) read_v(d0 + 2);
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                for (int d = 0; d < 4; d++)
+                for (int d = 0; d < 2; d++)
 #pragma unroll
                     for (int ct = 0; ct < CT; ct++)
 #pragma unroll
-                        for (int p = 0; p < NP; p++) o[ct][d0 + d] = mfma(xv[d0 >> 2 & 1][d], p8[ct][p], o[ct][d0 + d]);
+                        for (int p = 0; p < WP; p++) o[ct][d0 + d] = mfma(xv[d0 >> 1 & 1][d], p8[ct][p], o[ct][d0 + d]);
                 __builtin_amdgcn_sched_barrier(0);
             }
             now = next;
