@@ -16,10 +16,9 @@
 // of a V row, and nothing moves between lanes but the column's maximum.  Every load is 16 bytes
 // straight into registers.
 // q and p are split in fp16 pieces behind a power of two that puts a column's largest element
-// near 2^8 (2^14 for p, whose keys' value scales ride along relative to the largest seen), far above
-// the subnormals: q in two pieces (22 bits) for fp32 vectors, in one for bf16 ones, which it holds exactly; p in
-// two pieces for either (one piece's 11 bits are an error of 2^-12 of a weight: where the values cancel, percents of
-// a bf16 result).
+// near 2^8 (2^14 for p, whose keys' value scales ride along), far above the subnormals: q in two pieces (22 bits)
+// for fp32 vectors, in one for bf16 ones, which it holds exactly; p in two pieces for either (one piece's 11 bits are
+// an error of 2^-12 of a weight: where the values cancel, percents of a bf16 result).
 #include "fm_mix.h"
 
 namespace {
@@ -45,6 +44,46 @@ __device__ __forceinline__ void split(float f, _Float16 *piece) {
         piece[p] = (_Float16)f;
         f -= (float)piece[p];
     }
+}
+
+// The largest of a column's four lanes, in all of them.  (A swap with itself leaves either half in both: no way
+// through LDS as with a shuffle, whose latency two waves a SIMD do not cover.)
+__device__ __forceinline__ float column_max(float x) {
+    auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ int column_max(int x) {
+    auto a = __builtin_amdgcn_permlane16_swap((unsigned)x, (unsigned)x, false, false);
+    x = max((int)a[0], (int)a[1]);
+    auto b = __builtin_amdgcn_permlane32_swap((unsigned)x, (unsigned)x, false, false);
+    return max((int)b[0], (int)b[1]);
+}
+
+// Powers of two.  An output is held in units of 2^ref, above every weight times value scale so far: what a key
+// counts for goes by both, and a page of large values with next to no weight must not push the others below fp16.
+// NO_REF: of nothing seen.
+constexpr int NO_REF = -2000;
+// of a step: `top` the largest of the lane's scores, `base` the column's maximum.  (At most 120 below the page's own scale,
+// so that the scale in units of 2^ref stays in fp32's range; -246 of keys that are not seen, below all others.)
+__device__ __forceinline__ int ref_of(float v_scale, float top, float base) {
+    return (int)(__float_as_uint(v_scale) >> 23 & 255) - 126 + (int)ceilf(fmaxf(top - base, -120.0f));
+}
+// what is left of 2^ref when the maximum rises from m to base
+__device__ __forceinline__ int ref_falls(int ref, float m, float base) {
+    return max(ref + (int)ceilf(fmaxf(m - base, -1000.0f)), NO_REF);
+}
+// the power of two that a row's largest element is taken to 2^8 by, and back (the ends: zeros, infinities)
+__device__ __forceinline__ int q_power(float big) {
+    const int e = (int)(__float_as_uint(big) >> 23 & 255) - 127 - 8;
+    return e < -126 ? -126 : e > 119 ? 119 : e;
+}
+__device__ __forceinline__ float power2(int e) { return __uint_as_float((uint32_t)(127 + e) << 23); }
+__device__ __forceinline__ fm_v4f times_power2(fm_v4f x, int e) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) x[i] = ldexpf(x[i], e);
+    return x;
 }
 
 // eight signed bytes as fp16 numbers
@@ -87,8 +126,8 @@ template <int D, int NP, bool ONCE>
 struct Columns {
     static constexpr int KS = D / 32, DT = D / 16;
     fm_v4f o[DT];
-    float m, l, qscale;      // qscale: takes a score back from the power of two in q
-    int ref;                 // o is held in units of 2^ref, a power of two above every value scale seen
+    float m, l;
+    int qpow, ref;           // 2^qpow takes a score back from the power of two in q; o is held in units of 2^ref
     fm_v4u kc[D / 64][4], vc[DT];
     float ks, vs;
 
@@ -114,7 +153,7 @@ struct Columns {
                 x[u][h] = fm_ld4<BF16>(base, at + 64 * (s >> 1) + 16 * g + 8 * (s & 1) + 4 * h);
             }
     }
-    __device__ __forceinline__ void put_q(float scale_log2, int wave, fm_v8h *q, float (*s_big)[16]) {
+    __device__ __forceinline__ void put_q(int wave, fm_v8h *q, float (*s_big)[16]) {
         const int lane = threadIdx.x & 63, col = lane & 15;
         float big = 0.0f;
 #pragma unroll
@@ -128,10 +167,8 @@ struct Columns {
         if (lane < 16) s_big[wave][col] = big;
         lds_barrier();
         big = fmaxf(fmaxf(s_big[0][col], s_big[1][col]), fmaxf(s_big[2][col], s_big[3][col]));
-        int e = (int)(__float_as_uint(big) >> 23 & 255) - 127;
-        e = e > 100 ? 100 : e < -100 ? -100 : e;      // (zeros, infinities: any power will do)
-        const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
-        qscale = __uint_as_float((uint32_t)(127 - 8 + e) << 23) * scale_log2;
+        qpow = q_power(big);
+        const float up = power2(-qpow);
 #pragma unroll
         for (int u = 0; u < MY; u++) {
             fm_v8h v[NP];
@@ -148,7 +185,7 @@ struct Columns {
         }
         m = -INFINITY;
         l = 0.0f;
-        ref = -100;
+        ref = NO_REF;
 #pragma unroll
         for (int d = 0; d < DT; d++) o[d] = fm_v4f{0.f, 0.f, 0.f, 0.f};
     }
@@ -184,7 +221,7 @@ struct Columns {
     // 64 keys from position pos0, in the pages `now`; the column sees keys below `limit`.  MORE: each code register
     // takes the next step's (positions pos1, pages `next`) as soon as it is used.
     template <bool MORE>
-    __device__ __forceinline__ void step(const FmKv &c, int h, int pos0, int limit, const Runs &now, int pos1, const Runs &next,
+    __device__ __forceinline__ void step(const FmKv &c, float scale_log2, int h, int pos0, int limit, const Runs &now, int pos1, const Runs &next,
                                          const fm_v8h *q) {
         const int g = (threadIdx.x & 63) >> 4;
         const int vpos = pos0 + 16 * g;
@@ -216,7 +253,7 @@ struct Columns {
         }
         // (scales behind the last key may be anything)
         const bool live = now.v_page(c, pos0) >= 0 && vpos < limit;
-        const float f = (live ? ks : 0.0f) * qscale;
+        const float f = ldexpf((live ? ks : 0.0f) * scale_log2, qpow);
         float v_scale = live ? vs : 0.0f;
         if constexpr (MORE) load_scales(c, next, h, pos1);
         float top = -INFINITY;
@@ -227,18 +264,14 @@ struct Columns {
                 sc[t][i] = live && vpos + 4 * t + i < limit ? sc[t][i] * f : -INFINITY;
                 top = fmaxf(top, sc[t][i]);
             }
-        top = fmaxf(top, __shfl_xor(top, 16));
-        top = fmaxf(top, __shfl_xor(top, 32));
-        const float m1 = fmaxf(m, top);
+        const float m1 = fmaxf(m, column_max(top));
         // (nothing seen yet: any finite base keeps e^(-inf - base) at 0)
         const float base = m1 == -INFINITY ? 0.0f : m1;
         const float keep = fast_exp2(m - base);
+        const int left = ref_falls(ref, m, base);
         m = m1;
         l *= keep;
-        int up = live ? (int)(__float_as_uint(v_scale) >> 23 & 255) - 126 : -100;
-        up = max(ref, min(up, 100));
-        up = max(up, __shfl_xor(up, 16));
-        up = max(up, __shfl_xor(up, 32));
+        const int up = column_max(max(left, ref_of(v_scale, top, base)));
         const float keep_o = ldexpf(keep, ref - up);
         ref = up;
         v_scale = ldexpf(v_scale, -up);
@@ -316,6 +349,7 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c,
     constexpr int NP = BF16 ? 1 : 2, DT = D / 16;
     __shared__ float s_o[3][DT][64][4];
     __shared__ float s_big[4][16], s_m[4][16], s_l[4][16];   // (wave 0 may still read s_m when the others take the next tile)
+    __shared__ int s_ref[4][16];
     __shared__ fm_v8h s_q[NP * (D / 32) * 64];
     __shared__ Shares sh;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, col = lane & 15;
@@ -357,29 +391,38 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c,
         // (the queries first: who looks at a load's result waits for all that were issued before it)
         w.template fetch_q<BF16>(a.q, row * a.q_stride + (int64_t)qh * D);
         w.first(c, now, h, any ? pos : 0, any);
-        w.put_q(a.scale_log2, wave, s_q, s_big);
+        w.put_q(wave, s_q, s_big);
         lds_barrier();
         const fm_v8h *q = s_q + lane;
         if (any) {
             for (; pos + 4 * BK < end; pos += 4 * BK) {
                 Runs later;
                 later.load(c, table, min(pos + 8 * BK, end - BK));
-                w.template step<true>(c, h, pos, limit, now, pos + 4 * BK, next, q);
+                w.template step<true>(c, a.scale_log2, h, pos, limit, now, pos + 4 * BK, next, q);
                 now = next;
                 next = later;
             }
-            w.template step<false>(c, h, pos, limit, now, pos, now, q);
+            w.template step<false>(c, a.scale_log2, h, pos, limit, now, pos, now, q);
         }
         w.l += __shfl_xor(w.l, 16);
         w.l += __shfl_xor(w.l, 32);
 
-        // join the waves: wave 0 takes the others' sums at the common maximum
+        // join the waves: wave 0 takes the others' sums at the common maximum and power of two
         __syncthreads();                                          // (the last tile's sums have been read)
-        if (g == 0) s_m[wave][col] = w.m, s_l[wave][col] = w.l;
+        if (g == 0) s_m[wave][col] = w.m, s_l[wave][col] = w.l, s_ref[wave][col] = w.ref;
         __syncthreads();
         const float m = fmaxf(fmaxf(s_m[0][col], s_m[1][col]), fmaxf(s_m[2][col], s_m[3][col]));
         const float base = m == -INFINITY ? 0.0f : m;
-        const float f = ldexpf(fast_exp2(w.m - base), w.ref);
+        float l = 0.0f;
+        int ref = NO_REF;
+#pragma unroll
+        for (int v = 0; v < 4; v++) {
+            l = fmaf(s_l[v][col], fast_exp2(s_m[v][col] - base), l);
+            ref = max(ref, ref_falls(s_ref[v][col], s_m[v][col], base));
+        }
+        // (a part of a tile is normalised as well: its output is a mean of values)
+        const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+        const float f = ldexpf(fast_exp2(w.m - base) * inv, w.ref - ref);
 #pragma unroll
         for (int d = 0; d < DT; d++) w.o[d] *= f;
         if (wave) {
@@ -388,20 +431,18 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c,
         }
         __syncthreads();
         if (wave) continue;
-        float l = 0.0f;
-#pragma unroll
-        for (int v = 0; v < 4; v++) l = fmaf(s_l[v][col], fast_exp2(s_m[v][col] - base), l);
 #pragma unroll
         for (int d = 0; d < DT; d++)
 #pragma unroll
             for (int v = 0; v < 3; v++) w.o[d] += *(const fm_v4f *)s_o[v][d][lane];
         // register i of tile d: dim 16 d + 4 g + i
+#pragma unroll
+        for (int d = 0; d < DT; d++) w.o[d] = times_power2(w.o[d], ref);
         if (s0 == 0 && s1 == steps) {
             if (!there) continue;
-            const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
             const int64_t to = (row * a.q_heads + qh) * D + 4 * g;
 #pragma unroll
-            for (int d = 0; d < DT; d++) fm_st4<BF16>(a.out, to + 16 * d, w.o[d] * inv);
+            for (int d = 0; d < DT; d++) fm_st4<BF16>(a.out, to + 16 * d, w.o[d]);
         } else {
             const int64_t to = (int64_t)fm_attn_slot(blockIdx.x, s0) * COLS + col;
 #pragma unroll
@@ -418,8 +459,8 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c,
 // SIMD, so that one's softmax runs beside the other's products, in 256 registers each.
 // The codes of the next step are on their way in registers meanwhile; keys are replaced behind the first
 // product's barrier, values behind the second's, so a step has two barriers and one copy of each.
-// 2048 rows over 8192 keys, 16 heads of 256, bf16: 241 GFLOP in 390 us, 618 TFLOP/s (a large library product 1050);
-// with one piece of p 326 us.  A step of 128 columns x 64 keys x 256 dims has products for 3072 cycles a SIMD (1024 of
+// 2048 rows over 8192 keys, 16 heads of 256, bf16: 241 GFLOP in 398 us, 606 TFLOP/s (a large library product 1050);
+// with one piece of p and a power of two that goes by the value scales alone 326 us.  A step of 128 columns x 64 keys x 256 dims has products for 3072 cycles a SIMD (1024 of
 // the scores, 2048 of the two pieces).
 template <int D, bool BF16>
 __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs b, FmWide w) {
@@ -430,6 +471,7 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
     constexpr int O_ALL = 4 * CT * DT * 64;
     __shared__ fm_v8h lds[ALL > O_ALL ? ALL : O_ALL];
     __shared__ float s_m[4][CT][16], s_l[4][CT][16];
+    __shared__ int s_ref[4][CT][16];
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), lane = threadIdx.x & 63, g = lane >> 4, r = lane & 15;
     const int cg = wave & 3, half = wave >> 2;
     const fm_v8h *s_k = lds + K_AT + lane, *s_v = lds + V_AT + lane;
@@ -447,8 +489,8 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
         now.load(c, table, s0 * BK);
         next.load(c, table, max(min(s0 + 1, s1 - 1), 0) * BK);
         fm_v4f o[CT][DT];
-        float m[CT], l[CT], qscale[CT];
-        int ref[CT], limit[CT], all_limit = 0x7FFFFFFF;
+        float m[CT], l[CT];
+        int qpow[CT], ref[CT], limit[CT], all_limit = 0x7FFFFFFF;
         int64_t to[CT];          // the column's place in the output, -1 if it is not there
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
@@ -472,10 +514,8 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
                 for (int j = 0; j < 8; j++) big = fmaxf(big, fabsf(x[k][j >> 2][j & 3]));
             big = fmaxf(big, __shfl_xor(big, 16));
             big = fmaxf(big, __shfl_xor(big, 32));
-            int e = (int)(__float_as_uint(big) >> 23 & 255) - 127;
-            e = e > 100 ? 100 : e < -100 ? -100 : e;
-            const float up = __uint_as_float((uint32_t)(127 + 8 - e) << 23);
-            qscale[ct] = __uint_as_float((uint32_t)(127 - 8 + e) << 23) * a.scale_log2;
+            qpow[ct] = q_power(big);
+            const float up = power2(-qpow[ct]);
             // (both halves' waves have the columns: each writes half of the k steps)
             if (!ct) lds_barrier();                               // (the last tile's operands have been read)
 #pragma unroll
@@ -494,7 +534,7 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
             }
             m[ct] = -INFINITY;
             l[ct] = 0.0f;
-            ref[ct] = -100;
+            ref[ct] = NO_REF;
 #pragma unroll
             for (int d = 0; d < DT; d++) o[ct][d] = fm_v4f{0.f, 0.f, 0.f, 0.f};
         }
@@ -537,7 +577,7 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
         put_k();
         for (int st = s0; st < s1; st++) {
             const int pos = st * BK, vpos = pos + 16 * g + 8 * half;      // first of this lane's eight keys
-            const float k_scale = ks, v_scale0 = vs;
+            const float k_scale = ks * a.scale_log2, v_scale0 = vs;
             const bool there = now.v_page(c, pos) >= 0;
             lds_barrier();                                        // the step's keys are there, the last one's values read
             put_v();
@@ -582,7 +622,7 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
                 const bool live = there && vpos < limit[ct];
-                const float f = (live ? k_scale : 0.0f) * qscale[ct];
+                const float f = ldexpf(live ? k_scale : 0.0f, qpow[ct]);
                 float v_scale = live ? v_scale0 : 0.0f, top = -INFINITY;
                 if (whole) {
 #pragma unroll
@@ -598,15 +638,11 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
                             top = fmaxf(top, sc[ct][t][i]);
                         }
                 }
-                top = fmaxf(top, __shfl_xor(top, 16));
-                top = fmaxf(top, __shfl_xor(top, 32));
-                const float m1 = fmaxf(m[ct], top), base = m1 == -INFINITY ? 0.0f : m1;
+                const float m1 = fmaxf(m[ct], column_max(top)), base = m1 == -INFINITY ? 0.0f : m1;
                 const float keep = fast_exp2(m[ct] - base);
+                const int left = ref_falls(ref[ct], m[ct], base);
                 m[ct] = m1;
-                int up = live ? (int)(__float_as_uint(v_scale) >> 23 & 255) - 126 : -100;
-                up = max(ref[ct], min(up, 100));
-                up = max(up, __shfl_xor(up, 16));
-                up = max(up, __shfl_xor(up, 32));
+                const int up = column_max(max(left, ref_of(v_scale, top, base)));
                 const float keep_o = ldexpf(keep, ref[ct] - up);
                 ref[ct] = up;
                 v_scale = ldexpf(v_scale, -up);
@@ -643,7 +679,7 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
             now = next;
             next = later;
         }
-        // the second halves' outputs to the first halves' waves, at the common maximum
+        // the second halves' outputs to the first halves' waves, at the common maximum and power of two
 #pragma unroll
         for (int ct = 0; ct < CT; ct++) {
             l[ct] += __shfl_xor(l[ct], 16);
@@ -653,10 +689,9 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
         if (half) {
 #pragma unroll
             for (int ct = 0; ct < CT; ct++) {
-                const float unit2 = ldexpf(1.0f, ref[ct]);
-                if (g == 0) s_m[cg][ct][r] = m[ct], s_l[cg][ct][r] = l[ct];
+                if (g == 0) s_m[cg][ct][r] = m[ct], s_l[cg][ct][r] = l[ct], s_ref[cg][ct][r] = ref[ct];
 #pragma unroll
-                for (int d = 0; d < DT; d++) *(fm_v4f *)(lds + ((cg * CT + ct) * DT + d) * 64 + lane) = o[ct][d] * unit2;
+                for (int d = 0; d < DT; d++) *(fm_v4f *)(lds + ((cg * CT + ct) * DT + d) * 64 + lane) = o[ct][d];
             }
         }
         lds_barrier();
@@ -665,13 +700,16 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
         for (int ct = 0; ct < CT; ct++) {
             if (to[ct] < 0) continue;
             const float m2 = s_m[cg][ct][r], both = fmaxf(m[ct], m2), base = both == -INFINITY ? 0.0f : both;
-            const float e1 = fast_exp2(m[ct] - base), e2 = fast_exp2(m2 - base), f1 = ldexpf(e1, ref[ct]);
+            const float e1 = fast_exp2(m[ct] - base), e2 = fast_exp2(m2 - base);
+            const int ref2 = s_ref[cg][ct][r], top = max(ref_falls(ref[ct], m[ct], base), ref_falls(ref2, m2, base));
             const float sum = e1 * l[ct] + e2 * s_l[cg][ct][r];
-            const float inv = a.splits > 1 ? 1.0f : sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+            // (a part of a tile is normalised as well: its output is a mean of values)
+            const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
+            const float f1 = ldexpf(e1 * inv, ref[ct] - top), f2 = ldexpf(e2 * inv, ref2 - top);
             const int64_t part = (int64_t)unit * WIDE + (cg * CT + ct) * 16 + r;
 #pragma unroll
             for (int d = 0; d < DT; d++) {
-                const fm_v4f z = (o[ct][d] * f1 + *(const fm_v4f *)(lds + ((cg * CT + ct) * DT + d) * 64 + lane) * e2) * inv;
+                const fm_v4f z = times_power2(o[ct][d] * f1 + *(const fm_v4f *)(lds + ((cg * CT + ct) * DT + d) * 64 + lane) * f2, top);
                 if (a.splits == 1) fm_st4<BF16>(a.out, to[ct] + 16 * d + 4 * g, z);
                 else *(fm_v4f *)(a.part_o + part * D + 16 * d + 4 * g) = z;
             }
@@ -680,25 +718,34 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
     }
 }
 
-// One column out of `parts` parts, by a wave: D / 64 dims a lane, a lane per part for its weight
-// e^(m - base).  slot(k): where part k's column lies.
+// One column out of `parts` parts, by a wave: D / 64 dims a lane, a lane per part for its weight, its sum at
+// the common maximum over all of them.  slot(k): where part k's column lies.
 template <int D, bool BF16, class Slot>
 __device__ __forceinline__ void join_column(const FmAttn &a, int parts, Slot slot, int64_t to) {
     const int lane = threadIdx.x & 63;
-    float m = -INFINITY;
-    for (int k = lane; k < parts; k += 64) m = fmaxf(m, a.part_ml[2 * slot(k)]);
+    auto of = [&](int k) { return k < parts ? *(const float2 *)(a.part_ml + 2 * slot(k)) : float2{-INFINITY, 0.0f}; };
+    const float2 first = of(lane);
+    float m = first.x;
+    for (int k = lane + 64; k < parts; k += 64) m = fmaxf(m, of(k).x);
     for (int o = 32; o; o >>= 1) m = fmaxf(m, __shfl_xor(m, o));
-    const float base = m == -INFINITY ? 0.0f : m;
-    float l = 0.0f, o[D / 64];
+    const float base = m == -INFINITY ? 0.0f : m, first_l = fast_exp2(first.x - base) * first.y;
+    float l = first_l, o[D / 64];
+    for (int k = lane + 64; k < parts; k += 64) {
+        const float2 p = of(k);
+        l = fmaf(fast_exp2(p.x - base), p.y, l);
+    }
+    l = fm_group_sum<64>(l);
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
     for (int d = 0; d < D / 64; d++) o[d] = 0.0f;
     for (int k0 = 0; k0 < parts; k0 += 64) {
         const int some = min(64, parts - k0);
-        float f = 0.0f;
-        if (lane < some) {
-            f = fast_exp2(a.part_ml[2 * slot(k0 + lane)] - base);
-            l = fmaf(f, a.part_ml[2 * slot(k0 + lane) + 1], l);
+        float f = first_l;
+        if (k0) {
+            const float2 p = of(k0 + lane);
+            f = fast_exp2(p.x - base) * p.y;
         }
+        f *= inv;
 #pragma unroll 4
         for (int k = 0; k < some; k++) {
             const float *p = a.part_o + slot(k0 + k) * D + lane;
@@ -707,10 +754,8 @@ __device__ __forceinline__ void join_column(const FmAttn &a, int parts, Slot slo
             for (int d = 0; d < D / 64; d++) o[d] = fmaf(fk, p[64 * d], o[d]);
         }
     }
-    l = fm_group_sum<64>(l);
-    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
 #pragma unroll
-    for (int d = 0; d < D / 64; d++) fm_st1<BF16>(a.out, to + 64 * d + lane, o[d] * inv);
+    for (int d = 0; d < D / 64; d++) fm_st1<BF16>(a.out, to + 64 * d + lane, o[d]);
 }
 
 // Narrow tiles that several workgroups took: four columns a workgroup.

@@ -374,7 +374,7 @@ FM_API int fm_embed_lookup(fm_ctx *ctx, fm_tensor t, int token_id, float *out);
  * What stands between the quantized products of a token: the gated delta rule that the
  * GatedDeltaNet projections feed, and attention over a cache held in 8 bits.  Vectors are fp32,
  * or bfloat16 bits where dtype says so; sums, statistics and states are fp32 in either case, and
- * attention's weights keep 22 bits.
+ * attention's weights keep 22 bits of the largest weight times value scale.
  * Rows (tokens) of several sequences lie one behind the other; seq_start names where each begins:
  * n_seq + 1 ascending row numbers in HOST memory, the first of them 0 (a sequence may be empty).
  * seq_start == NULL: one row per sequence.  It is read during the call only; the launch carries

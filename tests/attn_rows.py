@@ -25,21 +25,25 @@ def attention(q, cache, table, lens, rows, scale, max_len):
     group, at = hq // ck.shape[1], R.starts(rows)
     for s, (length, r) in enumerate(zip(lens, rows)):
         m = max(0, min(length, max_len, table.shape[1] * page))
+        if not m or not r:
+            continue
         k, v, there = R.page_values(ck, cv, ks, vs, table[s], m, page)
         pos = torch.arange(m)
-        for i in range(r):
-            see = there & (pos <= length - r + i)
-            keys = int(see.sum())
-            if not keys:
-                continue
-            for h in range(hq):
-                kk, vv, qq = k[see][:, h // group], v[see][:, h // group], q[at[s] + i, h].double()
-                w = torch.softmax(kk @ qq * scale, 0)
-                big = float((kk.abs() @ qq.abs()).max()) * abs(scale)
-                of_page = torch.stack([vs[int(table[s, int(p) // page]), h // group].double() for p in pos[see]])
-                rel = math.expm1(min(2 * big * (d + 8) * R.U24, 50.0)) + (keys / 32 + 48) * R.U24
-                out[at[s] + i, h] = w @ vv
-                tol[at[s] + i, h] = w @ vv.abs() * rel + float((w * of_page.abs()).max()) * 127 * keys * 2.0 ** -38
+        see = there[None] & (pos[None] <= length - r + torch.arange(r)[:, None])
+        keys = see.sum(-1, keepdim=True).double()
+        on = table[s].long()[pos // page].clamp(0, ck.shape[0] - 1)
+        for h in range(hq):
+            kk, vv, qq = k[:, h // group], v[:, h // group], q[at[s]:at[s] + r, h].double()
+            z = (qq @ kk.t() * scale).masked_fill(~see, -math.inf)
+            w = torch.exp(z - z.amax(-1, keepdim=True).clamp(min=-1e300))
+            w = w / w.sum(-1, keepdim=True).clamp(min=1e-300)
+            big = (qq.abs() @ kk.abs().t() * abs(scale)).masked_fill(~see, 0.0).amax(-1, keepdim=True)
+            rel = torch.expm1((2 * big * (d + 8) * R.U24).clamp(max=50.0)) + (keys / 32 + 48) * R.U24
+            most = (w * vs[on, h // group].double().abs()[None]).masked_fill(~see, 0.0).amax(-1, keepdim=True)
+            w = w.masked_fill(~see, 0.0)
+            vv = vv.masked_fill(~there[:, None], 0.0)
+            out[at[s]:at[s] + r, h] = w @ vv
+            tol[at[s]:at[s] + r, h] = w @ vv.abs() * rel + most * 127 * keys * 2.0 ** -38
     return out, tol
 
 

@@ -30,3 +30,97 @@ def test_bf16_calls_keep_the_weights(hip, d, rows):
     cache, table = _cache(61, 8, 2, page, d), _table(62, lens, page, 8)
     q = (0.05 * torch.randn(sum(rows), 16, d, generator=g)).to(torch.bfloat16)
     _run(hip, cache, table, lens, rows, q, d ** -0.5)
+
+
+def _paged(seed, d, rows, dtype, lead, value_scale, page=32, size=1.0):
+    """Five pages; query head h and cache head 0 or 1 alike: dim 0 of a page's keys is +-127 and decides, `lead`
+    (natural units) above or below; the rest is small noise.  value_scale: a factor a page."""
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    lens = [150] if len(rows) == 1 and rows[0] <= 150 else [rows[0]] if len(rows) == 1 else [150] * len(rows)
+    n_pages = sum(-(-n // page) for n in lens) + 1
+    cache, table = _cache(seed + 1, n_pages, 2, page, d), _table(seed + 2, lens, page, n_pages)
+    cache[2].fill_(1.0 / 127)
+    cache[0].copy_((torch.randn(cache[0].shape, generator=g) * 4).round().clamp(-12, 12).to(torch.int8))
+    for s in range(len(lens)):
+        for at in range(-(-lens[s] // page)):
+            p = int(table[s, at])
+            cache[0][p, :, :, 0] = int(127 * lead[at % len(lead)])
+            cache[3][p] *= value_scale[at % len(value_scale)]
+    q = 0.5 * torch.randn(sum(rows), 4, d, generator=g)
+    q[:, :, 0] = 1.0
+    return cache, table, lens, (q * size).to(getattr(torch, dtype))
+
+
+ROWS = [[1], [1] * 9, [40], [600]]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ROWS, ids=str)
+@pytest.mark.parametrize("lead,values", [
+    ((1, -1, 1, -1, 1), (1.0, 2.0 ** 60, 0.5, 2.0 ** 70, 3.0)),       # large values with next to no weight, between
+    ((-1, -1, 1, 1, 1), (2.0 ** 60, 2.0 ** 65, 1.0, 0.3, 1.0)),       # ahead of the page that has the weight
+    ((1, 1, -1, -1, -1), (2.0 ** -60, 2.0 ** -61, 2.0 ** 25, 1.0, 1.0)),      # behind it
+    ((1, -1, 1, -1, 1), (1.0, 2.0 ** 115, 0.5, 2.0 ** 116, 3.0)),     # weight times value about alike
+])
+def test_values_count_by_their_weight(hip, lead, values, rows, dtype):
+    """pages whose values are up to 2^116 apart, the smaller ones with (nearly) all of the weight: score 40 above and 40
+    below, weights 2^115 apart"""
+    cache, table, lens, q = _paged(70, 64, rows, dtype, lead, values)
+    _run(hip, cache, table, lens, rows, q, 40.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ROWS, ids=str)
+@pytest.mark.parametrize("d", [64, 256])
+def test_values_far_apart_with_like_weights(hip, d, rows, dtype):
+    """small values count with the keys of their own row: rows that only see the small page keep its digits"""
+    cache, table, lens, q = _paged(75, d, rows, dtype, (0.02, 0.0, -0.02, 0.01, 0.0), (1e-9, 1e-4, 300.0, 1e7, 1.0))
+    _run(hip, cache, table, lens, rows, q, 1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ROWS, ids=str)
+@pytest.mark.parametrize("power", [118, 103, -100, -115])
+def test_values_near_the_ends_of_fp32(hip, power, rows, dtype):
+    """values of up to 2^119 and down to 2^-121: a weighted mean of finite numbers is one"""
+    f = 2.0 ** power
+    cache, table, lens, q = _paged(80, 128, rows, dtype, (0.02, 0.0, -0.02, 0.01, 0.0), (f, 0.5 * f, f, 0.3 * f, 0.1 * f))
+    _run(hip, cache, table, lens, rows, q, 1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ROWS, ids=str)
+@pytest.mark.parametrize("power", [120, 110, -105, -120])
+def test_queries_near_the_ends_of_fp32(hip, power, rows, dtype):
+    cache, table, lens, q = _paged(85, 64, rows, dtype, (0.02, 0.0, -0.02, 0.01, 0.0), (1.0, 2.0), size=2.0 ** power)
+    _run(hip, cache, table, lens, rows, q, 2.0 ** -power)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ROWS, ids=str)
+def test_large_scores(hip, rows, dtype):
+    """scores in the thousands, where one key takes nearly all: every row against its own bound"""
+    import torch
+    lens, page, d = [max(rows[0], 100)] * len(rows), 16, 64
+    n_pages = sum(-(-n // page) for n in lens) + 1
+    cache, table = _cache(90, n_pages, 1, page, d), _table(91, lens, page, n_pages)
+    g = torch.Generator().manual_seed(92)
+    q = (torch.randn(sum(rows), 2, d, generator=g) * 300).to(getattr(torch, dtype))
+    _run(hip, cache, table, lens, rows, q, 1.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_mixed_batches_with_values_far_apart(hip, dtype):
+    """a prompt and single rows, the prompt's tiles split in parts, and long sequences joined from many parts"""
+    rows = [200, 1, 1, 30]
+    cache, table, lens, q = _paged(95, 128, rows, dtype, (1, -1, 0.9, -1, 1), (1.0, 2.0 ** 60, 0.5, 2.0 ** 70, 3.0))
+    lens = [150] * 4
+    _run(hip, cache, table, lens, rows, q, 40.0)
+    import torch
+    lens, rows, page, d = [2600], [3], 32, 64
+    n_pages = 82
+    cache, table = _cache(97, n_pages + 1, 2, page, d), _table(98, lens, page, n_pages)
+    cache[3].mul_(torch.exp2(torch.randint(-30, 30, cache[3].shape, generator=torch.Generator().manual_seed(99)).float()))
+    q = torch.randn(3, 4, d, generator=torch.Generator().manual_seed(100)).to(getattr(torch, dtype))
+    _run(hip, cache, table, lens, rows, q, 6.0)
