@@ -34,6 +34,10 @@ __device__ __forceinline__ fm_v4f mfma(fm_v8h a, fm_v8h b, fm_v4f c) {
 // 2^x; below -126 (of which nothing is left in what follows) 0
 __device__ __forceinline__ float fast_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
+// A key's weight behind its power of two.  (The difference first: 14 - base would be rounded at the size of the scores, and
+// from 2^25 on p could pass fp16's largest number.)
+__device__ __forceinline__ float weight(float score, float base) { return fast_exp2((score - base) + P_SHIFT); }
+
 // f as NP fp16 pieces whose sum it is (to 11 bits each).  With two, f has to be one fp32 value: fused with the
 // product in front of it, the conversion and the remainder could round to different first pieces.
 template <int NP>
@@ -282,7 +286,7 @@ struct Columns {
         for (int t = 0; t < 4; t++)
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const float e = fast_exp2(sc[t][i] - base + P_SHIFT);
+                const float e = weight(sc[t][i], base);
                 l += e;
                 _Float16 piece[WP];
                 split<WP>(e * v_scale, piece);
@@ -651,12 +655,11 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
 #pragma unroll
                     for (int d = 0; d < DT; d++) o[ct][d] *= keep_o;
                 }
-                const float shift = P_SHIFT - base;
 #pragma unroll
                 for (int t = 0; t < 2; t++)
 #pragma unroll
                     for (int i = 0; i < 4; i++) {
-                        const float e = fast_exp2(sc[ct][t][i] + shift);
+                        const float e = weight(sc[ct][t][i], base);
                         l[ct] += e;
                         _Float16 piece[WP];
                         split<WP>(e * v_scale, piece);

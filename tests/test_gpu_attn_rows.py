@@ -124,3 +124,28 @@ def test_mixed_batches_with_values_far_apart(hip, dtype):
     cache[3].mul_(torch.exp2(torch.randint(-30, 30, cache[3].shape, generator=torch.Generator().manual_seed(99)).float()))
     q = torch.randn(3, 4, d, generator=torch.Generator().manual_seed(100)).to(getattr(torch, dtype))
     _run(hip, cache, table, lens, rows, q, 6.0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", ROWS, ids=str)
+@pytest.mark.parametrize("score", [3e7, 3.1e7, -5e7, 1e8, 1.3e8, 1e20, -1e30])
+def test_equal_scores_of_any_size(hip, score, rows, dtype):
+    """keys of one and the same score have like weights, however large it is: the mean of the values seen.  Bound: the
+    weights' own 8 half steps of fp32 and the sums', relative to the mean of |v|"""
+    import torch
+    page, d = 32, 128
+    lens = [max(rows[0], 100)] * len(rows)
+    n_pages = sum(-(-n // page) for n in lens) + 1
+    cache, table = _cache(110, n_pages, 2, page, d), _table(111, lens, page, n_pages)
+    cache[0].zero_()
+    cache[0][..., 0] = 127
+    cache[2].fill_(1.0 / 128)
+    cache[3].fill_((1 - 2.0 ** -16) / 64)       # (just below a power of two)
+    q = torch.randn(sum(rows), 4, d, generator=torch.Generator().manual_seed(112))
+    q[..., 0] = 1.0
+    q = q.to(getattr(torch, dtype))
+    ref, _ = A.attention(q, cache, table, lens, rows, 0.0, max(lens))
+    size = tuple(t.abs() if i in (1, 3) else t for i, t in enumerate(cache[:4])) + (page,)
+    mean, _ = A.attention(q, size, table, lens, rows, 0.0, max(lens))
+    got = Dev(hip, cache, table, lens).attn(q, rows, score, max(lens))
+    A.check(got, ref, mean * (max(lens) / 32 + 48) * R.U24, q.dtype)
