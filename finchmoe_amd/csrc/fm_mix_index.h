@@ -192,6 +192,7 @@ struct FmAttn {
 };
 #define FM_ATTN_KEYS 64     // keys of a wave's step
 #define FM_ATTN_WAVES 4     // waves of a narrow tile's workgroup
+#define FM_ATTN_MOST_STEPS (1 << 30)
 #define FM_ATTN_COLS 16     // columns of a narrow tile: its waves take different keys
 // columns of a wide one, whose queries lie in LDS: fp32 ones as two pieces
 FM_HDC int fm_attn_wide_cols(int bf16) { return bf16 ? 128 : 64; }
@@ -499,6 +500,13 @@ inline int fm_attn_narrow_most(const FmKv *c, const FmAttn *a, const FmSeqs *b, 
     return of_one <= FM_ATTN_MIXED_STEPS ? 0 : FM_ATTN_NARROW_MOST;
 }
 
+// Steps of the narrow launch's tiles if every sequence is max_len long.
+inline int64_t fm_attn_most_steps(const FmKv &c, const FmAttn &a, const FmSeqs &b) {
+    int64_t most = 0;
+    for (int s = 0; s < b.n_seq; s++)
+        most += (int64_t)c.kv_heads * fm_attn_tiles(fm_seq_rows(b, s), a.group, 0, a.narrow_most) * ((a.max_len + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS + 1);
+    return most;
+}
 // Attention: the workgroups that fit on the chip share the steps, fewer if there cannot be as many.  Sets
 // n_tiles (0: no sequence for this launch), groups and splits; returns the workspace: of narrow tiles two parts
 // per workgroup and the steps before each sequence, of wide ones the parts of split tiles.
@@ -509,12 +517,7 @@ inline size_t fm_attn_plan(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int
     a->narrow_most = fm_attn_narrow_most(c, a, b, n_cu);
     a->n_tiles = 0;
     a->splits = 1;
-    int64_t most = 0;
-    for (int s = 0; s < b->n_seq; s++) {
-        const int tiles = fm_attn_tiles(fm_seq_rows(*b, s), a->group, wide, a->narrow_most);
-        if (tiles > a->n_tiles) a->n_tiles = tiles;
-        most += (int64_t)c->kv_heads * tiles * ((a->max_len + FM_ATTN_KEYS - 1) / FM_ATTN_KEYS + 1);
-    }
+    for (int s = 0; s < b->n_seq; s++) a->n_tiles = std::max(a->n_tiles, fm_attn_tiles(fm_seq_rows(*b, s), a->group, wide, a->narrow_most));
     if (!a->n_tiles) return 0;
     if (wide) {
         FmWide w;
@@ -524,7 +527,7 @@ inline size_t fm_attn_plan(const FmKv *c, FmAttn *a, const FmSeqs *b, int D, int
         a->groups = (int)(tiles * a->splits < n_cu ? tiles * a->splits : n_cu);
         return a->splits == 1 ? 0 : (size_t)tiles * a->splits * wide * (D + 2) * sizeof(float);
     }
-    const int64_t groups = (most + FM_ATTN_WAVES - 1) / FM_ATTN_WAVES, fit = fm_attn_per_cu(D) * n_cu;
+    const int64_t groups = (fm_attn_most_steps(*c, *a, *b) + FM_ATTN_WAVES - 1) / FM_ATTN_WAVES, fit = fm_attn_per_cu(D) * n_cu;
     a->groups = (int)(groups < 1 ? 1 : groups > fit ? fit : groups);
     return (size_t)2 * a->groups * fm_attn_cols(wide) * (D + 2) * sizeof(float) + (FM_MAX_SEQ + 1) * sizeof(int);
 }
@@ -555,6 +558,10 @@ inline int fm_attn_check(FmWhy *w, const fm_attn_args *p, int n_cu, FmKv *k, FmA
     const size_t wide = fm_attn_plan(k, &other, b, p->cache.head_dim, n_cu, a->wide_cols);
     *ws = fm_attn_plan(k, a, b, p->cache.head_dim, n_cu, 0);
     if (wide > *ws) *ws = wide;
+    // (the device numbers the steps it finds in 32 bits)
+    const int64_t most = fm_attn_most_steps(*k, *a, *b);
+    if (most > FM_ATTN_MOST_STEPS)
+        return fm_why(w, FM_ERR_ARG, "%lld steps of %d keys at max_len, at most %d", (long long)most, FM_ATTN_KEYS, FM_ATTN_MOST_STEPS);
     return FM_OK;
 }
 

@@ -456,7 +456,9 @@ FM_API int fm_kv_read_dev(fm_ctx *ctx, const fm_kv_args *args);
  * h / (q_heads / kv_heads).  out [rows][q_heads][head_dim] contiguous =
  * sum softmax(scale * q.k) v; a row that sees nothing (d_len 0, pages that are not there) is
  * zeros.  max_len: upper bound of d_len; keys from it on are not seen.  The size of the
- * launch goes by it, so a captured graph takes the largest length it will be replayed at. */
+ * launch goes by it, so a captured graph takes the largest length it will be replayed at.  Sequences, cache heads and
+ * max_len whose single rows would take 2^30 steps of 64 keys and more (256 sequences of 8 heads over 32 million
+ * tokens) are FM_ERR_ARG. */
 typedef struct {
     fm_kv_cache cache;
     int32_t n_seq, q_heads, dtype;
