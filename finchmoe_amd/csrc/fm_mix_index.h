@@ -84,26 +84,26 @@ FM_HD FmGdnWs fm_gdn_ws(const FmGdn &a) {
     w.floats = w.end + (a.v_heads + 63) / 64 * 64;
     return w;
 }
-// Chunks of one pass over the sequences: as many of each as keep the workspace near 192 MB, where
-// the last-level cache still holds it between the two kernels.
-inline int fm_gdn_window(const FmGdn &a, int n_seq) {
-    const int64_t per = fm_gdn_ws(a).floats * 4;
-    const int64_t n = ((int64_t)192 << 20) / per / (n_seq < 1 ? 1 : n_seq);
-    return n < 1 ? 1 : n > 1024 ? 1024 : (int)n;
+// Chunks of one launch of the chunked form: the workspace stays within 192 MB, where the last-level cache
+// still holds it between the two kernels.
+inline int fm_gdn_budget(const FmGdn &a) {
+    const int64_t n = ((int64_t)192 << 20) / (fm_gdn_ws(a).floats * 4);
+    return n < 1 ? 1 : n > (1 << 20) ? 1 << 20 : (int)n;
 }
-// The launches of a call, in order: plan(i, &seqs) fills the i-th, false when there are no more.  The first
-// are those of the short sequences.
+// The launches of a call, in order: next(&seqs, &chunked) fills one, false when there are no more.  The first
+// are those of the short sequences.  One of the long ones takes the first of them that have not ended, as many as a launch
+// has room for, and of each the chunks left or, if that is too many, the same number: the largest that fits.
 struct FmGdnPlan {
     const FmGdn *a;
     const int *start;
     int n_seq;
     const float *const *in;
     float *const *out;
-    int at = 0;          // next sequence to look at
-    int pass = 0;        // 0: short sequences, 1: chunked
-    int done = 0;        // chunks of the group in hand that have run
-    int group0 = 0;      // its first sequence
+    int at = 0;                     // next sequence to look at
+    int pass = 0;                   // 0: short sequences, 1: chunked
+    int done[FM_MAX_SEQ] = {};      // chunks of a long sequence that have run
     int rows(int i) const { return start ? start[i + 1] - start[i] : 1; }
+    int left(int i) const { return rows(i) < FM_GDN_MIN_CHUNKED ? 0 : (rows(i) + FM_GDN_CHUNK - 1) / FM_GDN_CHUNK - done[i]; }
     bool next(FmGdnSeqs *b, int *chunked) {
         b->n = 0;
         if (pass == 0) {
@@ -115,29 +115,43 @@ struct FmGdnPlan {
             at = 0;
         }
         *chunked = 1;
-        for (;;) {
-            // a group: up to FM_GDN_SEQS long sequences, run window by window
-            int n_long = 0, most = 0, end = group0;
-            for (; end < n_seq && n_long < FM_GDN_SEQS; end++) {
-                n_long += rows(end) >= FM_GDN_MIN_CHUNKED;
-                most = rows(end) > most ? rows(end) : most;
+        const int budget = fm_gdn_budget(*a);
+        while (at < n_seq && !left(at)) at++;
+        int seqs[FM_GDN_SEQS], n = 0, most = 0, least = 0, all = 0;
+        bool whole = true;                 // these are all that are left
+        for (int i = at; i < n_seq; i++) {
+            const int c = left(i);
+            if (!c) continue;
+            if (n == FM_GDN_SEQS || n == budget) {
+                whole = false;
+                break;
             }
-            if (!n_long) return false;
-            // windows of one size rather than a short last one
-            const int chunks = (most + FM_GDN_CHUNK - 1) / FM_GDN_CHUNK, full = fm_gdn_window(*a, n_long);
-            const int passes = (chunks + full - 1) / full, win = (chunks + passes - 1) / passes * FM_GDN_CHUNK;
-            b->n = 0;
-            for (int i = group0; i < end; i++) {
-                const int left = rows(i) - done;
-                if (rows(i) >= FM_GDN_MIN_CHUNKED && left > 0) put(b, i, done, left < win ? left : win, done == 0);
-            }
-            if (b->n) {
-                done += win;
-                return true;
-            }
-            group0 = end;
-            done = 0;
+            seqs[n++] = i;
+            all += c;
+            most = std::max(most, c);
+            least = n == 1 ? c : std::min(least, c);
         }
+        if (!n) return false;
+        int win = 1, over = most + 1;      // win fits, `over` does not or is not needed
+        while (over - win > 1) {
+            const int mid = (win + over) / 2;
+            int64_t sum = 0;
+            for (int k = 0; k < n; k++) sum += std::min(left(seqs[k]), mid);
+            (sum <= budget ? win : over) = mid;
+        }
+        // Launches of one size rather than a short last one, where that makes no more of them: to the end of all that
+        // are left, or to that of the shortest in hand.
+        const int to = whole && (most + win - 1) / win == (all + budget - 1) / budget ? most : least;
+        if (to > win) {
+            const int passes = (to + win - 1) / win;
+            win = (to + passes - 1) / passes;
+        }
+        for (int k = 0; k < n; k++) {
+            const int i = seqs[k], first = done[i] * FM_GDN_CHUNK, c = std::min(left(i), win);
+            put(b, i, first, std::min(rows(i) - first, c * FM_GDN_CHUNK), done[i] == 0);
+            done[i] += c;
+        }
+        return true;
     }
     void put(FmGdnSeqs *b, int i, int first, int n, bool fresh) {
         const int k = b->n++;

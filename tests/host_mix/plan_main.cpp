@@ -70,9 +70,77 @@ static void count_steps() {
     CHECK(refused > 20 && taken > 2000);
 }
 
+// ---- the gated delta rule: long sequences' chunks run in launches that fill a workspace of 192 MB, however the
+// lengths differ, and none takes more
+struct Launches {
+    int n = 0;
+    size_t most = 0;      // bytes of the largest
+};
+static Launches run_gdn(const FmGdn &a, const std::vector<int> &rows) {
+    const int n = (int)rows.size();
+    std::vector<int> start(n + 1, 0), next(n, 0);
+    std::vector<float *> in(n), out(n);
+    for (int i = 0; i < n; i++) {
+        start[i + 1] = start[i] + rows[i];
+        in[i] = (float *)at(4096 + 64 * i), out[i] = (float *)at(1 << 20 | 64 * i);
+    }
+    FmGdnPlan plan{&a, start.data(), n, in.data(), out.data()};
+    FmGdnSeqs b;
+    int chunked;
+    Launches all;
+    while (plan.next(&b, &chunked)) {
+        CHECK(b.n >= 1 && b.n <= FM_GDN_SEQS);
+        for (int k = 0; k < b.n; k++) {
+            const int i = (int)(((uintptr_t)b.out[k] & ((1 << 20) - 1)) / 64);
+            CHECK(b.row[k] == start[i] + next[i] && b.in[k] == (next[i] ? out[i] : in[i]) && b.row[k] + b.rows[k] <= start[i + 1]);
+            CHECK(!chunked || b.rows[k] % FM_GDN_CHUNK == 0 || b.row[k] + b.rows[k] == start[i + 1]);
+            next[i] += b.rows[k];
+        }
+        if (!chunked) continue;
+        all.n++;
+        all.most = std::max(all.most, (size_t)b.chunk0[b.n] * fm_gdn_ws(a).floats * 4);
+    }
+    for (int i = 0; i < n; i++) CHECK(next[i] == rows[i]);
+    CHECK(all.most == fm_gdn_ws_bytes(&a, start.data(), n));
+    return all;
+}
+static void windows() {
+    FmGdn a{};
+    a.k_heads = 16, a.v_heads = 32, a.k_dim = a.v_dim = 128;
+    CHECK(run_gdn(a, {8192}).n == 2);
+    // a long prompt beside short ones
+    for (int others : {1, 7, 31, 100}) {
+        std::vector<int> rows(1, 8192);
+        rows.insert(rows.end(), others, others == 100 ? 24 : 64);
+        CHECK(run_gdn(a, rows).n <= 3);
+        std::reverse(rows.begin(), rows.end());
+        CHECK(run_gdn(a, rows).n <= 3);
+    }
+    const size_t full = (size_t)192 << 20;
+    a.k_heads = a.v_heads = 256, a.v_dim = 256;
+    CHECK(run_gdn(a, std::vector<int>(128, 64)).most <= full);
+    for (int round = 0; round < 3000; round++) {
+        a.k_heads = 1 + rnd(rnd(2) ? 16 : 256), a.v_heads = std::min(256 / a.k_heads, 1 + rnd(3)) * a.k_heads, a.k_dim = rnd(2) ? 64 : 128, a.v_dim = 128;
+        std::vector<int> rows(1 + rnd(rnd(3) ? 8 : FM_MAX_SEQ));
+        int left = FM_MAX_ROWS;
+        int64_t chunks = 0, many = 0;
+        for (int &r : rows) {
+            r = std::min(left, rnd(3) ? rnd(200) : rnd(rnd(2) ? 3000 : 20000));
+            left -= r;
+            if (r >= FM_GDN_MIN_CHUNKED) chunks += (r + FM_GDN_CHUNK - 1) / FM_GDN_CHUNK, many++;
+        }
+        const int64_t budget = (int64_t)full / (fm_gdn_ws(a).floats * 4);
+        const Launches got = run_gdn(a, rows);
+        CHECK(got.most <= full);
+        // (a launch that ends no sequence fills more than half of the budget, or has FM_GDN_SEQS of them)
+        CHECK(got.n <= 1 + 2 * (chunks + budget - 1) / budget + many / FM_GDN_SEQS * 2);
+    }
+}
+
 int main(int argc, char **argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     if (what == "steps") count_steps();
+    else if (what == "windows") windows();
     else bad = 1;
     if (!bad) printf("plans hold\n");
     return bad ? 1 : 0;

@@ -231,3 +231,19 @@ def test_refusals(hip):
     assert status(d_state_in=[p + 65536 + 16]) == fb.ERR_ARG
     hip.gated_delta_dev(hip.gated_delta_args(**good))
     hip.sync()
+
+
+@pytest.mark.parametrize("dtype", ["float32", "bfloat16"])
+@pytest.mark.parametrize("lens", [[9000] + [64] * 7 + [3], [64] * 6 + [9000, 7] + [24] * 30, [100] * 140], ids=["ahead", "between", "140 alike"])
+def test_long_and_short_sequences_of_one_batch(hip, lens, dtype):
+    """how many launches a long prompt takes is its own affair: every sequence comes out as in a call of its own"""
+    import torch
+    hk, hv, dk, dv = 8, 16, 64, 32
+    rows, gate, beta, state = _inputs(17, lens, hk, hv, dk, dv, getattr(torch, dtype))
+    got, new = _call(hip, rows, gate, beta, state, lens, hk, hv, dk, dv, True, 0.125)
+    again, last = _call(hip, rows, gate, beta, state, lens, hk, hv, dk, dv, True, 0.125, in_place=True)
+    assert torch.equal(got, again) and torch.equal(new, last)
+    at = R.starts(lens)
+    for i in sorted({0, 1, 5, 6, 7, len(lens) - 1}):
+        one, st = _call(hip, rows[at[i]:at[i + 1]], gate[at[i]:at[i + 1]], beta[at[i]:at[i + 1]], state[i:i + 1], lens[i:i + 1], hk, hv, dk, dv, True, 0.125)
+        assert torch.equal(got[at[i]:at[i + 1]], one) and torch.equal(new[i:i + 1], st), i
