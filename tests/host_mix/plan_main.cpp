@@ -70,6 +70,46 @@ static void count_steps() {
     CHECK(refused > 20 && taken > 2000);
 }
 
+// ---- attention: every column of every sequence with rows is in one tile of one of the two launches
+static void columns() {
+    int both = 0, only_wide = 0, only_narrow = 0;
+    for (int round = 0; round < 4000; round++) {
+        FmKv c{};
+        c.kv_heads = 1 + rnd(8), c.max_pages = 1 + rnd(rnd(2) ? 20 : 600), c.page_tokens = 16 << rnd(4);
+        FmAttn a{};
+        a.group = 1 + rnd(rnd(2) ? 4 : 16), a.q_heads = a.group * c.kv_heads, a.wide_cols = fm_attn_wide_cols(rnd(2));
+        a.max_len = rnd(3) ? c.max_pages * c.page_tokens : rnd(300);
+        FmSeqs b{};
+        b.n_seq = 1 + rnd(rnd(2) ? 5 : 40), b.one_row = !rnd(5);
+        for (int i = 0; i < b.n_seq; i++) b.start[i + 1] = b.start[i] + (rnd(2) ? rnd(3) : rnd(600));
+        FmAttn narrow = a, wide = a;
+        fm_attn_plan(&c, &narrow, &b, 128, 256, 0);
+        fm_attn_plan(&c, &wide, &b, 128, 256, a.wide_cols);
+        CHECK(narrow.narrow_most == wide.narrow_most);
+        both += narrow.n_tiles && wide.n_tiles, only_wide += !narrow.n_tiles && wide.n_tiles, only_narrow += narrow.n_tiles && !wide.n_tiles;
+        FmWide w;
+        fm_attn_wide_tiles(b, a.group, a.wide_cols, wide.narrow_most, &w);
+        std::vector<std::vector<int>> seen(b.n_seq * c.kv_heads);
+        for (int s = 0; s < b.n_seq; s++)
+            for (int h = 0; h < c.kv_heads; h++) seen[s * c.kv_heads + h].assign(fm_seq_rows(b, s) * a.group, 0);
+        auto mark = [&](int s, int h, int tile, int width) {
+            auto &v = seen[s * c.kv_heads + h];
+            CHECK(tile * width < (int)v.size());
+            for (int k = tile * width; k < (tile + 1) * width && k < (int)v.size(); k++) v[k]++;
+        };
+        for (int s = 0; s < b.n_seq && narrow.n_tiles; s++)
+            for (int h = 0; h < c.kv_heads; h++)
+                for (int t = 0; t < fm_attn_tiles(fm_seq_rows(b, s), a.group, 0, narrow.narrow_most); t++) mark(s, h, t, FM_ATTN_COLS);
+        for (int u = 0; wide.n_tiles && u < w.first[b.n_seq] * c.kv_heads; u++) {
+            const FmWideUnit at = fm_attn_wide_unit(w, b.n_seq, c.kv_heads, 1, u);
+            mark(at.s, at.h, at.tile, a.wide_cols);
+        }
+        for (auto &v : seen)
+            for (int n : v) CHECK(n == 1);
+    }
+    CHECK(both > 100 && only_wide > 100 && only_narrow > 100);
+}
+
 // ---- the gated delta rule: long sequences' chunks run in launches that fill a workspace of 192 MB, however the
 // lengths differ, and none takes more
 struct Launches {
@@ -140,6 +180,7 @@ static void windows() {
 int main(int argc, char **argv) {
     const std::string what = argc > 1 ? argv[1] : "";
     if (what == "steps") count_steps();
+    else if (what == "columns") columns();
     else if (what == "windows") windows();
     else bad = 1;
     if (!bad) printf("plans hold\n");

@@ -8,7 +8,7 @@ import pytest
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
 
-@pytest.mark.parametrize("what", ["steps", "windows"])
+@pytest.mark.parametrize("what", ["steps", "columns", "windows"])
 def test_plans(tmp_path, what):
     exe = str(tmp_path / "plan")
     subprocess.check_call(["g++", "-std=c++17", "-O1", "-g", "-fsanitize=address,undefined",
