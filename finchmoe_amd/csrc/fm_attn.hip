@@ -346,7 +346,7 @@ __device__ __forceinline__ void add_steps(const FmKv &c, const FmAttn &a, const 
 // Narrow tiles: a workgroup takes its share of the steps, tile by tile; the four waves take a tile's steps
 // in turn and are joined through LDS.
 // Bound by the codes' way from memory: 32 sequences of 8300 tokens on average, 2 cache heads of 256 in bf16, 272 MB
-// in 65 us, 4.2 TB/s; one sequence of 999 by latency, 12 us (lengths, table, codes, join wait for each other) and
+// in 68 us, 4.0 TB/s; one sequence of 999 by latency, 12.5 us (lengths, table, codes, join wait for each other) and
 // 4 us for the join of the parts.
 template <int D, bool BF16, bool ONCE>
 __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c, FmAttn a, FmSeqs b) {
@@ -463,9 +463,10 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c,
 // SIMD, so that one's softmax runs beside the other's products, in 256 registers each.
 // The codes of the next step are on their way in registers meanwhile; keys are replaced behind the first
 // product's barrier, values behind the second's, so a step has two barriers and one copy of each.
-// 2048 rows over 8192 keys, 16 heads of 256, bf16: 241 GFLOP in 398 us, 606 TFLOP/s (a large library product 1050);
-// with one piece of p and a power of two that goes by the value scales alone 326 us.  A step of 128 columns x 64 keys x 256 dims has products for 3072 cycles a SIMD (1024 of
-// the scores, 2048 of the two pieces).
+// 2048 rows over 8192 keys, 16 heads of 256, bf16: 241 GFLOP in 403 us, 598 TFLOP/s (a large library product 1050);
+// with one piece of p and a power of two that goes by the value scales alone 326 us.  A step of 128 columns x 64 keys x
+// 256 dims has products for 3072 cycles a SIMD (1024 of the scores, 2048 of the two pieces), 41 % of its time; the vector
+// ALU is busy for 61 %, with two waves per SIMD and two barriers.  Heads of 256 in bf16 spill 2 registers.
 template <int D, bool BF16>
 __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs b, FmWide w) {
     constexpr int NP = BF16 ? 1 : 2, CT = BF16 ? 2 : 1, KS = D / 32, DT = D / 16, LD = D / 64, WIDE = 64 * CT;
@@ -859,7 +860,7 @@ __global__ __launch_bounds__(KV_T) void fm_kv_append(FmKv c, FmKvRows x, int D, 
     __syncthreads();                                             // (everybody has read the old scale, too)
 #pragma unroll
     for (int i = 0; i < KV_T / 64; i++) big = fmaxf(big, red[i]);
-    const float scale = fmaxf(old, big * (1.0f / 127.0f));
+    const float scale = fmaxf(old, big * (1.0f / 127.0f));      // (the scale is this product, not the quotient: up to an ulp apart)
     if (tid == 0) *scale_at = scale;
     int8_t *codes = value ? c.v + fm_kv_v_at(c, D, page, h, 0, 0) : c.k + fm_kv_k_at(c, D, page, h, 0, 0);
     if (t0 > 0 && scale != old) {                               // the old codes go to the new scale

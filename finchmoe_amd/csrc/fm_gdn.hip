@@ -20,8 +20,9 @@
 // Everything that does not need the state — the inverse T of 1 + A, P = scale tril(E . Q K^T) and the
 // factors of a token — is computed for all chunks at once by fm_gdn_prep; fm_gdn_scan walks the chunks in
 // order, sixteen state rows (value dims) a workgroup, with five small products a chunk.  Both use
-// the fp32 matrix instruction v_mfma_f32_16x16x4_f32: the state is an fp32 result, which 16-bit
-// operands would have to be split in three pieces (six products) to keep.
+// the fp32 matrix instruction v_mfma_f32_16x16x4_f32, eight of them (256 cycles) for 16 x 16 x 32, and operands as they
+// are.  (Three bf16 pieces hold an fp32 number: six products of 16 cycles for fp32 K and Q, three for bf16 ones, which need
+// no pieces.  That form has not been built.)
 // G is summed in fp64: E_ij is a difference of sums that may be hundreds while it is small itself.
 #include "fm_mix.h"
 
@@ -133,8 +134,9 @@ __device__ __forceinline__ float exp2_of(float x) { return __builtin_amdgcn_exp2
 //   T_ij = -T_ii sum_{j <= m < i} A_im T_mj,
 // where a product's result registers are the next one's right operand as they are (lane 16 g + c has
 // rows 4 g .. 4 g + 3 of column c in both), so a block column never leaves its wave's registers.
-// Bound by what it reads and writes: 64 chunks of 16 / 32 heads of 128, 180 MB in 50 us, 3.6 TB/s; a few chunks
-// by their chain of phases, 12 us.
+// 64 chunks of 16 / 32 heads of 128 read and write 180 MB in 50 us, 3.6 TB/s; no unit is busy for more than 29 %, the
+// waves of the two workgroups a CU has room for (70 KB of LDS each) wait for 36 %: bound by the phases between the
+// barriers, as a few chunks are, 12 us.
 template <int DK, bool BF16>
 __global__ __launch_bounds__(256) void fm_gdn_prep(FmGdn a, FmGdnSeqs b, float *ws) {
     constexpr int LD = DK + 4, LA = 68;      // rows 4 banks apart: 16 lanes' 16-byte reads do not collide

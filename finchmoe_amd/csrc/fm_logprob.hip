@@ -4,7 +4,9 @@
 // A row is cut into segments, one workgroup each, E elements a thread in registers.  With d_i = x_i - m,
 // m the row's maximum and the (first) maximum's own term e^0 = 1 kept apart,
 //   Z' = sum over the others of e^d,  log p_i = d_i - log1p(Z'),  H = log1p(Z') - sum e^d d / (1 + Z')
-// so that neither loses its digits when one token holds nearly all the probability.  A segment
+// so that neither loses its digits when one token holds nearly all the probability.  (e^d is the instruction's 2^x of
+// d log2 e in fp32: with half of the probability 10 to 20 below the maximum the mean error of log p is 1.7e-8 at 0.69,
+// a quarter of a step, and that of the entropy 7.9e-8 at 6.2, a sixth.)  A segment
 // gives (m, Z', sum e^d d) for its own maximum, and its top_n largest elements.
 //
 // Order: an element's key is its value, made an unsigned number of the same order, above the complement
@@ -134,7 +136,8 @@ __device__ __forceinline__ void block_top(Key key, Reaches reaches, uint32_t big
 }
 
 // V4: rows are 16-byte aligned, a thread takes four elements side by side
-// (Five waves a SIMD: 257 rows 53 us; the 99 registers the compiler would take leave four, 57 us, and six spill, 55 us.)
+// (Five waves a SIMD: 257 rows 53 us, 14 registers spilled with E 32; the 99 the compiler would take leave four, 57 us, and
+// for six more are spilled, 55 us.)
 template <int E, bool V4>
 __global__ __launch_bounds__(LP_T, 5) void fm_logprob_seg(const float *x, int vocab, int64_t stride, int n_seg, int top_n,
                                                        Part *parts, LpKey *tops) {

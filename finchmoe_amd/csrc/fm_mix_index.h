@@ -213,11 +213,11 @@ FM_HDC int fm_attn_wide_cols(int bf16) { return bf16 ? 128 : 64; }
 // Which sequences have wide tiles: those of more than 48 columns, in a batch of 1024 columns over all its
 // sequences and cache heads.  Narrow tiles read the keys once per 16 columns but spread over the whole
 // chip; measured (narrow / wide, us; 2 cache heads of 256): one sequence over 4000 keys 256 columns
-// 33 / 33 (fp32) and 31 / 37 (bf16), 512 columns 43 / 33 and 41 / 38, 1024 columns 67 / 39 and 64 / 39;
-// 16 sequences over 3000 keys 32 columns 36 / 32 and 34 / 38, 64 columns 49 / 35 and 46 / 39.
+// 33 / 34 (fp32) and 32 / 39 (bf16), 512 columns 44 / 34 and 43 / 40, 1024 columns 68 / 41 and 67 / 42;
+// 16 sequences over 3000 keys 32 columns 37 / 32 and 36 / 41, 64 columns 50 / 35 and 49 / 43.
 // Beside wide ones the narrow tiles' two launches cost more than wide tiles for all where those are short: one
 // sequence of 300 rows and single rows, 2 cache heads of 256 (wide for all / separate, us; by the steps a workgroup then has):
-// bf16 4 steps 29 / 44, 8 42 / 48, 11 50 / 55 and 53 / 64, 21 78 / 74, 32 102 / 70; fp32 16 45 / 46, 21 65 / 52.
+// bf16 3 steps 32 / 46, 8 46 / 50 and 48 / 55, 11 56 / 57, 42 161 / 74; fp32 11 42 / 44, 16 54 / 51, 21 67 / 53.
 #define FM_ATTN_NARROW_MOST 48
 #define FM_ATTN_WIDE_LEAST 1024
 #define FM_ATTN_MIXED_STEPS 12
@@ -267,8 +267,8 @@ FM_HD int fm_kv_page(const FmKv &c, int s, int pos) {
     return p >= 0 && p < c.n_pages ? p : -1;
 }
 // byte offset of a code: keys [page][head][token][dim], values [page][head][dim][token]
-// (A shift for the values' page size: 2048 rows over 8192 keys 329 us, 335 with a 64-bit product.  With one for the
-// keys', too, narrow tiles come out slower, one row 17.2 us instead of 16.3.)
+// (A shift for the values' page size: 2048 rows over 8192 keys 403 us in bf16, 410 with a 64-bit product.  One for the
+// keys' makes that 406, and 513 of 526 us in fp32; single rows take the same time.)
 FM_HD int64_t fm_kv_k_at(const FmKv &c, int D, int page, int head, int pos, int dim) {
     return (((int64_t)page * c.kv_heads + head) * c.page_tokens + (pos & (c.page_tokens - 1))) * D + dim;
 }
@@ -496,8 +496,8 @@ inline int fm_attn_splits(int64_t tiles, int groups, int most_steps) {
 }
 
 // Workgroups of a CU.  Narrow tiles: heads of 256 take a wave more registers than half a SIMD has (and a
-// spilled one would wait for the codes in flight); heads of 128 gain by a second one where few tiles are
-// long (one bf16 row over 30000 keys 38.7 us with two, 48.8 with one; 32 rows over 8000 keys 36.8 / 35.9).
+// spilled one would wait for the codes in flight); heads of 128 have room for a second one (one bf16 row over
+// 30000 keys 38.1 us with two, 38.6 with one; 32 rows over 8000 keys 38.1 / 37.2).
 FM_HDC int fm_attn_per_cu(int D) { return D == 256 ? 1 : 2; }
 // Columns of a sequence up to which it has narrow tiles: none where with wide tiles for all a workgroup would have
 // FM_ATTN_MIXED_STEPS steps at most.

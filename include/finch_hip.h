@@ -374,7 +374,7 @@ FM_API int fm_embed_lookup(fm_ctx *ctx, fm_tensor t, int token_id, float *out);
  * What stands between the quantized products of a token: the gated delta rule that the
  * GatedDeltaNet projections feed, and attention over a cache held in 8 bits.  Vectors are fp32,
  * or bfloat16 bits where dtype says so; sums, statistics and states are fp32 in either case, and
- * attention's weights keep 22 bits of the largest weight times value scale.
+ * attention's weights keep 22 bits, down to 2^-38 of a row's largest weight times value scale.
  * Rows (tokens) of several sequences lie one behind the other; seq_start names where each begins:
  * n_seq + 1 ascending row numbers in HOST memory, the first of them 0 (a sequence may be empty).
  * seq_start == NULL: one row per sequence.  It is read during the call only; the launch carries
@@ -433,10 +433,11 @@ typedef struct {
 
 /* fm_kv_append_dev: rows k, v [rows][kv_heads][head_dim] become the last tokens of their
  * sequences (positions d_len - rows of the sequence .. d_len - 1).  A page's scale is the largest finite
- * magnitude in it times the fp32 number 1/127; a page that already holds tokens keeps its scale unless a new token
- * exceeds it, then the old codes are rounded to the new scale.  code = round to nearest even of value / scale,
- * decided exactly; a NaN becomes 0, an infinity +-127.  The same rows appended again change nothing.
- * A page that two sequences of the call append to is not defined.
+ * magnitude in it times the fp32 number 1/127, rounded to fp32 (this is the definition: the rounded quotient by 127 may be
+ * the next number, and values half-way between two codes then have the other one); a page that already holds tokens keeps
+ * its scale unless a new token exceeds it, then the old codes are rounded to the new scale.  code = round to nearest even
+ * of value / scale, decided exactly; a NaN becomes 0, an infinity +-127.  The same rows appended again change nothing.
+ * What a page holds that two sequences of the call, or two places of one sequence's table, append to is not defined.
  * fm_kv_read_dev: the last rows of each sequence back as fp32 (dtype must be FM_DTYPE_F32);
  * positions below 0 read as zeros. */
 typedef struct {

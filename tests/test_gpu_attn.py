@@ -1,7 +1,7 @@
 """The 8-bit paged cache and its attention (fm_kv_append_dev, fm_kv_read_dev, fm_attn_dev) against
 64-bit forms.
 
-What the cache holds is compared exactly: codes are rounded quotients, scales one fp32 division.
+What the cache holds is compared exactly: codes are rounded quotients, scales one fp32 product with 1/127.
 
 Tolerance of attention.  With A the largest scale * sum |q_i k_i| of a visible pair and V the
 largest |v|: fp32 queries keep 22 bits of a row's largest element and the sums over head_dim round

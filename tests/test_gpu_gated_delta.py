@@ -184,7 +184,7 @@ def test_many_sequences_in_several_launches(hip):
 
 
 def test_windows_of_chunks(hip):
-    """more chunks than one pass over the workspace holds: 40 sequences of 32 heads, three chunks each a pass"""
+    """more chunks than one launch's workspace holds: 40 sequences of 32 heads, up to five chunks each"""
     import torch
     hk, hv, dk, dv = 16, 32, 128, 16
     lens = [100 + 5 * i for i in range(38)] + [7, 64]
