@@ -424,9 +424,10 @@ __global__ __launch_bounds__(256, fm_attn_per_cu(D)) void fm_attn_narrow(FmKv c,
             l = fmaf(s_l[v][col], fast_exp2(s_m[v][col] - base), l);
             ref = max(ref, ref_falls(s_ref[v][col], s_m[v][col], base));
         }
-        // (a part of a tile is normalised as well: its output is a mean of values)
+        // (a part of a tile is normalised as well: its output is a mean of values; the power of two before the sum, or a
+        // small weight of large values would fall below fp32 in between)
         const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
-        const float f = ldexpf(fast_exp2(w.m - base) * inv, w.ref - ref);
+        const float f = ldexpf(fast_exp2(w.m - base), w.ref - ref) * inv;
 #pragma unroll
         for (int d = 0; d < DT; d++) w.o[d] *= f;
         if (wave) {
@@ -709,7 +710,7 @@ __global__ __launch_bounds__(512, 2) void fm_attn_wide(FmKv c, FmAttn a, FmSeqs 
             const float sum = e1 * l[ct] + e2 * s_l[cg][ct][r];
             // (a part of a tile is normalised as well: its output is a mean of values)
             const float inv = sum > 0.0f || sum != sum ? 1.0f / sum : 0.0f;
-            const float f1 = ldexpf(e1 * inv, ref[ct] - top), f2 = ldexpf(e2 * inv, ref2 - top);
+            const float f1 = ldexpf(e1, ref[ct] - top) * inv, f2 = ldexpf(e2, ref2 - top) * inv;
             const int64_t part = (int64_t)unit * WIDE + (cg * CT + ct) * 16 + r;
 #pragma unroll
             for (int d = 0; d < DT; d++) {

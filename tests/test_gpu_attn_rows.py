@@ -149,3 +149,33 @@ def test_equal_scores_of_any_size(hip, score, rows, dtype):
     mean, _ = A.attention(q, size, table, lens, rows, 0.0, max(lens))
     got = Dev(hip, cache, table, lens).attn(q, rows, score, max(lens))
     A.check(got, ref, mean * (max(lens) / 32 + 48) * R.U24, q.dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows", [[1], [1] * 9, [600]], ids=str)
+@pytest.mark.parametrize("page,lead", [(64, (1, -1, 1)), (64, (-1, 1, -1, 1, 1)), (128, (-1, 1, -1)), (16, (1, -1))])
+def test_small_weights_of_large_values_are_joined(hip, page, lead, rows, dtype):
+    """whole steps of keys 2^-121 the weight of the others, with values 2^121 their size: what one wave, half or part has
+    counts as much as what another has.  Bound: one product a score, exact but for the scales' (three half steps), the
+    difference and its shift (three more), twice; weights and sums as everywhere"""
+    import math
+    import torch
+    d = 64
+    lens = [max(rows[0], 64 * 5)] * len(rows)
+    n_pages = sum(-(-n // page) for n in lens) + 1
+    cache, table = _cache(120, n_pages, 2, page, d), _table(121, lens, page, n_pages)
+    cache[0].zero_()
+    cache[2].fill_(1.0 / 127)
+    for s in range(len(lens)):
+        for at in range(-(-lens[s] // page)):
+            p = int(table[s, at])
+            cache[0][p, :, :, 0] = 127 * lead[at % len(lead)]
+            cache[3][p] = (1.0 + 0.1 * (at % 7)) * (2.0 ** 119 if lead[at % len(lead)] < 0 else 0.25)
+    q = torch.randn(sum(rows), 4, d, generator=torch.Generator().manual_seed(122))
+    q[..., 0] = 1.0
+    q = q.to(getattr(torch, dtype))
+    ref, _ = A.attention(q, cache, table, lens, rows, 42.0, max(lens))
+    size = tuple(t.abs() if i in (1, 3) else t for i, t in enumerate(cache[:4])) + (page,)
+    of_size, _ = A.attention(q, size, table, lens, rows, 42.0, max(lens))
+    got = Dev(hip, cache, table, lens).attn(q, rows, 42.0, max(lens))
+    A.check(got, ref, of_size * (math.expm1(2 * 6 * 42 * R.U24) + (max(lens) / 32 + 48) * R.U24), q.dtype)
