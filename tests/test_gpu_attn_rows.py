@@ -179,3 +179,17 @@ def test_small_weights_of_large_values_are_joined(hip, page, lead, rows, dtype):
     of_size, _ = A.attention(q, size, table, lens, rows, 42.0, max(lens))
     got = Dev(hip, cache, table, lens).attn(q, rows, 42.0, max(lens))
     A.check(got, ref, of_size * (math.expm1(2 * 6 * 42 * R.U24) + (max(lens) / 32 + 48) * R.U24), q.dtype)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("lens,rows", [([20011], [1]), ([40000, 3], [3, 1])], ids=["20011", "40000 and 3"])
+def test_more_parts_than_a_wave_has_lanes(hip, lens, rows, dtype):
+    """a row's keys over 79 and 157 workgroups, values of pages 2^40 apart"""
+    import torch
+    page, d = 128, 64
+    n_pages = sum(-(-n // page) for n in lens) + 1
+    g = torch.Generator().manual_seed(130)
+    cache, table = _cache(131, n_pages, 1, page, d), _table(132, lens, page, n_pages)
+    cache[3].mul_(torch.exp2(torch.randint(-20, 20, cache[3].shape, generator=g).float()))
+    q = (1.5 * torch.randn(sum(rows), 2, d, generator=g)).to(getattr(torch, dtype))
+    _run(hip, cache, table, lens, rows, q, 0.125)
